@@ -308,7 +308,7 @@ def _own_route(s):
     gates = torch.empty(T, k, **f32)
     counts, offsets, order, used = torch.empty(E, **i32), torch.empty(E + 1, **i32), torch.empty(cap, **i32), torch.empty(1, **i32)
     probs, loss = torch.empty(E, **f32), torch.empty(1, **f32)
-    r = G.Route(T, E, k, c["align"], G.DTYPES[c["dtype"]], int(c["renorm"]), COEF, cap, x.data_ptr(), E,
+    r = G.Router(T, E, k, c["align"], G.DTYPES[c["dtype"]], int(c["renorm"]), COEF, cap, x.data_ptr(), E,
                 s["mask"].data_ptr() if s["mask"] is not None else None, ids.data_ptr(), gates.data_ptr(), pos.data_ptr(),
                 counts.data_ptr(), offsets.data_ptr(), order.data_ptr(), used.data_ptr(), probs.data_ptr(), loss.data_ptr())
     n = G.lib().ggemm_route_workspace(T, E, k)

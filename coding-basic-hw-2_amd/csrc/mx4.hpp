@@ -1,0 +1,57 @@
+// mx4.hpp -- what the kernels on microscaled 4-bit operands and the router share: element types, block
+// scales, lane exchanges inside a row of 16 lanes.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "common.hpp"
+#include "ggemm_mx4.h"
+
+namespace ggemm {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// Element types by their number in the ABI.
+template <int D> struct Elem;
+template <> struct Elem<GGEMM_F32> { using T = float; };
+template <> struct Elem<GGEMM_BF16> { using T = __bf16; };
+template <> struct Elem<GGEMM_F16> { using T = _Float16; };
+
+inline int elem_bytes(int dtype) { return dtype == GGEMM_F32 ? 4 : 2; }
+inline bool elem_known(int dtype) { return dtype == GGEMM_F32 || dtype == GGEMM_BF16 || dtype == GGEMM_F16; }
+inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// f(integral_constant<int, D>) for the element type of a call
+template <class F>
+inline void with_elem(int dtype, F&& f) {
+  if (dtype == GGEMM_F32) f(std::integral_constant<int, GGEMM_F32>{});
+  else if (dtype == GGEMM_BF16) f(std::integral_constant<int, GGEMM_BF16>{});
+  else f(std::integral_constant<int, GGEMM_F16>{});
+}
+
+// The scale byte s as a number: 2^(s - 127), exact (s = 0 is the subnormal 2^-127); s < 255.
+__device__ __forceinline__ float mx4_scale(uint32_t s) { return __uint_as_float(s ? s << 23 : 1u << 22); }
+
+// Scale byte of a block whose largest magnitude has the bits `amax` (as a 32-bit float, sign cleared):
+// 255 for NaN and Inf, else clamp(floor(log2 amax) - 2, -127, 127) + 127 = max(exponent field - 2, 0)
+// (zeros and subnormals have field 0, and 252 is the largest result).
+__device__ __forceinline__ uint32_t mx4_scale_byte(uint32_t amax) {
+  const uint32_t e = amax >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+
+// x of another lane of the same row of 16, by a data-parallel-primitive control word
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
+}
+constexpr int kDppXor1 = 0xb1, kDppXor2 = 0x4e;      // quad_perm [1,0,3,2] and [2,3,0,1]
+constexpr int kDppHalfMirror = 0x141, kDppMirror = 0x140;   // lane i <-> 7 - i and 15 - i
+
+}  // namespace ggemm

@@ -1,0 +1,519 @@
+// route.hip -- the router of a mixture-of-experts layer (include/ggemm_route.h).
+//
+// A token's logits lie in L lanes of one wave, V consecutive experts to a lane (L V >= experts, L a power
+// of two, 64 / L tokens a wave), in registers from the load to the last use.  Selection works on
+// 32-bit keys that order like the logits (NaN highest, barred experts 0): per place a maximum over the
+// lane's keys and then over the L lanes, and the lowest lane, then the lowest of its experts, that holds
+// it.  Softmax is the usual exp2((x - max) log2 e) over its sum, the maximum being the first choice.
+// Counting: a workgroup takes `span` consecutive tokens.  One bit per (expert, token) in LDS gives each pair
+// its rank among the workgroup's tokens by counting bits (no atomic whose order matters), and the
+// expert's count.  A second launch turns the workgroups' counts into starting ranks and sums their partial
+// softmax sums in a fixed order; a third one writes rows, order and loss.  A call of one workgroup does
+// all of it in the first launch.
+#include <algorithm>
+#include <type_traits>
+
+#include "mx4.hpp"
+#include "ggemm_route.h"
+
+namespace ggemm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Workspace: per workgroup of the first launch and expert the count (then the starting rank) and the
+// softmax sum, and per workgroup the tokens used.
+struct RouteWs {
+  int* hist;     // groups x experts
+  float* psum;   // groups x experts
+  int* used;     // groups
+};
+
+struct Shape {
+  int span, groups;
+};
+// Tokens a workgroup takes (a multiple of 32: whole words of the bit table).  Few tokens are spread over
+// the compute units, many take longer spans, which makes the tables of the second launch shorter.
+Shape shape_of(int tokens) {
+  const int span = tokens <= 32768 ? 64 : 256;
+  return Shape{span, tokens > 0 ? ceil_div(tokens, span) : 1};
+}
+
+RouteWs carve(void* ws, const Shape& sh, int experts) {
+  char* p = static_cast<char*>(ws);
+  const size_t table = align_up((size_t)sh.groups * experts * 4, 16);
+  return RouteWs{reinterpret_cast<int*>(p), reinterpret_cast<float*>(p + table), reinterpret_cast<int*>(p + 2 * table)};
+}
+
+// A key that orders like x: 0 for -inf, above every other for NaN; x + 0 makes -0 equal to +0.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  x += 0.0f;
+  const uint32_t b = __float_as_uint(x);
+  if (x != x) return 0xffffffffu;
+  if (b == 0xff800000u) return 0u;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return k == 0xffffffffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// Reductions over the L lanes of a token; every lane gets the result.
+template <int L, class T, class F>
+__device__ __forceinline__ T over_lanes(T x, F&& f) {
+#pragma unroll
+  for (int d = 1; d < L; d *= 2) x = f(x, __shfl_xor(x, d));
+  return x;
+}
+template <int L>
+__device__ __forceinline__ float sum_lanes(float x) {
+  return over_lanes<L>(x, [](float a, float b) { return a + b; });
+}
+template <int L>
+__device__ __forceinline__ uint32_t max_lanes(uint32_t x) {
+  return over_lanes<L>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+
+// The lane's V logits of token t (experts lane V ...; -inf past the last expert).
+template <int D, int V>
+__device__ __forceinline__ void load_logits(const ggemm_router_t& r, int t, int e0, float (&x)[V]) {
+  using T = typename Elem<D>::T;
+  const T* p = static_cast<const T*>(r.logits) + (int64_t)t * r.ld + e0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) x[v] = e0 + v < r.experts ? (float)p[v] : -__builtin_inff();
+}
+
+// p[v] = exp(x[v] - max) for a token's lanes, and the reciprocal of the sum.  m: the largest logit.
+template <int L, int V>
+__device__ __forceinline__ float exps(const float (&x)[V], float m, float (&p)[V]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    p[v] = x[v] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((x[v] - m) * kLog2e);
+    sum += p[v];
+  }
+  return 1.0f / sum_lanes<L>(sum);
+}
+
+__device__ __forceinline__ bool masked(const ggemm_router_t& r, int t) { return r.mask && r.mask[t] == 0; }
+
+// Rows of order that belong to no pair: expert e's padding, and what follows the last expert.
+__device__ __forceinline__ void pad_order(const ggemm_router_t& r, int from, int to, int lane, int lanes) {
+  for (int i = from + lane; i < to; i += lanes) r.order[i] = -1;
+}
+
+// The balance loss from counts, probs and the tokens used: one wave, fixed order.
+__device__ __forceinline__ void write_loss(const ggemm_router_t& r, const int* counts, const float* probs, int used) {
+  const int lane = threadIdx.x & 63;
+  float s = 0.0f;
+  for (int e = lane; e < r.experts; e += 64) s += (float)counts[e] * probs[e];
+  s = sum_lanes<64>(s);
+  if (lane == 0) r.loss[0] = used ? s * (r.balance_coef * (float)r.experts / ((float)r.topk * (float)used)) : 0.0f;
+}
+
+// Exclusive sums over experts of the counts rounded up to row_align, into off[0 .. experts]; called by
+// the whole workgroup (at most 4 experts a thread), ends with a barrier.
+__device__ __forceinline__ void scan_offsets(const int* counts, int experts, int align, int* off, int* tmp) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int c[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int e = 4 * tid + i;
+    c[i] = e < experts ? (counts[e] + align - 1) & -align : 0;
+    sum += c[i];
+  }
+  int inc = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int up = __shfl_up(inc, d);
+    inc += lane >= d ? up : 0;
+  }
+  if (lane == 63) tmp[wave] = inc;
+  __syncthreads();
+  int at = inc - sum;
+  for (int w = 0; w < wave; ++w) at += tmp[w];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (4 * tid + i <= experts) off[4 * tid + i] = at;
+    at += c[i];
+  }
+  if (tid == kThreads - 1 && experts == 4 * kThreads) off[experts] = at;
+  __syncthreads();
+}
+
+// First launch: choices, gates, ranks within the workgroup's tokens (into pos), counts and softmax sums
+// per workgroup.  kOne: the only workgroup, which finishes the call.
+template <int D, int L, int V, bool kOne>
+__global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, RouteWs ws, int span) {
+  constexpr int kRows = 64 / L, kPar = 4 * kRows;   // tokens a wave and a workgroup hold at a time
+  extern __shared__ uint32_t lds[];
+  const int words = span / 32, E = r.experts, K = r.topk;
+  uint32_t* bits = lds;                                        // E x words
+  float* part = reinterpret_cast<float*>(lds + E * words);     // 4 x (L V): the waves' softmax sums
+  __shared__ int s_used[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = sub * V;
+  const int t0 = blockIdx.x * span, t1 = min(t0 + span, r.tokens);
+  for (int i = tid; i < E * words; i += kThreads) bits[i] = 0;
+  __syncthreads();
+  float acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+  int used = 0;
+  for (int tb = t0; tb < t1; tb += kPar) {
+    const int t = tb + slot;
+    const bool on = t < t1 && !masked(r, t);
+    float x[V], p[V];
+    uint32_t key[V];
+    if (on) {
+      load_logits<D, V>(r, t, e0, x);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = -__builtin_inff();
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
+    float inv = 0.0f, chosen = 0.0f, m = 0.0f;
+    float mine = 0.0f;   // gate of place `sub` (+ L, ...) is stored as it is found; kept for renormalising
+    bool live = false;
+    for (int j = 0; j < K; ++j) {
+      uint32_t top = key[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) top = max(top, key[v]);
+      const uint32_t best = max_lanes<L>(top);
+      if (j == 0) {
+        live = best != 0;
+        m = of_key(best);
+        inv = exps<L, V>(x, m, p);
+      }
+      // the lowest lane of the token that holds it
+      const uint64_t holds = __ballot(top == best) >> (lane & ~(L - 1));
+      const bool here = best != 0 && __builtin_ctzll(holds) == sub;
+      float g = 0.0f;
+      if (here) {
+        int at = 0;
+#pragma unroll
+        for (int v = V - 1; v >= 0; --v)
+          if (key[v] == best) at = v;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v == at) {
+            key[v] = 0;
+            g = p[v] * inv;
+          }
+        const int e = e0 + at;
+        r.ids[(int64_t)t * K + j] = e;
+        r.gates[(int64_t)t * K + j] = g;
+        atomicOr(&bits[e * words + ((t - t0) >> 5)], 1u << ((t - t0) & 31));
+      }
+      if (best == 0 && t < t1 && sub == 0) {
+        r.ids[(int64_t)t * K + j] = -1;
+        r.gates[(int64_t)t * K + j] = 0.0f;
+      }
+      mine += g;
+    }
+    if (live) {
+      used += sub == 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += p[v] * inv;
+    }
+    if (r.renormalize) {
+      chosen = sum_lanes<L>(mine);
+      __threadfence_block();   // the gates were stored by the lanes that held them
+      for (int j = sub; j < K && live; j += L) {
+        float* g = r.gates + (int64_t)t * K + j;
+        if (r.ids[(int64_t)t * K + j] >= 0) *g = *g / chosen;
+      }
+    }
+  }
+  // softmax sums: over the tokens of a wave, then over the waves
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+#pragma unroll
+    for (int d = L; d < 64; d *= 2) acc[v] += __shfl_xor(acc[v], d);
+    if (lane < L) part[wave * L * V + e0 + v] = acc[v];
+  }
+  used = over_lanes<64>(used, [](int a, int b) { return a + b; });
+  if (lane == 0) s_used[wave] = used;
+  __syncthreads();
+  used = s_used[0] + s_used[1] + s_used[2] + s_used[3];
+  // ranks, counts
+  for (int i = tid; i < (t1 - t0) * K; i += kThreads) {
+    const int64_t at = (int64_t)t0 * K + i;
+    const int e = r.ids[at], t = i / K;
+    int rank = -1;
+    if (e >= 0) {
+      rank = __popc(bits[e * words + (t >> 5)] & ((1u << (t & 31)) - 1u));
+      for (int w = 0; w < t >> 5; ++w) rank += __popc(bits[e * words + w]);
+    }
+    r.pos[at] = rank;
+  }
+  __shared__ int s_off[kOne ? GGEMM_ROUTE_MAX_EXPERTS + 1 : 1], s_tmp[4];
+  for (int e = tid; e < E; e += kThreads) {
+    int c = 0;
+    for (int w = 0; w < words; ++w) c += __popc(bits[e * words + w]);
+    const float ps = part[e] + part[L * V + e] + part[2 * L * V + e] + part[3 * L * V + e];
+    if constexpr (kOne) {
+      r.counts[e] = c;
+      r.probs[e] = used ? ps / (float)used : 0.0f;
+    } else {
+      ws.hist[(int64_t)blockIdx.x * E + e] = c;
+      ws.psum[(int64_t)blockIdx.x * E + e] = ps;
+    }
+  }
+  if constexpr (!kOne) {
+    if (tid == 0) ws.used[blockIdx.x] = used;
+  } else {
+    __syncthreads();
+    scan_offsets(r.counts, E, r.row_align, s_off, s_tmp);
+    for (int e = tid; e <= E; e += kThreads) r.offsets[e] = s_off[e];
+    for (int i = tid; i < r.tokens * K; i += kThreads) {
+      const int e = r.ids[i];
+      if (e >= 0) {
+        const int row = s_off[e] + r.pos[i];
+        r.pos[i] = row;
+        if (row < r.max_rows) r.order[row] = i / K;
+      }
+    }
+    for (int e = tid; e < E; e += kThreads)
+      if (r.row_align > 1) pad_order(r, s_off[e] + r.counts[e], s_off[e + 1], 0, 1);
+    pad_order(r, s_off[E], r.max_rows, tid, kThreads);
+    if (tid == 0) r.used[0] = used;
+    if (wave == 0) write_loss(r, r.counts, r.probs, used);
+  }
+}
+
+// Second launch: a workgroup per 16 experts, 16 threads along the workgroups of the first launch each
+// taking a run of them: sums per run, then starting ranks.
+__global__ void __launch_bounds__(kThreads) route_scan_kernel(ggemm_router_t r, RouteWs ws, int groups) {
+  __shared__ int s_cnt[16][17], s_use[16];
+  __shared__ float s_p[16][17];
+  const int i = threadIdx.x & 15, c = threadIdx.x >> 4, e = blockIdx.x * 16 + i, E = r.experts;
+  const int run = ceil_div(groups, 16), g0 = min(c * run, groups), g1 = min(g0 + run, groups);
+  int cnt = 0;
+  float ps = 0.0f;
+  if (e < E) {
+    for (int g = g0; g < g1; ++g) {
+      cnt += ws.hist[(int64_t)g * E + e];
+      ps += ws.psum[(int64_t)g * E + e];
+    }
+  }
+  s_cnt[c][i] = cnt;
+  s_p[c][i] = ps;
+  int use = 0;
+  for (int g = threadIdx.x; g < groups; g += kThreads) use += ws.used[g];
+  use = over_lanes<64>(use, [](int a, int b) { return a + b; });
+  if ((threadIdx.x & 63) == 0) s_use[threadIdx.x >> 6] = use;
+  __syncthreads();
+  use = s_use[0] + s_use[1] + s_use[2] + s_use[3];
+  int at = 0;
+  for (int q = 0; q < c; ++q) at += s_cnt[q][i];
+  if (e < E) {
+    if (c == 15) r.counts[e] = at + cnt;
+    if (c == 0) {
+      float sum = 0.0f;
+      for (int q = 0; q < 16; ++q) sum += s_p[q][i];
+      r.probs[e] = use ? sum / (float)use : 0.0f;
+    }
+    for (int g = g0; g < g1; ++g) {
+      int* h = ws.hist + (int64_t)g * E + e;
+      const int n = *h;
+      *h = at;
+      at += n;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) r.used[0] = use;
+}
+
+// Third launch: rows of the pairs, order, padding, loss.  Workgroup b takes the pairs of workgroup b of
+// the first launch.
+__global__ void __launch_bounds__(kThreads) route_place_kernel(ggemm_router_t r, RouteWs ws, int span) {
+  __shared__ int s_off[GGEMM_ROUTE_MAX_EXPERTS + 1], s_tmp[4];
+  const int tid = threadIdx.x, E = r.experts, K = r.topk;
+  scan_offsets(r.counts, E, r.row_align, s_off, s_tmp);
+  const int t0 = blockIdx.x * span, t1 = min(t0 + span, r.tokens);
+  for (int i = tid; i < (t1 - t0) * K; i += kThreads) {
+    const int64_t at = (int64_t)t0 * K + i;
+    const int e = r.ids[at];
+    if (e >= 0) {
+      const int row = s_off[e] + ws.hist[(int64_t)blockIdx.x * E + e] + r.pos[at];
+      r.pos[at] = row;
+      if (row < r.max_rows) r.order[row] = t0 + i / K;
+    }
+  }
+  const int all = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
+  if (r.row_align > 1)
+    for (int e = me; e < E; e += all) pad_order(r, s_off[e] + r.counts[e], s_off[e + 1], 0, 1);
+  pad_order(r, s_off[E], r.max_rows, me, all);
+  if (blockIdx.x == 0) {
+    for (int e = tid; e <= E; e += kThreads) r.offsets[e] = s_off[e];
+    if (tid < 64) write_loss(r, r.counts, r.probs, r.used[0]);
+  }
+}
+
+// Gradient: dx = p (s - <p, s>) + c, with s_e = d_loss coef E counts_e / (topk used^2) and, for the chosen
+// places, c_j = g_j (dg_j - <g, dg>) when the gates are renormalised; else s_e takes dg_j too and c = 0.
+// The token's dg (or c) by expert goes through a row of LDS that is zero outside the chosen places.
+template <int D, int L, int V>
+__global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t r, const float* __restrict__ d_gates,
+                                                                  const float* __restrict__ d_loss, void* d_logits,
+                                                                  int64_t ld_d, int per) {
+  using T = typename Elem<D>::T;
+  constexpr int kRows = 64 / L, kPar = 4 * kRows;
+  __shared__ float s_row[kPar * L * V];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = sub * V, E = r.experts, K = r.topk;
+  float* row = s_row + slot * L * V;
+  const int used = r.used[0];
+  const float n = (float)used;
+  const float f = d_loss && used ? d_loss[0] * (r.balance_coef * (float)E / ((float)K * n * n)) : 0.0f;
+  float s[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    s[v] = e0 + v < E ? f * (float)r.counts[e0 + v] : 0.0f;
+    row[e0 + v] = 0.0f;
+  }
+  const int t0 = blockIdx.x * per, t1 = min(t0 + per, r.tokens);
+  for (int tb = t0; tb < t1; tb += kPar) {
+    const int t = tb + slot;
+    const bool in = t < t1, on = in && !masked(r, t);
+    float x[V], p[V], d[V];
+    if (on) {
+      load_logits<D, V>(r, t, e0, x);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = -__builtin_inff();
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) top = max(top, key_of(x[v]));
+    top = max_lanes<L>(top);
+    const float inv = exps<L, V>(x, of_key(top), p);
+    const bool live = on && top != 0;
+    float dot = 0.0f;
+    if (r.renormalize && d_gates) {
+      for (int j = sub; j < K && live; j += L)
+        dot += r.gates[(int64_t)t * K + j] * (r.ids[(int64_t)t * K + j] >= 0 ? d_gates[(int64_t)t * K + j] : 0.0f);
+      dot = sum_lanes<L>(dot);
+    }
+    for (int j = sub; j < K && live && d_gates; j += L) {
+      const int e = r.ids[(int64_t)t * K + j];
+      const float dg = d_gates[(int64_t)t * K + j];
+      if (e >= 0 && e < E) row[e] = r.renormalize ? r.gates[(int64_t)t * K + j] * (dg - dot) : dg;
+    }
+    __threadfence_block();
+    float c[V], ps = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      c[v] = row[e0 + v];
+      p[v] = live ? p[v] * inv : 0.0f;
+      d[v] = r.renormalize ? s[v] : s[v] + c[v];
+      ps += p[v] * d[v];
+    }
+    ps = sum_lanes<L>(ps);
+    __threadfence_block();
+#pragma unroll
+    for (int v = 0; v < V; ++v) row[e0 + v] = 0.0f;
+    __threadfence_block();
+    if (in) {
+      T* out = static_cast<T*>(d_logits) + (int64_t)t * ld_d + e0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float g = p[v] * (d[v] - ps) + (r.renormalize ? c[v] : 0.0f);
+        // a barred expert has p = 0 and no place, but 0 times a NaN sum is not 0
+        if (e0 + v < E) out[v] = (T)(live && x[v] != -__builtin_inff() ? g : 0.0f);
+      }
+    }
+  }
+}
+
+// f(L, V) for the lanes and values per lane that hold `experts` logits
+template <class F>
+void with_lanes(int experts, F&& f) {
+#define GGEMM_LV(l, v) f(std::integral_constant<int, l>{}, std::integral_constant<int, v>{})
+  if (experts <= 8) GGEMM_LV(8, 1);
+  else if (experts <= 16) GGEMM_LV(8, 2);
+  else if (experts <= 32) GGEMM_LV(8, 4);
+  else if (experts <= 64) GGEMM_LV(16, 4);
+  else if (experts <= 128) GGEMM_LV(16, 8);
+  else if (experts <= 256) GGEMM_LV(16, 16);
+  else if (experts <= 512) GGEMM_LV(32, 16);
+  else GGEMM_LV(64, 16);
+#undef GGEMM_LV
+}
+
+bool sizes_ok(int tokens, int experts, int topk) {
+  return tokens >= 0 && experts >= 1 && experts <= GGEMM_ROUTE_MAX_EXPERTS && topk >= 1 &&
+         topk <= GGEMM_ROUTE_MAX_TOPK && topk <= experts && (int64_t)tokens * topk <= 0x7fffffff;
+}
+
+bool route_ok(const ggemm_router_t* r) {
+  if (!r || !sizes_ok(r->tokens, r->experts, r->topk) || !elem_known(r->dtype)) return false;
+  if (r->tokens > 0 && (!r->logits || !aligned(r->logits, elem_bytes(r->dtype)) || r->ld < r->experts)) return false;
+  if (r->tokens > 0 && (!r->ids || !r->gates)) return false;
+  return r->counts && r->used;
+}
+
+}  // namespace
+
+size_t route_workspace(int tokens, int experts, int topk) {
+  if (!sizes_ok(tokens, experts, topk)) return 0;
+  const Shape sh = shape_of(tokens);
+  return 2 * align_up((size_t)sh.groups * experts * 4, 16) + align_up((size_t)sh.groups * 4, 16);
+}
+
+int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
+  if (!route_ok(r) || !r->offsets || !r->probs || !r->loss || (r->tokens > 0 && !r->pos)) return GGEMM_ERR_INVALID;
+  if (r->row_align < 1 || r->row_align > GGEMM_ROUTE_MAX_ALIGN || (r->row_align & (r->row_align - 1)) != 0)
+    return GGEMM_ERR_INVALID;
+  const int64_t cap = (int64_t)r->tokens * r->topk + (int64_t)r->experts * (r->row_align - 1);
+  if (cap > 0x7fffffff || r->max_rows < cap || (r->max_rows > 0 && !r->order)) return GGEMM_ERR_INVALID;
+  if (ws_bytes < route_workspace(r->tokens, r->experts, r->topk)) return GGEMM_ERR_WORKSPACE;
+  if (!ws || !aligned(ws, 16)) return GGEMM_ERR_INVALID;
+  const Shape sh = shape_of(r->tokens);
+  const RouteWs w = carve(ws, sh, r->experts);
+  with_elem(r->dtype, [&](auto d) {
+    with_lanes(r->experts, [&](auto l, auto v) {
+      constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
+      const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + 4 * L * V * 4;
+      if (sh.groups == 1)
+        route_kernel<D, L, V, true><<<1, kThreads, lds, s>>>(*r, w, sh.span);
+      else
+        route_kernel<D, L, V, false><<<sh.groups, kThreads, lds, s>>>(*r, w, sh.span);
+    });
+  });
+  if (sh.groups > 1) {
+    route_scan_kernel<<<ceil_div(r->experts, 16), kThreads, 0, s>>>(*r, w, sh.groups);
+    route_place_kernel<<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+  }
+  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+}
+
+int route_backward(const ggemm_router_t* r, const float* d_gates, const float* d_loss, void* d_logits, int64_t ld_d,
+                   hipStream_t s) {
+  if (!route_ok(r)) return GGEMM_ERR_INVALID;
+  if (r->tokens == 0) return GGEMM_OK;
+  if (!d_logits || !aligned(d_logits, elem_bytes(r->dtype)) || ld_d < r->experts) return GGEMM_ERR_INVALID;
+  with_elem(r->dtype, [&](auto d) {
+    with_lanes(r->experts, [&](auto l, auto v) {
+      constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
+      constexpr int kPar = 256 / L;
+      const int per = std::max(kPar, (int)align_up((size_t)ceil_div(r->tokens, 2048), kPar));
+      route_backward_kernel<D, L, V><<<ceil_div(r->tokens, per), kThreads, 0, s>>>(*r, d_gates, d_loss, d_logits, ld_d, per);
+    });
+  });
+  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+}
+
+}  // namespace ggemm
+
+extern "C" size_t ggemm_route_workspace(int tokens, int experts, int topk) {
+  return ggemm::route_workspace(tokens, experts, topk);
+}
+extern "C" int ggemm_route(const ggemm_router_t* r, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  return ggemm::route(r, workspace, workspace_bytes, stream);
+}
+extern "C" int ggemm_route_backward(const ggemm_router_t* r, const float* d_gates, const float* d_loss, void* d_logits,
+                                    int64_t ld_d, hipStream_t stream) {
+  return ggemm::route_backward(r, d_gates, d_loss, d_logits, ld_d, stream);
+}

@@ -1,7 +1,8 @@
 """ctypes binding of the MI355X grouped Ozaki-II DGEMM library (libggemm_mi355x.so).
 
 Mirrors the C ABI of include/ggemm.h, include/ggemm_graph.h and include/ggemm_oz2.h: same names,
-struct layouts and return codes as the reference's interface.  Device memory is passed as plain
+struct layouts and return codes as the reference's interface; and that of include/ggemm_mx4.h (4-bit
+quantisation and grouped products) and include/ggemm_route.h (the router of an expert layer).  Device memory is passed as plain
 integer addresses (e.g. torch_tensor.data_ptr()); streams as integer handles (0 = default).
 The library must be built (coding-basic-hw-2_amd/build_lib.py); there is no fallback path.
 """
@@ -101,6 +102,48 @@ class ReuseBytes(C.Structure):
                 ("ws_B8", C.c_double)]
 
 
+F32, BF16, F16 = 0, 1, 2
+DTYPES = {"f32": F32, "bf16": BF16, "f16": F16}
+MX4_ROWS, MX4_INNER = 0, 1
+MX4_BLOCK, MX4_MAX_GROUPS = 32, 4096
+ROUTE_MAX_EXPERTS, ROUTE_MAX_TOPK, ROUTE_MAX_ALIGN = 1024, 64, 1024
+
+
+class Mx4Quant(C.Structure):
+    """include/ggemm_mx4.h ggemm_mx4_quant_t"""
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int), ("x_rows", C.c_int),
+                ("x", C.c_void_p), ("ld", C.c_int64), ("index", C.c_void_p),
+                ("codes", C.c_void_p), ("ld_codes", C.c_int64), ("scales", C.c_void_p), ("ld_scales", C.c_int64),
+                ("codes_t", C.c_void_p), ("ld_codes_t", C.c_int64), ("scales_t", C.c_void_p),
+                ("ld_scales_t", C.c_int64)]
+
+
+class Mx4Dequant(C.Structure):
+    """include/ggemm_mx4.h ggemm_mx4_dequant_t"""
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int),
+                ("codes", C.c_void_p), ("ld_codes", C.c_int64), ("scales", C.c_void_p), ("ld_scales", C.c_int64),
+                ("y", C.c_void_p), ("ld", C.c_int64)]
+
+
+class Mx4Gemm(C.Structure):
+    """include/ggemm_mx4.h ggemm_mx4_gemm_t"""
+    _fields_ = [("form", C.c_int), ("groups", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int),
+                ("dtype", C.c_int), ("alpha", C.c_float), ("beta", C.c_float),
+                ("a", C.c_void_p), ("lda", C.c_int64), ("a_scales", C.c_void_p), ("lda_scales", C.c_int64),
+                ("b", C.c_void_p), ("ldb", C.c_int64), ("b_stride", C.c_int64),
+                ("b_scales", C.c_void_p), ("ldb_scales", C.c_int64), ("b_scales_stride", C.c_int64),
+                ("offsets", C.c_void_p), ("c", C.c_void_p), ("ldc", C.c_int64), ("c_stride", C.c_int64)]
+
+
+class Router(C.Structure):
+    """include/ggemm_route.h ggemm_router_t"""
+    _fields_ = [("tokens", C.c_int), ("experts", C.c_int), ("topk", C.c_int), ("row_align", C.c_int),
+                ("dtype", C.c_int), ("renormalize", C.c_int), ("balance_coef", C.c_float), ("max_rows", C.c_int),
+                ("logits", C.c_void_p), ("ld", C.c_int64), ("mask", C.c_void_p), ("ids", C.c_void_p),
+                ("gates", C.c_void_p), ("pos", C.c_void_p), ("counts", C.c_void_p), ("offsets", C.c_void_p),
+                ("order", C.c_void_p), ("used", C.c_void_p), ("probs", C.c_void_p), ("loss", C.c_void_p)]
+
+
 REUSE_EXACT_N, REUSE_PROMOTE = 0, 1
 REUSE_OK, REUSE_ERR_CAPACITY, REUSE_ERR_INVALID = 0, 1, 2
 
@@ -152,6 +195,13 @@ SIGNATURES = [
     ("build_operand_reuse", ReusePlan, [_P, C.POINTER(Problem), C.c_int, C.POINTER(C.c_int), C.c_int]),
     ("operand_reuse_bytes", None, [C.POINTER(ReusePlan), C.POINTER(Problem), C.POINTER(C.c_int),
                                    C.POINTER(ReuseBytes), C.POINTER(ReuseBytes)]),
+    ("ggemm_mx4_quantize", C.c_int, [C.POINTER(Mx4Quant), _P]),
+    ("ggemm_mx4_dequantize", C.c_int, [C.POINTER(Mx4Dequant), _P]),
+    ("ggemm_mx4_gemm_workspace", C.c_size_t, [C.POINTER(Mx4Gemm)]),
+    ("ggemm_mx4_gemm", C.c_int, [C.POINTER(Mx4Gemm), _P, C.c_size_t, _P]),
+    ("ggemm_route_workspace", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("ggemm_route", C.c_int, [C.POINTER(Router), _P, C.c_size_t, _P]),
+    ("ggemm_route_backward", C.c_int, [C.POINTER(Router), _P, _P, _P, C.c_int64, _P]),
 ]
 
 _lib = None

@@ -10,11 +10,9 @@
 namespace ggemm {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 64;
+constexpr int kCus = 256;   // compute units of an MI355X
 
-// Where a workgroup's tile lies: its group, its first row and the group's end (rows form), or the blocks of
-// the inner dimension it sums over (inner form).
+// The rows [lo, hi) of a group; g = -1: none.
 struct Span {
   int g, lo, hi;
 };
@@ -24,99 +22,524 @@ __device__ __forceinline__ int clamp_to(int x, int n) { return min(max(x, 0), n)
 // The block that an offset along an inner dimension of k starts at.
 __device__ __forceinline__ int block_at(int x, int k) { return x >= k ? ceil_div(k, 32) : max(x, 0) / 32; }
 
-// Row tile t of the groups' tiles in order, each group cut into tiles of TM rows; g = -1 past the last.
-// Every wave finds it on its own: 64 groups a step, an inclusive sum of their tile counts over the lanes.
+// Tiles of the groups in order (TM rows, nt of them along n).  Every wave looks a tile's group up on its own: a lane
+// has one of 64 consecutive groups, with an inclusive sum over the lanes of their tile counts.
 template <int TM>
-__device__ __forceinline__ Span find_rows(const ggemm_mx4_gemm_t& p, int t) {
-  const int lane = threadIdx.x & 63;
-  if (!p.offsets) return t * TM < p.m ? Span{0, t * TM, p.m} : Span{-1, 0, 0};
-  for (int g0 = 0; g0 < p.groups; g0 += 64) {
-    const int g = min(g0 + lane, p.groups - 1);
-    const int lo = clamp_to(p.offsets[g], p.m), hi = clamp_to(p.offsets[g + 1], p.m);
-    int sum = g0 + lane < p.groups ? (max(hi - lo, 0) + TM - 1) / TM : 0;
-    const int own = sum;
+struct Groups {
+  int lo, hi, own, sum, all;   // this lane's group: rows, tiles, tiles up to it; tiles of the 64
+  __device__ __forceinline__ Groups(const ggemm_mx4_gemm_t& p, int g0, int nt) {
+    const int lane = threadIdx.x & 63, g = min(g0 + lane, p.groups - 1);
+    lo = p.offsets ? clamp_to(p.offsets[g], p.m) : 0;
+    hi = p.offsets ? clamp_to(p.offsets[g + 1], p.m) : p.m;
+    own = sum = g0 + lane < p.groups ? ceil_div(max(hi - lo, 0), TM) * nt : 0;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int up = __shfl_up(sum, d);
       sum += lane >= d ? up : 0;
     }
-    const uint64_t hit = __ballot(sum > t);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int before = __shfl(sum - own, l);
-      return Span{g0 + l, __shfl(lo, l) + (t - before) * TM, __shfl(hi, l)};
-    }
-    t -= __shfl(sum, 63);
+    all = __builtin_amdgcn_readlane(sum, 63);
   }
-  return Span{-1, 0, 0};
+  // The group of tile t; t becomes the number within the group.
+  __device__ __forceinline__ bool find(int g0, int& t, Span& s) const {
+    if (t >= all) {
+      t -= all;
+      return false;
+    }
+    const int l = __builtin_ctzll(__ballot(sum > t));
+    t -= __builtin_amdgcn_readlane(sum - own, l);
+    s = Span{g0 + l, __builtin_amdgcn_readlane(lo, l), __builtin_amdgcn_readlane(hi, l)};
+    return true;
+  }
+};
+// `first`: the first 64 groups, which a kernel looks up in more than once.
+template <int TM>
+__device__ __forceinline__ Span find_tile(const ggemm_mx4_gemm_t& p, const Groups<TM>& first, int& t, int nt) {
+  Span s{-1, 0, 0};
+  if (first.find(0, t, s)) return s;
+  for (int g0 = 64; g0 < p.groups; g0 += 64)
+    if (Groups<TM>(p, g0, nt).find(g0, t, s)) return s;
+  return s;
 }
 
-template <int D>
-__device__ __forceinline__ void store_c(const ggemm_mx4_gemm_t& p, typename Elem<D>::T* c, float v) {
-  v *= p.alpha;
-  if (p.beta != 0.0f) v += p.beta * (float)*c;
-  *c = (typename Elem<D>::T)v;
+// Where results go: c = alpha v + beta c, rounded once.
+struct Out {
+  float alpha, beta;
+  int64_t ldc;
+};
+template <class T>
+__device__ __forceinline__ void store_one(T* c, float v, const Out& o) {
+  v *= o.alpha;
+  if (o.beta != 0.0f) v += o.beta * (float)*c;
+  *c = (T)v;
+}
+// N = 16 / sizeof(T) (or half of it) values side by side, c aligned to them.  The stores are non-temporal: C is not
+// read here again and would push the operands out of L2 (32 groups of 2048 x 4096 x 4096: 701 -> 623 us).
+template <class T, int N>
+__device__ __forceinline__ void store_run(T* c, const float (&v)[N], const Out& o) {
+  typedef uint32_t words __attribute__((ext_vector_type(N * sizeof(T) / 4)));
+  struct alignas(N * sizeof(T)) Run { T x[N]; } w;
+  float u[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) u[e] = o.alpha * v[e];
+  if (o.beta != 0.0f) {
+    w = *reinterpret_cast<const Run*>(c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) u[e] += o.beta * (float)w.x[e];
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) w.x[e] = (T)u[e];
+  __builtin_nontemporal_store(__builtin_bit_cast(words, w), reinterpret_cast<words*>(c));
 }
 
-// Four waves, 32 x 32 each, operands straight from memory.
-template <int D, bool kInner>
-__global__ void __launch_bounds__(kThreads) gemm_simple_kernel(ggemm_mx4_gemm_t p) {
+// ---------------------------------------------------------------- tiles through LDS
+// A workgroup computes a BM x BN tile with WGM x WGN waves of FM x FN blocks of 32 x 32.  The inner dimension goes
+// in stages of 256 codes: 128 bytes, one memory line, of every row of A and B, from memory to LDS
+// directly, into a ring of two stages.  One barrier a stage: a wave waits for its part of stage s + 1 (a
+// whole stage's products old) and for its last fragments of stage s, passes the barrier, sends for stage
+// s + 2 into the slot of stage s, and has half of stage s's products still to issue, which cover the
+// barrier and the first reads of stage s + 1.
+// Scale bytes come in windows of 32 per row (four stages), two windows in LDS: the compute unit's line
+// requests bound this kernel, and 8 bytes of every row per stage took as many as the codes (256 x 256 tiles,
+// 8192 x 8192 x 16384: %%SCALE%%).
+// LDS: chunk c (16 bytes, one block's codes) of row r lies at position c ^ (r / 2) % 8 of the row, so that the 16
+// rows of a group of lanes reading one chunk hit all banks.  Step t of a stage takes block t of the
+// stage's first four from lanes 0-31 and block 4 + t from lanes 32-63 (any pairing will do as long as
+// A and B agree), so that one scale word per lane and row block serves the four steps.
+// A stage may begin before the group's first block or end past its last one (or the row's).  Those blocks get
+// scale byte 0 on both sides: codes are finite, so their products are below 2^11 2^-254, and adding them
+// leaves every 32-bit sum as it is.
+template <int BM_, int BN_, int WGM_, int WGN_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, NW = WGM * WGN, NT = 64 * NW;
+  static constexpr int FM = BM / WGM / 32, FN = BN / WGN / 32;
+  static constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;
+  static constexpr int WIN = (BM + BN) * 32;                 // scales of a window
+  static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;   // 1 KB pieces of A and B per wave
+  static constexpr int PS = (BM + BN) / 32 / NW;             // 1 KB pieces of a window per wave
+  static constexpr int EPI = 32 * FN * 32 * 4;               // epilogue bytes per wave, in the second slot
+  static constexpr int SMEM = 2 * STAGE + 2 * WIN;
+  static constexpr int WAVES = BM * BN >= 256 * 256 ? NW / 4 : 2;   // per SIMD: one workgroup of 256 x 256 a compute unit, else two
+  static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && (BM + BN) / 32 % NW == 0 && NW % 2 == 0, "pieces");
+  static_assert(NW * EPI <= STAGE, "epilogue");
+};
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+// 64 lanes' 16 (or 4) bytes at base + off to LDS byte address lds + 16 (4) lane.  Written as assembly so that the
+// compiler does not wait for all of them before the next LDS read; the waits are stage_wait's.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma4(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+// This wave's transfers to LDS landed.
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// This wave's LDS operations done; then every wave's.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Both.
+__device__ __forceinline__ void stage_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ i32x8 frag(u32x4 x) {
+  return __builtin_bit_cast(i32x8, __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1));
+}
+
+// Sources of a tile's stages and scale windows: uniform bases and this lane's offsets.
+template <class C>
+struct Source {
+  const uint8_t *a, *b, *as, *bs;
+  uint32_t va[C::PA], vb[C::PB], vs[C::PS];
+  int chunk, nb;   // this lane's chunk of a row, blocks of a row
+  int lda_scales, ldb_scales, rows, cols;
+
+  __device__ __forceinline__ Source(const ggemm_mx4_gemm_t& p, const uint8_t* b0, const uint8_t* bs0, int row0, int rows_,
+                                    int col0, int cols_, int wave, int lane)
+      : a(p.a + (int64_t)row0 * p.lda), b(b0 + (int64_t)col0 * p.ldb), as(p.a_scales + (int64_t)row0 * p.lda_scales),
+        bs(bs0 + (int64_t)col0 * p.ldb_scales), nb(ceil_div(p.k, 32)), lda_scales((int)p.lda_scales),
+        ldb_scales((int)p.ldb_scales), rows(rows_), cols(cols_) {
+    // pieces wave, wave + NW, ... of 8 rows; NW is even, so the swizzle's upper bit is the wave's
+    chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+#pragma unroll
+    for (int q = 0; q < C::PA; ++q) va[q] = (uint32_t)min(8 * (wave + C::NW * q) + (lane >> 3), rows - 1) * (uint32_t)p.lda + 16 * chunk;
+#pragma unroll
+    for (int q = 0; q < C::PB; ++q) vb[q] = (uint32_t)min(8 * (wave + C::NW * q) + (lane >> 3), cols - 1) * (uint32_t)p.ldb + 16 * chunk;
+    // windows: a piece is 32 rows (of A, then of B) of two 16-byte halves, exchanged in rows with bit 3 set
+#pragma unroll
+    for (int q = 0; q < C::PS; ++q) vs[q] = scale_row(32 * (wave + C::NW * q) + (lane >> 1)) + 16 * ((lane ^ (lane >> 4)) & 1);
+  }
+  __device__ __forceinline__ uint32_t scale_row(int r) const {
+    return r < C::BM ? (uint32_t)min(r, rows - 1) * (uint32_t)lda_scales : (uint32_t)min(r - C::BM, cols - 1) * (uint32_t)ldb_scales;
+  }
+  // Blocks blk .. blk + 7 (blk a multiple of 4, blk < nb) into the slot at `slot`.  Chunks past the row's last block
+  // are read from the stage's first.
+  __device__ __forceinline__ void load(int blk, uint32_t slot, int wave) const {
+    const uint32_t back = blk + chunk >= nb ? 16 * chunk : 0;
+    const uint8_t *ak = a + (int64_t)16 * blk, *bk = b + (int64_t)16 * blk;
+#pragma unroll
+    for (int q = 0; q < C::PA; ++q) dma16(ak, va[q] - back, slot + 1024 * (wave + C::NW * q));
+#pragma unroll
+    for (int q = 0; q < C::PB; ++q) dma16(bk, vb[q] - back, slot + C::SA + 1024 * (wave + C::NW * q));
+  }
+  // The scale bytes of blocks blk .. blk + 31 (blk a multiple of 32, blk < nb).  A window that the row ends in
+  // goes by words: those past the last block are read from the window's first.
+  __device__ __forceinline__ void load_scales(int blk, uint32_t slot, int wave, int lane) const {
+    if (blk + 32 <= nb) {
+#pragma unroll
+      for (int q = 0; q < C::PS; ++q) {
+        const int piece = wave + C::NW * q;
+        dma16((piece < C::BM / 32 ? as : bs) + blk, vs[q], slot + 1024 * piece);
+      }
+    } else {
+#pragma unroll 1
+      for (int piece = wave; piece < (C::BM + C::BN) / 8; piece += C::NW) {   // 8 rows of 8 words
+        const int r = 8 * piece + (lane >> 3), w = 4 * ((lane & 7) ^ (r >> 1 & 4));
+        dma4((piece < C::BM / 8 ? as : bs) + blk, scale_row(r) + (blk + w < nb ? w : 0), slot + 256 * piece);
+      }
+    }
+  }
+};
+
+// The codes of blocks blk .. blk + 7 into the slot at offset so of the ring, and the scale window that begins in them.
+template <class C>
+__device__ __forceinline__ void load_stage(const Source<C>& src, uint32_t ring, int blk, int so, int wave, int lane) {
+  const int win = (blk + 7) & ~31;
+  if (win >= blk && win < src.nb) src.load_scales(win, ring + 2 * C::STAGE + (win >> 5 & 1) * C::WIN, wave, lane);
+  src.load(blk, ring + so, wave);
+}
+// The first stage of blocks [b0, b1) into the first slot.
+template <class C>
+__device__ __forceinline__ void load_first(const Source<C>& src, uint32_t ring, int b0, int wave, int lane) {
+  const int start = b0 & ~3;
+  if (start & 31) src.load_scales(start & ~31, ring + 2 * C::STAGE + (start >> 5 & 1) * C::WIN, wave, lane);
+  load_stage(src, ring, start, 0, wave, lane);
+}
+
+// The wave's FM x FN blocks, as C's transpose: lane l holds of block (i, j) row 32 i + l % 32 and columns
+// 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.  The first stage has landed (every wave's part).
+template <class C>
+__device__ __forceinline__ void tile_products(uint8_t* lds, const Source<C>& src, int b0, int b1, f32x16 (&acc)[C::FM][C::FN]) {
+  constexpr int FM = C::FM, FN = C::FN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % C::WGM, wn = wave / C::WGM;
+  const int start = b0 & ~3, nk = ceil_div(b1 - start, 8);
+  const uint32_t base = lds_addr(lds);
+  const int fr = lane & 31, half = lane >> 5, x = (fr >> 1) & 7;
+  const uint8_t* const pa = lds + (wm * FM * 32 + fr) * 128;
+  const uint8_t* const pb = lds + C::SA + (wn * FN * 32 + fr) * 128;
+  const uint8_t* const psa = lds + 2 * C::STAGE + (wm * FM * 32 + fr) * 32;
+  const uint8_t* const psb = lds + 2 * C::STAGE + (C::BM + wn * FN * 32 + fr) * 32;
+
+  u32x4 a[2][FM], b[2][FN];
+  uint32_t sa[FM], sb[FN];
+  auto read = [&](int s, int t, int so) {   // fragments of step t of the stage at so, into set s
+    const int ch = ((4 * half + t) ^ x) * 16;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) a[s][i] = *reinterpret_cast<const u32x4*>(pa + so + i * 4096 + ch);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) b[s][j] = *reinterpret_cast<const u32x4*>(pb + so + j * 4096 + ch);
+  };
+  auto scales = [&](int kt) {   // of stage kt's four steps; blocks outside [b0, b1) get byte 0
+    const int at = start + 8 * kt + 4 * half;
+    const int so = (at >> 5 & 1) * C::WIN + ((at & 28) ^ (fr << 1 & 16));
+    const int lo = min(max(b0 - at, 0), 4), hi = min(max(b1 - at, 0), 4);
+    const uint64_t ones = 0xffffffffull;
+    const uint32_t keep = lo < hi ? (uint32_t)(ones << (8 * lo)) & (uint32_t)(ones >> (32 - 8 * hi)) : 0u;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(psa + so + i * 1024) & keep;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const uint32_t*>(psb + so + j * 1024) & keep;
+  };
+  auto products = [&](int s, auto t) {
+    constexpr int T = decltype(t)::value;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(b[s][j]), frag(a[s][i]), acc[i][j], 4, 4, T, (int)sb[j], T, (int)sa[i]);
+  };
+  // the products issued so far stay before what follows (else they would sink below the next reads and barrier)
+  auto pin = [&]() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));
+  };
+  using std::integral_constant;
+  if (nk > 1) load_stage(src, base, start + 8, C::STAGE, wave, lane);
+  scales(0);
+  read(0, 0, 0);
+  int so = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    read(1, 1, so);
+    products(0, integral_constant<int, 0>{});
+    read(0, 2, so);
+    products(1, integral_constant<int, 1>{});
+    read(1, 3, so);
+    const int sn = C::STAGE - so;
+    pin();
+    stage_wait();
+    if (kt + 2 < nk) load_stage(src, base, start + 8 * (kt + 2), so, wave, lane);
+    products(0, integral_constant<int, 2>{});
+    read(0, 0, sn);   // after the last stage: what an earlier one left, not used
+    products(1, integral_constant<int, 3>{});
+    pin();
+    scales(kt + 1);
+    so = sn;
+  }
+}
+
+// Blocks to C: a wave turns one row of blocks at a time through its own part of the ring's second slot (32-bit; the
+// 16-byte piece q of row r lies at q ^ r % (pieces of a row), which spreads both the writes and the reads over
+// the banks), then stores whole 16-byte pieces along C's rows.
+// Before the first store it waits for the transfers in flight, the next tile's first stage.
+template <class C, int D, bool kVec>
+__device__ __forceinline__ void tile_store(uint8_t* lds, const Out& o, typename Elem<D>::T* c, int m_rem, int n_rem,
+                                           const f32x16 (&acc)[C::FM][C::FN]) {
   using T = typename Elem<D>::T;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n0 = blockIdx.x * kTile + (wave & 1) * 32;
-  int m0, m_end, b0 = 0, b1, g;
+  constexpr int FM = C::FM, FN = C::FN, W = 32 * FN, Q = W / 4;    // columns, 16-byte pieces of an LDS row
+  constexpr int E = 16 / (int)sizeof(T), LR = W / E, RI = 64 / LR; // elements a lane, lanes a row, rows at a time
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % C::WGM, wn = wave / C::WGM;
+  f32x4* const st = reinterpret_cast<f32x4*>(lds + C::STAGE + wave * C::EPI);
+  const int r0 = wm * FM * 32, c0 = wn * W + (lane % LR) * E;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        st[(lane & 31) * Q + ((8 * j + 2 * q + (lane >> 5)) ^ (lane & (Q - 1)))] =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    if (i == 0) landed();
+#pragma unroll 2
+    for (int r = lane / LR; r < 32; r += RI) {
+      const int row = r0 + 32 * i + r;
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 u = st[r * Q + (((lane % LR) * (E / 4) + e / 4) ^ (r & (Q - 1)))];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) v[e + z] = u[z];
+      }
+      if (row >= m_rem) continue;
+      T* const out = c + (int64_t)row * o.ldc + c0;
+      if (kVec && c0 + E <= n_rem) {
+        store_run<T, E>(out, v, o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (c0 + e < n_rem) store_one(out + e, v[e], o);
+      }
+    }
+  }
+}
+
+constexpr int kChunk = 32;   // consecutive tiles that one XCD gets
+// The tile of workgroup b: workgroups go to the XCDs in turn, so runs of kChunk tiles that share rows of A and B
+// share an L2.  Ragged ends of 8 kChunk tiles keep their number.
+__device__ __forceinline__ int tile_number(int b, int total) {
+  constexpr int span = kXcds * kChunk;
+  if (b >= total / span * span) return b;
+  const int q = b / kXcds;
+  return q / kChunk * span + b % kXcds * kChunk + q % kChunk;
+}
+// Tile t of a rows x cols arrangement of tiles, in bands of 4 rows, down each band's columns.
+__device__ __forceinline__ void raster(int t, int rows, int cols, int& r, int& c) {
+  const int band = t / (4 * cols), r0 = 4 * band, h = min(4, rows - r0), l = t - r0 * cols;
+  r = r0 + l % h;
+  c = l / h;
+}
+
+// Where a tile lies: its group, first row, the group's last row + 1, first column, blocks of the inner dimension.
+struct Place {
+  int g, m0, m_end, n0, b0, b1;
+};
+template <class C, bool kInner>
+__device__ __forceinline__ Place place_of(const ggemm_mx4_gemm_t& p, const Groups<C::BM>& first, int t) {
+  const int nt = ceil_div(p.n, C::BN);
+  Place a{-1, 0, 0, 0, 0, ceil_div(p.k, 32)};
+  int tm, tn;
   if constexpr (kInner) {
-    g = blockIdx.z;
-    m0 = blockIdx.y * kTile;
-    m_end = p.m;
-    b1 = ceil_div(p.k, 32);
+    const int mt = ceil_div(p.m, C::BM);
+    a.g = t / (mt * nt);
+    raster(t - a.g * mt * nt, mt, nt, tm, tn);
+    a.m0 = tm * C::BM;
+    a.m_end = p.m;
     if (p.offsets) {
-      b0 = block_at(p.offsets[g], p.k);
-      b1 = block_at(p.offsets[g + 1], p.k);
+      a.b0 = block_at(p.offsets[a.g], p.k);
+      a.b1 = block_at(p.offsets[a.g + 1], p.k);
     }
   } else {
-    const Span s = find_rows<kTile>(p, blockIdx.y + blockIdx.z * gridDim.y);
-    if (s.g < 0) return;
-    g = s.g;
-    m0 = s.lo;
-    m_end = s.hi;
-    b1 = ceil_div(p.k, 32);
+    const Span s = find_tile(p, first, t, nt);
+    a.g = s.g;
+    if (s.g < 0) return a;
+    raster(t, ceil_div(s.hi - s.lo, C::BM), nt, tm, tn);
+    a.m0 = s.lo + tm * C::BM;
+    a.m_end = s.hi;
   }
-  m0 += (wave >> 1) * 32;
-  const int row = min(m0 + (lane & 31), m_end - 1), col = min(n0 + (lane & 31), p.n - 1);
-  const uint8_t* a = p.a + (int64_t)row * p.lda;
-  const uint8_t* as = p.a_scales + (int64_t)row * p.lda_scales;
-  const uint8_t* b = p.b + (int64_t)col * p.ldb;
-  const uint8_t* bs = p.b_scales + (int64_t)col * p.ldb_scales;
-  if constexpr (!kInner) {
-    b += g * p.b_stride;
-    bs += g * p.b_scales_stride;
-  }
-  f32x16 acc = {};
-  for (int k = b0; k < b1; k += 2) {
-    const int blk = k + (lane >> 5);
-    i32x8 av = {}, bv = {};
-    int sa = 127, sb = 127;
-    if (blk < b1) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(a + 16 * (int64_t)blk);
-      const u32x4 y = *reinterpret_cast<const u32x4*>(b + 16 * (int64_t)blk);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        av[i] = (int)x[i];
-        bv[i] = (int)y[i];
-      }
-      sa = as[blk];
-      sb = bs[blk];
+  a.n0 = tn * C::BN;
+  return a;
+}
+
+// Part s of S of the blocks [b0, b1), cut at multiples of four (so that no scale word is shared).
+__device__ __forceinline__ void take_part(int& b0, int& b1, int s, int S) {
+  const int start = b0 & ~3, words = max(ceil_div(b1 - start, 4), 0);
+  const int lo = start + 4 * (int)((int64_t)words * s / S), hi = start + 4 * (int)((int64_t)words * (s + 1) / S);
+  b0 = max(b0, lo);
+  b1 = min(b1, hi);
+}
+
+// Workgroup b takes tiles b, b + grid, ... of `total` (some past the last of a ragged rows form).  The next
+// tile's first stage is on its way while this one's results are stored.  kSplit: blockIdx.y is one of gridDim.y parts
+// of the inner dimension; its sums go to `parts`, tile after tile, for join_kernel.
+template <class C, int D, bool kInner, bool kVec, bool kSplit>
+__global__ void __launch_bounds__(C::NT, C::WAVES) gemm_tile_kernel(ggemm_mx4_gemm_t p, int total, float* parts) {
+  __shared__ __attribute__((aligned(128))) uint8_t tile_lds[C::SMEM];
+  using T = typename Elem<D>::T;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t ring = lds_addr(tile_lds);
+  const Groups<C::BM> first(p, 0, ceil_div(p.n, C::BN));
+  const Out o{p.alpha, p.beta, p.ldc};
+  int64_t it = blockIdx.x;
+  int number = 0;
+  auto next = [&]() {
+    Place a{-1, 0, 0, 0, 0, 0};
+    for (; a.g < 0 && it < total; it += gridDim.x) {
+      number = tile_number((int)it, total);
+      a = place_of<C, kInner>(p, first, number);
+      if constexpr (kSplit) take_part(a.b0, a.b1, blockIdx.y, gridDim.y);
     }
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, 4, 4, 0, sa, 0, sb);
+    return a;
+  };
+  auto source = [&](const Place& a) {
+    return Source<C>(p, p.b + (kInner ? 0 : a.g * p.b_stride), p.b_scales + (kInner ? 0 : a.g * p.b_scales_stride), a.m0,
+                     a.m_end - a.m0, a.n0, p.n - a.n0, wave, lane);
+  };
+  Place cur = next();
+  if (cur.g < 0) return;
+  Source<C> src = source(cur);
+  if (cur.b0 < cur.b1) load_first(src, ring, cur.b0, wave, lane);
+  landed();
+  while (true) {
+    lds_barrier();
+    f32x16 acc[C::FM][C::FN] = {};
+    if (cur.b0 < cur.b1) tile_products<C>(tile_lds, src, cur.b0, cur.b1, acc);
+    const int done = number;
+    const Place nxt = next();
+    if (nxt.g >= 0) {
+      src = source(nxt);
+      if (nxt.b0 < nxt.b1) load_first(src, ring, nxt.b0, wave, lane);
+    }
+    if constexpr (kSplit) {
+      float* const c = parts + ((int64_t)blockIdx.y * total + done) * C::BM * C::BN;
+      tile_store<C, GGEMM_F32, true>(tile_lds, Out{1.0f, 0.0f, C::BN}, c, C::BM, C::BN, acc);
+    } else {
+      T* const c = static_cast<T*>(p.c) + (kInner ? cur.g * p.c_stride : 0) + (int64_t)cur.m0 * p.ldc + cur.n0;
+      tile_store<C, D, kVec>(tile_lds, o, c, cur.m_end - cur.m0, p.n - cur.n0, acc);
+    }
+    if (nxt.g < 0) return;
+    cur = nxt;
   }
-  T* c = static_cast<T*>(p.c) + (kInner ? g * p.c_stride : 0);
-  const int j = n0 + (lane & 31);
-  if (j >= p.n) return;
+}
+
+// Sums of the `splits` parts of a tile, in order: a workgroup takes 8 rows of tile blockIdx.x.
+template <class C, int D, bool kInner>
+__global__ void __launch_bounds__(256) join_kernel(ggemm_mx4_gemm_t p, int total, int splits, const float* __restrict__ parts) {
+  using T = typename Elem<D>::T;
+  const Groups<C::BM> first(p, 0, ceil_div(p.n, C::BN));
+  const int t = blockIdx.x;
+  const Place a = place_of<C, kInner>(p, first, t);
+  if (a.g < 0) return;
+  const Out o{p.alpha, p.beta, p.ldc};
+  T* const c = static_cast<T*>(p.c) + (kInner ? a.g * p.c_stride : 0) + (int64_t)a.m0 * p.ldc + a.n0;
+  for (int i = threadIdx.x; i < 8 * C::BN; i += 256) {
+    const int row = 8 * blockIdx.y + i / C::BN, col = i % C::BN;
+    if (a.m0 + row >= a.m_end || a.n0 + col >= p.n) continue;
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += parts[((int64_t)s * total + t) * C::BM * C::BN + row * C::BN + col];
+    store_one(c + (int64_t)row * p.ldc + col, v, o);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// A workgroup computes 32 rows x 32 columns; its NW waves take every NW-th run of 256 codes (one line of every
+// row) straight from memory into registers, two runs ahead of the products, and join their sums in
+// LDS in order.  Bound: the bytes of B, which nobody else reads.
+struct FewTile {
+  static constexpr int BM = 32, BN = 32;
+};
+template <int D, bool kInner, bool kVec, int NW>
+__global__ void __launch_bounds__(64 * NW) gemm_few_kernel(ggemm_mx4_gemm_t p) {
+  using T = typename Elem<D>::T;
+  __shared__ f32x4 sums[NW][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const Place t = place_of<FewTile, kInner>(p, Groups<32>(p, 0, ceil_div(p.n, 32)), blockIdx.x);
+  if (t.g < 0) return;
+  const int row = min(t.m0 + (lane & 31), t.m_end - 1), col = min(t.n0 + (lane & 31), p.n - 1), nb = ceil_div(p.k, 32);
+  const uint8_t* const a = p.a + (int64_t)row * p.lda;
+  const uint8_t* const as = p.a_scales + (int64_t)row * p.lda_scales;
+  const uint8_t* const b = p.b + (kInner ? 0 : t.g * p.b_stride) + (int64_t)col * p.ldb;
+  const uint8_t* const bs = p.b_scales + (kInner ? 0 : t.g * p.b_scales_stride) + (int64_t)col * p.ldb_scales;
+  const int start = t.b0 & ~3, runs = t.b0 < t.b1 ? ceil_div(t.b1 - start, 8) : 0;
+  struct Run {
+    u32x4 a[4], b[4];
+    uint32_t sa, sb;
+  };
+  // run r: blocks past the row's last are read from the run's first, those outside [b0, b1) get scale byte 0
+  auto load = [&](int r) {
+    Run x;
+    const int first = start + 8 * r, at = first + 4 * half;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int i = m0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-    if (i < m_end) store_c<D>(p, c + (int64_t)i * p.ldc + j, acc[r]);
+    for (int s = 0; s < 4; ++s) {
+      const int64_t off = 16 * (int64_t)(at + s < nb ? at + s : first);
+      x.b[s] = *reinterpret_cast<const u32x4*>(b + off);
+      x.a[s] = *reinterpret_cast<const u32x4*>(a + off);
+    }
+    const int w = at < nb ? at : first;
+    const int lo = min(max(t.b0 - at, 0), 4), hi = min(max(t.b1 - at, 0), 4);
+    const uint64_t ones = 0xffffffffull;
+    const uint32_t keep = lo < hi ? (uint32_t)(ones << (8 * lo)) & (uint32_t)(ones >> (32 - 8 * hi)) : 0u;
+    x.sb = *reinterpret_cast<const uint32_t*>(bs + w) & keep;
+    x.sa = *reinterpret_cast<const uint32_t*>(as + w) & keep;
+    return x;
+  };
+  f32x16 acc = {};
+  auto products = [&](const Run& x) {
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[0]), frag(x.a[0]), acc, 4, 4, 0, (int)x.sb, 0, (int)x.sa);
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[1]), frag(x.a[1]), acc, 4, 4, 1, (int)x.sb, 1, (int)x.sa);
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[2]), frag(x.a[2]), acc, 4, 4, 2, (int)x.sb, 2, (int)x.sa);
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[3]), frag(x.a[3]), acc, 4, 4, 3, (int)x.sb, 3, (int)x.sa);
+  };
+  if (wave < runs) {
+    const int last = wave + (runs - 1 - wave) / NW * NW;   // loads past it repeat it
+    Run x = load(wave), y = load(min(wave + NW, last));
+    for (int r = wave; r <= last; r += NW) {
+      const Run z = load(min(r + 2 * NW, last));
+      products(x);
+      x = y;
+      y = z;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sums[wave][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  if (wave >= 4) return;
+  f32x4 v = sums[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) v += sums[w][wave][lane];
+  // C's transpose: row lane % 32, columns 8 wave + 4 (lane / 32) + 0 .. 3
+  const int i = t.m0 + (lane & 31), j = t.n0 + 8 * wave + 4 * half;
+  if (i >= t.m_end) return;
+  const Out o{p.alpha, p.beta, p.ldc};
+  T* const c = static_cast<T*>(p.c) + (kInner ? t.g * p.c_stride : 0) + (int64_t)i * p.ldc + j;
+  const float u[4] = {v[0], v[1], v[2], v[3]};
+  if (kVec && j + 4 <= p.n) {
+    store_run<T, 4>(c, u, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < p.n) store_one(c + e, u[e], o);
   }
 }
 
@@ -143,33 +566,78 @@ int64_t row_tiles(const ggemm_mx4_gemm_t& p, int tm) {
   return p.offsets ? (int64_t)p.m / tm + std::min(p.groups, p.m) : ceil_div(p.m, tm);
 }
 
+using Tile256 = Tile<256, 256, 2, 4>;
+using Tile128 = Tile<128, 128, 2, 2>;
+
+constexpr int64_t kMaxLd = 1 << 23;   // leading dimensions whose 256 rows stay within a 32-bit offset
+
+int64_t tiles_of(const ggemm_mx4_gemm_t& p, int bm, int bn) {
+  return (p.form == GGEMM_MX4_INNER ? (int64_t)ceil_div(p.m, bm) * p.groups : row_tiles(p, bm)) * ceil_div(p.n, bn);
+}
+
+// How a call is computed.
+struct Way {
+  int tile;     // 32 (few rows), 128 or 256
+  int splits;   // parts of the inner dimension
+  int64_t tiles;
+};
+Way way_of(const ggemm_mx4_gemm_t& p) {
+  const int64_t widest = std::max(std::max(p.lda, p.ldb), std::max(p.lda_scales, p.ldb_scales));
+  const bool inner = p.form == GGEMM_MX4_INNER;
+  if (widest > kMaxLd || (inner ? p.m <= 32 : p.m <= 32 * (int64_t)p.groups)) return Way{32, 1, tiles_of(p, 32, 32)};
+  const int64_t big = tiles_of(p, 256, 256);
+  if (big >= kCus) return Way{256, 1, big};
+  const int64_t tiles = tiles_of(p, 128, 128), runs = ceil_div(p.k, 256) / (inner ? p.groups : 1);
+  int splits = 1;
+  if (tiles < kCus) splits = (int)std::max<int64_t>(1, std::min(2 * kCus / tiles, runs / 4));
+  return Way{128, splits, tiles};
+}
+
+template <class C, int D, bool kInner, bool kVec>
+void launch_tiles(const ggemm_mx4_gemm_t& p, const Way& w, float* parts, hipStream_t s) {
+  if (w.splits > 1) {
+    gemm_tile_kernel<C, D, kInner, kVec, true><<<dim3((unsigned)w.tiles, w.splits), C::NT, 0, s>>>(p, (int)w.tiles, parts);
+    join_kernel<C, D, kInner><<<dim3((unsigned)w.tiles, C::BM / 8), 256, 0, s>>>(p, (int)w.tiles, w.splits, parts);
+  } else {
+    const int64_t at_once = (int64_t)kCus * 4 * C::WAVES / C::NW;
+    gemm_tile_kernel<C, D, kInner, kVec, false>
+        <<<(unsigned)std::min(w.tiles, at_once), C::NT, 0, s>>>(p, (int)w.tiles, nullptr);
+  }
+}
+
 }  // namespace
 
 size_t mx4_gemm_workspace(const ggemm_mx4_gemm_t* p) {
-  if (!gemm_ok(p)) return 0;
-  return 16;
+  if (!gemm_ok(p) || p->m == 0 || p->n == 0) return 0;
+  const Way w = way_of(*p);
+  return w.splits > 1 ? (size_t)w.tiles * w.splits * 128 * 128 * sizeof(float) : 0;
 }
 
 int mx4_gemm(const ggemm_mx4_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
   if (!gemm_ok(p)) return GGEMM_ERR_INVALID;
   if (p->m == 0 || p->n == 0) return GGEMM_OK;
-  if (ws_bytes < mx4_gemm_workspace(p)) return GGEMM_ERR_WORKSPACE;
-  if (!ws || !aligned(ws, 16)) return GGEMM_ERR_INVALID;
-  const int nt = ceil_div(p->n, kTile);
-  bool fits = true;
+  const size_t need = mx4_gemm_workspace(p);
+  if (ws_bytes < need) return GGEMM_ERR_WORKSPACE;
+  if (need && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
+  const Way w = way_of(*p);
+  if (w.tiles >= (1 << 23)) return GGEMM_ERR_INVALID;   // 512 threads each: a grid of 2^32
+  const size_t es = elem_bytes(p->dtype);
+  const bool vec = aligned(p->c, 16) && p->ldc * es % 16 == 0 && p->c_stride * es % 16 == 0;
   with_elem(p->dtype, [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    if (p->form == GGEMM_MX4_INNER) {
-      const int mt = ceil_div(p->m, kTile);
-      if (mt > 65535) { fits = false; return; }
-      gemm_simple_kernel<D, true><<<dim3(nt, mt, p->groups), kThreads, 0, s>>>(*p);
-    } else {
-      const int64_t mt = row_tiles(*p, kTile);
-      const int64_t z = (mt + 32767) / 32768;
-      gemm_simple_kernel<D, false><<<dim3(nt, (unsigned)std::min<int64_t>(mt, 32768), (unsigned)z), kThreads, 0, s>>>(*p);
-    }
+    auto go = [&](auto inner, auto v) {
+      constexpr int D = decltype(d)::value;
+      constexpr bool I = decltype(inner)::value, V = decltype(v)::value;
+      float* const parts = static_cast<float*>(ws);
+      if (w.tile == 256) launch_tiles<Tile256, D, I, V>(*p, w, parts, s);
+      else if (w.tile == 128) launch_tiles<Tile128, D, I, V>(*p, w, parts, s);
+      else if (w.tiles < kCus && p->k >= 4096) gemm_few_kernel<D, I, V, 16><<<(unsigned)w.tiles, 1024, 0, s>>>(*p);
+      else gemm_few_kernel<D, I, V, 4><<<(unsigned)w.tiles, 256, 0, s>>>(*p);
+    };
+    using std::true_type;
+    using std::false_type;
+    if (p->form == GGEMM_MX4_INNER) vec ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
+    else vec ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
   });
-  if (!fits) return GGEMM_ERR_INVALID;
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
 }
 

@@ -115,11 +115,11 @@ struct Tile {
   static constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;
   static constexpr int WIN = (BM + BN) * 32;                 // scales of a window
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;   // 1 KB pieces of A and B per wave
-  static constexpr int PS = (BM + BN) / 32 / NW;             // 1 KB pieces of a window per wave
+  static constexpr int NS = (BM + BN) / 32, PS = (NS + NW - 1) / NW;   // 1 KB pieces of a window, and per wave
   static constexpr int EPI = 32 * FN * 32 * 4;               // epilogue bytes per wave, in the second slot
   static constexpr int SMEM = 2 * STAGE + 2 * WIN;
-  static constexpr int WAVES = BM * BN >= 256 * 256 ? NW / 4 : 2;   // per SIMD: one workgroup of 256 x 256 a compute unit, else two
-  static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && (BM + BN) / 32 % NW == 0 && NW % 2 == 0, "pieces");
+  static constexpr int WAVES = 163840 / SMEM * NW / 4;       // per SIMD, as many workgroups as LDS holds
+  static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && NW % 2 == 0, "pieces");
   static_assert(NW * EPI <= STAGE, "epilogue");
 };
 
@@ -188,7 +188,7 @@ struct Source {
 #pragma unroll
       for (int q = 0; q < C::PS; ++q) {
         const int piece = wave + C::NW * q;
-        dma16((piece < C::BM / 32 ? as : bs) + blk, vs[q], slot + 1024 * piece);
+        if (C::NS % C::NW == 0 || piece < C::NS) dma16((piece < C::BM / 32 ? as : bs) + blk, vs[q], slot + 1024 * piece);
       }
     } else {
 #pragma unroll 1
@@ -463,73 +463,74 @@ __global__ void __launch_bounds__(256) join_kernel(ggemm_mx4_gemm_t p, int total
 }
 
 // ---------------------------------------------------------------- few rows
-// A workgroup computes 32 rows x 32 columns; its NW waves take every NW-th run of 256 codes (one line of every
-// row) straight from memory into registers, two runs ahead of the products, and join their sums in
-// LDS in order.  Bound: the bytes of B, which nobody else reads.
+// A workgroup computes 16 rows x 32 columns; its NW waves take every NW-th run of 512 codes straight from
+// memory into registers and join their sums in LDS in order; the waves of a compute unit (24) cover each
+// other's latency.  Products are v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds the block l / 16 of four of
+// row l % 16, so that a load takes 64 bytes side by side of each of 16 rows (the 32 x 32 x 64 form takes
+// 16 bytes twice of 32 rows, four times the line accesses).  A run's 16 scale bytes of a row are one load of
+// every lane of the row, which picks its byte of each word.
+// Bound: the bytes of B, which nobody else reads.
 struct FewTile {
-  static constexpr int BM = 32, BN = 32;
+  static constexpr int BM = 16, BN = 32;
 };
 template <int D, bool kInner, bool kVec, int NW>
-__global__ void __launch_bounds__(64 * NW) gemm_few_kernel(ggemm_mx4_gemm_t p) {
+__global__ void __launch_bounds__(64 * NW, 4) gemm_few_kernel(ggemm_mx4_gemm_t p) {
   using T = typename Elem<D>::T;
-  __shared__ f32x4 sums[NW][4][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const Place t = place_of<FewTile, kInner>(p, Groups<32>(p, 0, ceil_div(p.n, 32)), blockIdx.x);
+  __shared__ f32x4 sums[NW][2][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+  const Place t = place_of<FewTile, kInner>(p, Groups<FewTile::BM>(p, 0, ceil_div(p.n, FewTile::BN)), blockIdx.x);
   if (t.g < 0) return;
-  const int row = min(t.m0 + (lane & 31), t.m_end - 1), col = min(t.n0 + (lane & 31), p.n - 1), nb = ceil_div(p.k, 32);
-  const uint8_t* const a = p.a + (int64_t)row * p.lda;
-  const uint8_t* const as = p.a_scales + (int64_t)row * p.lda_scales;
-  const uint8_t* const b = p.b + (kInner ? 0 : t.g * p.b_stride) + (int64_t)col * p.ldb;
-  const uint8_t* const bs = p.b_scales + (kInner ? 0 : t.g * p.b_scales_stride) + (int64_t)col * p.ldb_scales;
-  const int start = t.b0 & ~3, runs = t.b0 < t.b1 ? ceil_div(t.b1 - start, 8) : 0;
-  struct Run {
-    u32x4 a[4], b[4];
-    uint32_t sa, sb;
-  };
-  // run r: blocks past the row's last are read from the run's first, those outside [b0, b1) get scale byte 0
-  auto load = [&](int r) {
-    Run x;
-    const int first = start + 8 * r, at = first + 4 * half;
+  const int nb = ceil_div(p.k, 32);
+  const int row = min(t.m0 + (lane & 15), t.m_end - 1);
+  const int col0 = min(t.n0 + (lane & 15), p.n - 1), col1 = min(t.n0 + 16 + (lane & 15), p.n - 1);
+  const uint8_t* const b = p.b + (kInner ? 0 : t.g * p.b_stride);
+  const uint8_t* const bs = p.b_scales + (kInner ? 0 : t.g * p.b_scales_stride);
+  const uint8_t* const codes[3] = {b + (int64_t)col0 * p.ldb, b + (int64_t)col1 * p.ldb, p.a + (int64_t)row * p.lda};
+  const uint8_t* const scales[3] = {bs + (int64_t)col0 * p.ldb_scales, bs + (int64_t)col1 * p.ldb_scales,
+                                    p.a_scales + (int64_t)row * p.lda_scales};
+  const int start = t.b0 & ~3, runs = t.b0 < t.b1 ? ceil_div(t.b1 - start, 16) : 0;
+  f32x4 acc[2] = {};
+  for (int r = wave; r < runs; r += NW) {
+    const int first = start + 16 * r;   // blocks past the row's last are read from the run's first
+    u32x4 c[3][4], sc[3];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int64_t off = 16 * (int64_t)(at + s < nb ? at + s : first);
-      x.b[s] = *reinterpret_cast<const u32x4*>(b + off);
-      x.a[s] = *reinterpret_cast<const u32x4*>(a + off);
+      const int at = first + 4 * s + quarter;
+      const int64_t off = 16 * (int64_t)(at < nb ? at : first);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) c[i][s] = *reinterpret_cast<const u32x4*>(codes[i] + off);
     }
-    const int w = at < nb ? at : first;
-    const int lo = min(max(t.b0 - at, 0), 4), hi = min(max(t.b1 - at, 0), 4);
-    const uint64_t ones = 0xffffffffull;
-    const uint32_t keep = lo < hi ? (uint32_t)(ones << (8 * lo)) & (uint32_t)(ones >> (32 - 8 * hi)) : 0u;
-    x.sb = *reinterpret_cast<const uint32_t*>(bs + w) & keep;
-    x.sa = *reinterpret_cast<const uint32_t*>(as + w) & keep;
-    return x;
-  };
-  f32x16 acc = {};
-  auto products = [&](const Run& x) {
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[0]), frag(x.a[0]), acc, 4, 4, 0, (int)x.sb, 0, (int)x.sa);
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[1]), frag(x.a[1]), acc, 4, 4, 1, (int)x.sb, 1, (int)x.sa);
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[2]), frag(x.a[2]), acc, 4, 4, 2, (int)x.sb, 2, (int)x.sa);
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(frag(x.b[3]), frag(x.a[3]), acc, 4, 4, 3, (int)x.sb, 3, (int)x.sa);
-  };
-  if (wave < runs) {
-    const int last = wave + (runs - 1 - wave) / NW * NW;   // loads past it repeat it
-    Run x = load(wave), y = load(min(wave + NW, last));
-    for (int r = wave; r <= last; r += NW) {
-      const Run z = load(min(r + 2 * NW, last));
-      products(x);
-      x = y;
-      y = z;
+    if (first + 16 <= nb) {
+      struct __attribute__((packed, aligned(4))) Words { u32x4 w; };
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sc[i] = reinterpret_cast<const Words*>(scales[i] + first)->w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) sc[i][s] = *reinterpret_cast<const uint32_t*>(scales[i] + (first + 4 * s < nb ? first + 4 * s : first));
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int at = first + 4 * s + quarter;
+      const uint32_t keep = at >= t.b0 && at < t.b1 ? 0xffu : 0u;   // blocks outside [b0, b1) get scale byte 0
+      uint32_t sb[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sb[i] = sc[i][s] >> (8 * quarter) & keep;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(frag(c[j][s]), frag(c[2][s]), acc[j], 4, 4, 0, (int)sb[j], 0, (int)sb[2]);
     }
   }
-#pragma unroll
-  for (int q = 0; q < 4; ++q) sums[wave][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  sums[wave][0][lane] = acc[0];
+  sums[wave][1][lane] = acc[1];
   __syncthreads();
-  if (wave >= 4) return;
+  if (wave >= 2) return;
   f32x4 v = sums[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < NW; ++w) v += sums[w][wave][lane];
-  // C's transpose: row lane % 32, columns 8 wave + 4 (lane / 32) + 0 .. 3
-  const int i = t.m0 + (lane & 31), j = t.n0 + 8 * wave + 4 * half;
+  // C's transpose: row lane % 16, columns 16 wave + 4 (lane / 16) + 0 .. 3
+  const int i = t.m0 + (lane & 15), j = t.n0 + 16 * wave + 4 * quarter;
   if (i >= t.m_end) return;
   const Out o{p.alpha, p.beta, p.ldc};
   T* const c = static_cast<T*>(p.c) + (kInner ? t.g * p.c_stride : 0) + (int64_t)i * p.ldc + j;
@@ -568,6 +569,7 @@ int64_t row_tiles(const ggemm_mx4_gemm_t& p, int tm) {
 
 using Tile256 = Tile<256, 256, 2, 4>;
 using Tile128 = Tile<128, 128, 2, 2>;
+using Tile32 = Tile<32, 128, 1, 4>;
 
 constexpr int64_t kMaxLd = 1 << 23;   // leading dimensions whose 256 rows stay within a 32-bit offset
 
@@ -577,20 +579,32 @@ int64_t tiles_of(const ggemm_mx4_gemm_t& p, int bm, int bn) {
 
 // How a call is computed.
 struct Way {
-  int tile;     // 32 (few rows), 128 or 256
+  int tile;     // rows of a tile: 16, 32, 128 or 256
   int splits;   // parts of the inner dimension
   int64_t tiles;
 };
+// Rules on the sizes that the host knows (the groups' own are on the device).  Measured, us:
+//   few rows or 32 x 128 tiles: by what the card holds at once.  4096 x 2048 weights, one row in each group: 1
+//   group 4.2 / 6.5, 8 groups (256 tiles) 8.3 / 8.5, 16 groups 15.3 / 13.6
+//   32 x 128 or 128 x 128 tiles: up to 64 rows a group on average.  64 groups of 4096 x 2048: 64 rows each 66 /
+//   80, 128 rows 117 / 88
+//   256 x 256 tiles (one workgroup a compute unit) as soon as there is one for every compute unit.
+//   32768 rows: %%BIG%%
+//   parts of the inner dimension: fewer tiles than compute units, so that two tiles' worth per compute unit
+//   run, each part four stages or more.  64 rows, 1024 x 16384: 27 / %%SPLIT%%
 Way way_of(const ggemm_mx4_gemm_t& p) {
   const int64_t widest = std::max(std::max(p.lda, p.ldb), std::max(p.lda_scales, p.ldb_scales));
   const bool inner = p.form == GGEMM_MX4_INNER;
-  if (widest > kMaxLd || (inner ? p.m <= 32 : p.m <= 32 * (int64_t)p.groups)) return Way{32, 1, tiles_of(p, 32, 32)};
-  const int64_t big = tiles_of(p, 256, 256);
-  if (big >= kCus) return Way{256, 1, big};
-  const int64_t tiles = tiles_of(p, 128, 128), runs = ceil_div(p.k, 256) / (inner ? p.groups : 1);
-  int splits = 1;
-  if (tiles < kCus) splits = (int)std::max<int64_t>(1, std::min(2 * kCus / tiles, runs / 4));
-  return Way{128, splits, tiles};
+  const int64_t groups = inner ? 1 : p.groups, thin = tiles_of(p, 32, 128);
+  if (widest > kMaxLd || (p.m <= 16 * groups && thin <= kCus)) return Way{16, 1, tiles_of(p, 16, 32)};
+  Way w{32, 1, thin};
+  if (p.m > 64 * groups) {
+    w = Way{256, 1, tiles_of(p, 256, 256)};
+    if (w.tiles < kCus) w = Way{128, 1, tiles_of(p, 128, 128)};
+  }
+  const int64_t runs = ceil_div(p.k, 256) / (inner ? p.groups : 1);
+  if (w.tiles < kCus) w.splits = (int)std::max<int64_t>(1, std::min(2 * kCus / w.tiles, runs / 4));
+  return w;
 }
 
 template <class C, int D, bool kInner, bool kVec>
@@ -610,7 +624,7 @@ void launch_tiles(const ggemm_mx4_gemm_t& p, const Way& w, float* parts, hipStre
 size_t mx4_gemm_workspace(const ggemm_mx4_gemm_t* p) {
   if (!gemm_ok(p) || p->m == 0 || p->n == 0) return 0;
   const Way w = way_of(*p);
-  return w.splits > 1 ? (size_t)w.tiles * w.splits * 128 * 128 * sizeof(float) : 0;
+  return w.splits > 1 ? (size_t)w.tiles * w.splits * w.tile * 128 * sizeof(float) : 0;
 }
 
 int mx4_gemm(const ggemm_mx4_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
@@ -629,6 +643,7 @@ int mx4_gemm(const ggemm_mx4_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s
       constexpr bool I = decltype(inner)::value, V = decltype(v)::value;
       float* const parts = static_cast<float*>(ws);
       if (w.tile == 256) launch_tiles<Tile256, D, I, V>(*p, w, parts, s);
+      else if (w.tile == 32) launch_tiles<Tile32, D, I, V>(*p, w, parts, s);
       else if (w.tile == 128) launch_tiles<Tile128, D, I, V>(*p, w, parts, s);
       else if (w.tiles < kCus && p->k >= 4096) gemm_few_kernel<D, I, V, 16><<<(unsigned)w.tiles, 1024, 0, s>>>(*p);
       else gemm_few_kernel<D, I, V, 4><<<(unsigned)w.tiles, 256, 0, s>>>(*p);

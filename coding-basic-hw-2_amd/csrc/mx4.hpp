@@ -54,4 +54,14 @@ __device__ __forceinline__ uint32_t dpp(uint32_t x) {
 constexpr int kDppXor1 = 0xb1, kDppXor2 = 0x4e;      // quad_perm [1,0,3,2] and [2,3,0,1]
 constexpr int kDppHalfMirror = 0x141, kDppMirror = 0x140;   // lane i <-> 7 - i and 15 - i
 
+constexpr int kChunk = 32;   // consecutive tiles that one XCD gets
+// The tile of workgroup b: workgroups go to the XCDs in turn, so runs of kChunk tiles that share rows of A and B
+// share an L2.  Ragged ends of 8 kChunk tiles keep their number.
+__device__ __forceinline__ int tile_number(int b, int total) {
+  constexpr int span = kXcds * kChunk;
+  if (b >= total / span * span) return b;
+  const int q = b / kXcds;
+  return q / kChunk * span + b % kXcds * kChunk + q % kChunk;
+}
+
 }  // namespace ggemm

@@ -335,15 +335,6 @@ __device__ __forceinline__ void tile_store(uint8_t* lds, const Out& o, typename 
   }
 }
 
-constexpr int kChunk = 32;   // consecutive tiles that one XCD gets
-// The tile of workgroup b: workgroups go to the XCDs in turn, so runs of kChunk tiles that share rows of A and B
-// share an L2.  Ragged ends of 8 kChunk tiles keep their number.
-__device__ __forceinline__ int tile_number(int b, int total) {
-  constexpr int span = kXcds * kChunk;
-  if (b >= total / span * span) return b;
-  const int q = b / kXcds;
-  return q / kChunk * span + b % kXcds * kChunk + q % kChunk;
-}
 // Tile t of a rows x cols arrangement of tiles, in bands of 4 rows, down each band's columns.
 __device__ __forceinline__ void raster(int t, int rows, int cols, int& r, int& c) {
   const int band = t / (4 * cols), r0 = 4 * band, h = min(4, rows - r0), l = t - r0 * cols;

@@ -3,9 +3,11 @@
 // Per block of 32 values: s = max(exponent(max |v|) - 2, 0) as a biased byte, codes = v / 2^(s - 127) on the
 // grid 0, 0.5, 1, 1.5, 2, 3, 4, 6.  The quotient by a power of two is exact, so the conversion
 // instruction (v_cvt_scalef32_pk_fp4_*: two values a time, nearest, ties to even, saturating) rounds
-// once; the largest magnitude lands in [4, 8).
+// once; the largest magnitude lands in [4, 8).  Magnitudes are compared as integers with the sign bit
+// cleared (two 16-bit ones in a word), which orders them with NaN above Inf above all else.
 // Along the rows a lane holds 8 consecutive values and the four lanes of a block exchange their
-// maxima; down the columns a lane holds a block of its own column.
+// maxima.  Down the columns a workgroup turns a tile through LDS: it is read once, quantised along
+// the rows on the way if that is asked too, and a lane then walks down a block of its columns.
 // Bound: HBM.
 #include <algorithm>
 #include <type_traits>
@@ -17,36 +19,73 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Eight consecutive values of a row.
+// Results are stored non-temporally: they would push what is still to be read out of L2.  32768 x 4096 bf16: along
+// the rows 63 -> 49 us, down the columns 90 -> 69, back to values 117 -> 51.
+template <class V>
+__device__ __forceinline__ void put(V v, void* p) {
+  __builtin_nontemporal_store(v, static_cast<V*>(p));
+}
+
+// Eight consecutive values: two words of four, or four words of two.
 template <int D>
 struct Oct {
   typename Elem<D>::T v[8];
 };
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
+// The larger magnitudes of two words of two 16-bit values, sign bits cleared.
+__device__ __forceinline__ uint32_t max_mag2(uint32_t m, uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+// A 16-bit magnitude (low half) as the bits of a 32-bit float.
 template <int D>
-__device__ __forceinline__ uint32_t mag_bits(typename Elem<D>::T v) {   // |v| as the bits of a 32-bit float
-  return __float_as_uint((float)v) & 0x7fffffffu;
+__device__ __forceinline__ uint32_t wide_mag(uint32_t m) {
+  if constexpr (D == GGEMM_BF16) return m << 16;
+  else return __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)m));
+}
+// The largest of 8 magnitudes (16-bit: both halves of a word; 32-bit: bits).
+template <int D>
+__device__ __forceinline__ uint32_t oct_mag(const Oct<D>& o) {
+  uint32_t m = 0;
+  if constexpr (D == GGEMM_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(o.v[i]) & 0x7fffffffu);
+  } else {
+    const u32x4 w = __builtin_bit_cast(u32x4, o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max_mag2(m, w[i]);
+    m = max(m & 0xffffu, m >> 16);
+  }
+  return m;
+}
+// Scale byte of a block from the largest magnitude that oct_mag gave.
+template <int D>
+__device__ __forceinline__ uint32_t block_scale(uint32_t m) {
+  if constexpr (D == GGEMM_F32) return mx4_scale_byte(m);
+  else return mx4_scale_byte(wide_mag<D>(m));
 }
 
+// A byte of codes of two values (word: two 16-bit values) into byte I of r.
+template <int D, int I>
+__device__ __forceinline__ uint32_t code2(uint32_t r, uint32_t w, float scale) {
+  if constexpr (D == GGEMM_BF16) return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w), scale, I);
+  else return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, w), scale, I);
+}
 // codes of 8 values, the first in the low four bits
 template <int D>
-__device__ __forceinline__ uint32_t codes8(const typename Elem<D>::T (&v)[8], float scale) {
+__device__ __forceinline__ uint32_t codes8(const Oct<D>& o, float scale) {
   uint32_t r = 0;
   if constexpr (D == GGEMM_F32) {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
-  } else if constexpr (D == GGEMM_BF16) {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2{v[0], v[1]}, scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2{v[2], v[3]}, scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2{v[4], v[5]}, scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, bf16x2{v[6], v[7]}, scale, 3);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, o.v[0], o.v[1], scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, o.v[2], o.v[3], scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, o.v[4], o.v[5], scale, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, o.v[6], o.v[7], scale, 3);
   } else {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2{v[0], v[1]}, scale, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2{v[2], v[3]}, scale, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2{v[4], v[5]}, scale, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, f16x2{v[6], v[7]}, scale, 3);
+    const u32x4 w = __builtin_bit_cast(u32x4, o);
+    r = code2<D, 0>(r, w[0], scale);
+    r = code2<D, 1>(r, w[1], scale);
+    r = code2<D, 2>(r, w[2], scale);
+    r = code2<D, 3>(r, w[3], scale);
   }
   return r;
 }
@@ -57,29 +96,36 @@ __device__ __forceinline__ int64_t source_row(const ggemm_mx4_quant_t& q, int ro
   return r >= 0 && r < q.x_rows ? r : -1;
 }
 
-// Chunk `chunk` of a row; the four lanes of a block call it together.
+// Columns 8 chunk .. of a row (zeros past its end and for a row that does not exist).
 template <int D, bool kVec>
-__device__ __forceinline__ void quant_chunk(const ggemm_mx4_quant_t& q, int64_t row, int chunk) {
+__device__ __forceinline__ Oct<D> load_chunk(const ggemm_mx4_quant_t& q, int64_t src, int chunk) {
   using T = typename Elem<D>::T;
-  const int64_t src = source_row(q, (int)row);
   const int c0 = 8 * chunk;
-  Oct<D> o;
   const T* p = static_cast<const T*>(q.x) + src * q.ld + c0;
+  Oct<D> o;
   if (kVec && src >= 0 && c0 + 8 <= q.cols) {
     o = *reinterpret_cast<const Oct<D>*>(__builtin_assume_aligned(p, 16));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.v[i] = src >= 0 && c0 + i < q.cols ? p[i] : (T)0.0f;
   }
-  uint32_t amax = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = max(amax, mag_bits<D>(o.v[i]));
-  amax = max(amax, dpp<kDppXor1>(amax));
-  amax = max(amax, dpp<kDppXor2>(amax));
-  const uint32_t s = mx4_scale_byte(amax);
-  const uint32_t w = s == 255u ? 0u : codes8<D>(o.v, mx4_scale(s));
-  *reinterpret_cast<uint32_t*>(q.codes + row * q.ld_codes + 4 * chunk) = w;
-  if ((chunk & 3) == 0) q.scales[row * q.ld_scales + (chunk >> 2)] = (uint8_t)s;
+  return o;
+}
+// Its codes, and the block's scale byte; the four lanes of a block call it together.
+template <int D>
+__device__ __forceinline__ uint32_t code_chunk(const Oct<D>& o, uint32_t& s) {
+  uint32_t m = oct_mag<D>(o);
+  m = max(m, dpp<kDppXor1>(m));
+  m = max(m, dpp<kDppXor2>(m));
+  s = block_scale<D>(m);
+  return s == 255u ? 0u : codes8<D>(o, mx4_scale(s));
+}
+template <int D>
+__device__ __forceinline__ void store_chunk(const ggemm_mx4_quant_t& q, int64_t row, int chunk, const Oct<D>& o) {
+  uint32_t s;
+  const uint32_t w = code_chunk<D>(o, s);
+  put(w, q.codes + row * q.ld_codes + 4 * chunk);
+  if ((chunk & 3) == 0) put((uint8_t)s, q.scales + row * q.ld_scales + (chunk >> 2));
 }
 
 // Blocks along the rows.  A workgroup of 256 lanes covers cx chunks of 8 columns (cx a power of two)
@@ -89,86 +135,225 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(ggemm_mx4_quant_t 
   const int chunks = 4 * ceil_div(q.cols, 32);
   const int chunk = (blockIdx.y << log_cx) + (threadIdx.x & ((1 << log_cx) - 1));
   if (chunk >= chunks) return;   // whole blocks: four lanes together
-  for (int64_t row = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx); row < q.rows;
-       row += (int64_t)gridDim.x << (8 - log_cx))
-    quant_chunk<D, kVec>(q, row, chunk);
+  const int64_t step = (int64_t)gridDim.x << (8 - log_cx);
+  int64_t row = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx);
+  for (; row + step < q.rows; row += 2 * step) {   // two rows' loads before their stores
+    const int64_t s0 = source_row(q, (int)row), s1 = source_row(q, (int)(row + step));
+    const Oct<D> a = load_chunk<D, kVec>(q, s0, chunk), b = load_chunk<D, kVec>(q, s1, chunk);
+    store_chunk<D>(q, row, chunk, a);
+    store_chunk<D>(q, row + step, chunk, b);
+  }
+  if (row < q.rows) store_chunk<D>(q, row, chunk, load_chunk<D, kVec>(q, source_row(q, (int)row), chunk));
 }
 
-// Block b (32 rows) of column col.
+// Blocks down the columns, and along the rows too with kAlong: a workgroup takes a tile of kRows rows (a
+// memory line of codes of every column; half of one for 32-bit values) and 128 columns through 64 KB of LDS.
+// Codes and scales of both kinds go back through LDS and leave as 16 and 4 bytes a lane, runs of 128 (64)
+// bytes.  A tile has 4 scale bytes of a row; runs of tiles side by side go to one XCD and these bytes are stored
+// the ordinary way, so that its L2 makes lines of them (32768 x 4096 bf16, both kinds: 127 us as they come, 104;
+// the two kinds one after the other 118).  Half the tile and twice the workgroups per compute unit is slower
+// by 5 to 20 %.
 template <int D>
-__device__ __forceinline__ void quant_column_block(const ggemm_mx4_quant_t& q, int64_t col, int64_t b) {
+struct Turn {
+  static constexpr int kRows = D == GGEMM_F32 ? 128 : 256, kCols = 128, kThreads = 512;
+  static constexpr int kLanes = kCols / 8;   // lanes of a row
+  static constexpr int kBlocks = kRows / 32, kRowBytes = kCols * (int)sizeof(typename Elem<D>::T);
+};
+template <int D, bool kVec, bool kAlong>
+__global__ void __launch_bounds__(Turn<D>::kThreads, 4) quant_turn_kernel(ggemm_mx4_quant_t q) {
   using T = typename Elem<D>::T;
-  const int64_t r0 = 32 * b;
-  T v[32];
-  uint32_t amax = 0;
+  using U = Turn<D>;
+  constexpr int B = U::kBlocks;
+  constexpr int kAlongCodes = U::kCols * B * 16;            // the rows' codes in the tile's LDS, after the columns'
+  constexpr int kPer = D == GGEMM_F32 ? 1 : 2;              // columns of a lane
+  constexpr int kStep = U::kThreads / U::kLanes, kN = U::kRows / kStep;   // rows at a time, rows of a lane
+  __shared__ __attribute__((aligned(16))) uint8_t tile[U::kRows * U::kRowBytes];
+  __shared__ __attribute__((aligned(4))) uint8_t down_scale[U::kCols][B], along_scale[U::kRows][4];
+  const int tid = threadIdx.x, lane_row = tid / U::kLanes, lane_chunk = tid % U::kLanes;
+  const int tiles_c = ceil_div(q.cols, U::kCols);
+  const int64_t tiles = (int64_t)ceil_div(q.rows, U::kRows) * tiles_c;
+  for (int64_t it = blockIdx.x; it < tiles; it += gridDim.x) {
+    const int64_t t = kAlong ? tile_number((int)it, (int)tiles) : it;
+    const int64_t r0 = t / tiles_c * U::kRows;
+    const int c0 = (int)(t % tiles_c) * U::kCols;
+    const int rows_left = (int)min((int64_t)U::kRows, q.rows - r0), cols_left = min(U::kCols, q.cols - c0);
+    uint32_t wa[kAlong ? kN : 1], sa[kAlong ? kN : 1];
+    {
+      Oct<D> o[kN];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    v[i] = (T)0.0f;
-    if (r0 + i < q.rows) {
-      const int64_t src = source_row(q, (int)(r0 + i));
-      if (src >= 0) v[i] = static_cast<const T*>(q.x)[src * q.ld + col];
+      for (int i = 0; i < kN; ++i) {
+        const int r = i * kStep + lane_row;
+        o[i] = load_chunk<D, kVec>(q, r < rows_left ? source_row(q, (int)(r0 + r)) : -1, c0 / 8 + lane_chunk);
+      }
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        *reinterpret_cast<Oct<D>*>(tile + (i * kStep + lane_row) * U::kRowBytes + lane_chunk * (int)sizeof o[i]) = o[i];
+        if constexpr (kAlong) wa[i] = code_chunk<D>(o[i], sa[i]);
+      }
     }
-    amax = max(amax, mag_bits<D>(v[i]));
-  }
-  const uint32_t s = mx4_scale_byte(amax);
-  u32x4 w = {0u, 0u, 0u, 0u};
-  if (s != 255u) {
+    __syncthreads();
+    u32x4 w[kPer];
+    uint32_t sc[kPer];
+    const int col = kPer * (tid % (U::kCols / kPer)), blk = tid / (U::kCols / kPer);
+    if constexpr (D == GGEMM_F32) {
+      const T* p = reinterpret_cast<const T*>(tile) + 32 * blk * U::kCols + col;
+      Oct<D> y[4];
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      T u[8];
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = v[8 * i + j];
-      w[i] = codes8<D>(u, mx4_scale(s));
+        for (int j = 0; j < 8; ++j) y[i].v[j] = p[(8 * i + j) * U::kCols];
+        m = max(m, oct_mag<D>(y[i]));
+      }
+      sc[0] = block_scale<D>(m);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[0][i] = sc[0] == 255u ? 0u : codes8<D>(y[i], mx4_scale(sc[0]));
+    } else {                          // two columns side by side in a word
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(tile) + 32 * blk * (U::kCols / 2) + col / 2;
+      uint32_t x[32], m = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        x[i] = p[i * (U::kCols / 2)];
+        m = max_mag2(m, x[i]);
+      }
+      sc[0] = block_scale<D>(m & 0xffffu);
+      sc[1] = block_scale<D>(m >> 16);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float scale = mx4_scale(sc[c]);
+        const uint32_t pick = c ? 0x07060302u : 0x05040100u;   // the column's halves of two rows
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t r = 0;
+          r = code2<D, 0>(r, __builtin_amdgcn_perm(x[8 * i + 1], x[8 * i], pick), scale);
+          r = code2<D, 1>(r, __builtin_amdgcn_perm(x[8 * i + 3], x[8 * i + 2], pick), scale);
+          r = code2<D, 2>(r, __builtin_amdgcn_perm(x[8 * i + 5], x[8 * i + 4], pick), scale);
+          r = code2<D, 3>(r, __builtin_amdgcn_perm(x[8 * i + 7], x[8 * i + 6], pick), scale);
+          w[c][i] = sc[c] == 255u ? 0u : r;
+        }
+      }
     }
+    __syncthreads();
+    // the columns' codes: [column][block] of 16 bytes, the block's place exchanged by the column against bank conflicts
+    auto place = [&](int c, int b) { return tile + (c * B + (b ^ (c / kPer & (B - 1)))) * 16; };
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      *reinterpret_cast<u32x4*>(place(col + c, blk)) = w[c];
+      down_scale[col + c][blk] = (uint8_t)sc[c];
+    }
+    if constexpr (kAlong) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int r = i * kStep + lane_row;
+        *reinterpret_cast<uint32_t*>(tile + kAlongCodes + r * 64 + 4 * lane_chunk) = wa[i];
+        if ((lane_chunk & 3) == 0) along_scale[r][lane_chunk / 4] = (uint8_t)sa[i];
+      }
+    }
+    __syncthreads();
+    // up to four scale bytes of a row or column; a word's bytes past the last block are not written
+    auto put_scales = [&](const uint8_t* from, uint8_t* to, int left, auto stream) {
+      if (left < 4) {
+        for (int i = 0; i < left; ++i) to[i] = from[i];
+      } else if (decltype(stream)::value) {
+        put(*reinterpret_cast<const uint32_t*>(from), to);
+      } else {
+        *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+      }
+    };
+    const int blocks_down = ceil_div(rows_left, 32), blocks_along = ceil_div(cols_left, 32);
+    for (int i = tid; i < U::kCols * B; i += U::kThreads) {
+      const int c = i / B, b = i % B;
+      if (c < cols_left && b < blocks_down) put(*reinterpret_cast<const u32x4*>(place(c, b)), q.codes_t + (int64_t)(c0 + c) * q.ld_codes_t + r0 / 2 + 16 * b);
+    }
+    for (int i = tid; i < U::kCols * B / 4; i += U::kThreads) {
+      const int c = i / (B / 4), b = i % (B / 4) * 4;
+      if (c < cols_left) put_scales(&down_scale[c][b], q.scales_t + (int64_t)(c0 + c) * q.ld_scales_t + r0 / 32 + b, blocks_down - b, std::true_type{});
+    }
+    if constexpr (kAlong) {
+      for (int i = tid; i < U::kRows * 4; i += U::kThreads) {
+        const int r = i / 4, b = i % 4;
+        if (r < rows_left && b < blocks_along)
+          put(*reinterpret_cast<const u32x4*>(tile + kAlongCodes + 16 * i), q.codes + (r0 + r) * q.ld_codes + c0 / 2 + 16 * b);
+      }
+      for (int r = tid; r < rows_left; r += U::kThreads) put_scales(along_scale[r], q.scales + (r0 + r) * q.ld_scales + c0 / 32, blocks_along, std::false_type{});
+    }
+    __syncthreads();
   }
-  *reinterpret_cast<u32x4*>(q.codes_t + col * q.ld_codes_t + 16 * b) = w;
-  q.scales_t[col * q.ld_scales_t + b] = (uint8_t)s;
 }
 
-// Blocks down the columns: a lane quantises 32 rows of one column.
+// 16 bytes of values: 8 (f32: 4) codes w with scale byte s, two a time by the conversion instructions (exact but
+// for f16, which rounds).
 template <int D>
-__global__ void __launch_bounds__(kThreads) quant_cols_kernel(ggemm_mx4_quant_t q) {
-  const int64_t col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  if (col >= q.cols) return;
-  for (int64_t b = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); 32 * b < q.rows; b += 4 * (int64_t)gridDim.y)
-    quant_column_block<D>(q, col, b);
+struct Sixteen {
+  static constexpr int N = 16 / (int)sizeof(typename Elem<D>::T);
+  using Codes = std::conditional_t<D == GGEMM_F32, uint16_t, uint32_t>;
+  typename Elem<D>::T v[N];
+};
+template <int D>
+__device__ __forceinline__ Sixteen<D> values_of(uint32_t w, uint32_t s) {
+  const float scale = mx4_scale(s);
+  Sixteen<D> o;
+  if constexpr (D == GGEMM_F32) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
+    o = __builtin_bit_cast(Sixteen<D>, f32x4{a[0], a[1], b[0], b[1]});
+  } else {
+    auto word = [&](auto x) { return __builtin_bit_cast(uint32_t, x); };
+    u32x4 x;
+    if constexpr (D == GGEMM_BF16)
+      x = u32x4{word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)), word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)), word(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+    else
+      x = u32x4{word(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)), word(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+                word(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)), word(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+    o = __builtin_bit_cast(Sixteen<D>, x);
+  }
+  if (s == 255u) {
+#pragma unroll
+    for (int i = 0; i < Sixteen<D>::N; ++i) o.v[i] = (typename Elem<D>::T)__uint_as_float(0x7fc00000u);
+  }
+  return o;
 }
 
-// A lane turns 8 codes into values.
+// A lane turns the codes of chunk `chunk` (16 bytes of values) of a row into values.
+template <int D>
+__device__ __forceinline__ void load_codes(const ggemm_mx4_dequant_t& d, int64_t row, int chunk, uint32_t& w, uint32_t& s) {
+  constexpr int N = Sixteen<D>::N;
+  w = *reinterpret_cast<const typename Sixteen<D>::Codes*>(d.codes + row * d.ld_codes + chunk * (N / 2));
+  s = d.scales[row * d.ld_scales + chunk / (32 / N)];
+}
 template <int D, bool kVec>
-__device__ __forceinline__ void dequant_chunk(const ggemm_mx4_dequant_t& d, int64_t row, int chunk) {
-  using T = typename Elem<D>::T;
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(d.codes + row * d.ld_codes + 4 * chunk);
-  const uint32_t s = d.scales[row * d.ld_scales + (chunk >> 2)];
-  Oct<D> o;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t c = w >> (4 * i), e = (c >> 1) & 3u, m = c & 1u;
-    // magnitude: e = 0: m / 2, else (1 + m / 2) 2^(e - 1); exact in 32 bits times any scale
-    const float mag = e ? __uint_as_float(((126u + e) << 23) | (m << 22)) : 0.5f * (float)m;
-    float v = mag * mx4_scale(s);
-    v = c & 8u ? -v : v;
-    o.v[i] = (T)(s == 255u ? __uint_as_float(0x7fc00000u) : v);
-  }
-  const int c0 = 8 * chunk;
-  T* p = static_cast<T*>(d.y) + row * d.ld + c0;
-  if (kVec && c0 + 8 <= d.cols) {
-    *reinterpret_cast<Oct<D>*>(__builtin_assume_aligned(p, 16)) = o;
+__device__ __forceinline__ void store_values(const ggemm_mx4_dequant_t& d, int64_t row, int chunk, uint32_t w, uint32_t s) {
+  constexpr int N = Sixteen<D>::N;
+  const Sixteen<D> o = values_of<D>(w, s);
+  const int c0 = N * chunk;
+  auto* p = static_cast<typename Elem<D>::T*>(d.y) + row * d.ld + c0;
+  if (kVec && c0 + N <= d.cols) {
+    put(__builtin_bit_cast(u32x4, o), p);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N; ++i)
       if (c0 + i < d.cols) p[i] = o.v[i];
   }
 }
-
 template <int D, bool kVec>
 __global__ void __launch_bounds__(kThreads) dequant_kernel(ggemm_mx4_dequant_t d, int log_cx) {
-  const int chunks = ceil_div(d.cols, 8);
+  const int chunks = ceil_div(d.cols, Sixteen<D>::N);
   const int chunk = (blockIdx.y << log_cx) + (threadIdx.x & ((1 << log_cx) - 1));
   if (chunk >= chunks) return;
-  for (int64_t row = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx); row < d.rows;
-       row += (int64_t)gridDim.x << (8 - log_cx))
-    dequant_chunk<D, kVec>(d, row, chunk);
+  const int64_t step = (int64_t)gridDim.x << (8 - log_cx);
+  int64_t row = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx);
+  for (; row + 3 * step < d.rows; row += 4 * step) {   // four rows' loads before their stores
+    uint32_t w[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_codes<D>(d, row + i * step, chunk, w[i], s[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_values<D, kVec>(d, row + i * step, chunk, w[i], s[i]);
+  }
+  for (; row < d.rows; row += step) {
+    uint32_t w, s;
+    load_codes<D>(d, row, chunk, w, s);
+    store_values<D, kVec>(d, row, chunk, w, s);
+  }
 }
 
 // Lanes of a workgroup along a row of `chunks` chunks: the power of two at or above, at most 256.
@@ -178,14 +363,15 @@ int log_lanes(int chunks) {
   return l;
 }
 
-// Grid of a row kernel: x strides over the rows (at most 2^20 workgroups), y stays within its 65535 for
-// every valid size.
+// Grid of a row kernel: x strides over the rows, y stays within its 65535 for every valid size.  About 2048
+// workgroups, eight a compute unit, so that a lane has several rows in flight (32768 x 4096 bf16 along the
+// rows: 77 us with a workgroup for every 256 chunks, 64 with 2048).
 dim3 row_grid(int rows, int chunks, int log_cx) {
-  const int per = 256 >> log_cx;
-  return dim3((unsigned)std::min(ceil_div(rows, per), 1 << 20), (unsigned)ceil_div(chunks, 1 << log_cx));
+  const int per = 256 >> log_cx, y = ceil_div(chunks, 1 << log_cx);
+  return dim3((unsigned)std::min(ceil_div(rows, per), std::max(1, 2048 / y)), (unsigned)y);
 }
 
-constexpr int kMaxCols = 1 << 26;   // 8 columns a lane, 256 lanes a workgroup: at most 32768 workgroups along a row
+constexpr int kMaxCols = 1 << 25;   // 4 columns a lane or more, 256 lanes a workgroup: at most 32768 workgroups along a row
 
 bool codes_ok(const uint8_t* codes, int64_t ld_codes, const uint8_t* scales, int64_t ld_scales, int cols) {
   const int64_t nb = ceil_div(cols, 32);
@@ -207,17 +393,22 @@ int mx4_quantize(const ggemm_mx4_quant_t* q, hipStream_t s) {
   if (down && !codes_ok(q->codes_t, q->ld_codes_t, q->scales_t, q->ld_scales_t, q->rows)) return GGEMM_ERR_INVALID;
   with_elem(q->dtype, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (along) {
+    const bool vec = aligned(q->x, 16) && q->ld * elem_bytes(D) % 16 == 0;
+    if (down) {
+      const int64_t tiles = (int64_t)ceil_div(q->rows, Turn<D>::kRows) * ceil_div(q->cols, Turn<D>::kCols);
+      const unsigned grid = (unsigned)std::min<int64_t>(tiles, 1 << 20);
+      auto go = [&](auto v, auto a) {
+        quant_turn_kernel<D, decltype(v)::value, decltype(a)::value><<<grid, Turn<D>::kThreads, 0, s>>>(*q);
+      };
+      using std::true_type;
+      using std::false_type;
+      if (vec) along ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
+      else along ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
+    } else {
       const int chunks = 4 * ceil_div(q->cols, 32), l = log_lanes(chunks);
       const dim3 grid = row_grid(q->rows, chunks, l);
-      if (aligned(q->x, 16) && q->ld * elem_bytes(D) % 16 == 0)
-        quant_rows_kernel<D, true><<<grid, kThreads, 0, s>>>(*q, l);
-      else
-        quant_rows_kernel<D, false><<<grid, kThreads, 0, s>>>(*q, l);
-    }
-    if (down) {
-      const dim3 grid((unsigned)ceil_div(q->cols, 64), (unsigned)std::min(ceil_div(q->rows, 128), 32768));
-      quant_cols_kernel<D><<<grid, kThreads, 0, s>>>(*q);
+      if (vec) quant_rows_kernel<D, true><<<grid, kThreads, 0, s>>>(*q, l);
+      else quant_rows_kernel<D, false><<<grid, kThreads, 0, s>>>(*q, l);
     }
   });
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
@@ -231,7 +422,7 @@ int mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t s) {
     return GGEMM_ERR_INVALID;
   with_elem(d->dtype, [&](auto t) {
     constexpr int D = decltype(t)::value;
-    const int chunks = ceil_div(d->cols, 8), l = log_lanes(chunks);
+    const int chunks = ceil_div(d->cols, Sixteen<D>::N), l = log_lanes(chunks);
     const dim3 grid = row_grid(d->rows, chunks, l);
     if (aligned(d->y, 16) && d->ld * elem_bytes(D) % 16 == 0)
       dequant_kernel<D, true><<<grid, kThreads, 0, s>>>(*d, l);

@@ -2,9 +2,11 @@
 //
 // A token's logits lie in L lanes of one wave, V consecutive experts to a lane (L V >= experts, L a power
 // of two, 64 / L tokens a wave), in registers from the load to the last use.  Selection works on
-// 32-bit keys that order like the logits (NaN highest, barred experts 0): per place a maximum over the
-// lane's keys and then over the L lanes, and the lowest lane, then the lowest of its experts, that holds
-// it.  Softmax is the usual exp2((x - max) log2 e) over its sum, the maximum being the first choice.
+// integer keys that order like the logits (NaN highest, barred experts 0): per place a maximum over the
+// lane's keys and then over the L lanes, whose holder is struck out.  16-bit logits have the expert's number,
+// inverted, in the key's low half, so that a key is unique and tells the expert to all lanes; 32-bit ones
+// take a second reduction, the least expert that holds the maximum.  Softmax is the usual exp2((x - max)
+// log2 e) over its sum, the maximum being the first choice; its sums are 32-bit.
 // Counting: a workgroup takes `span` consecutive tokens.  One bit per (expert, token) in LDS gives each pair
 // its rank among the workgroup's tokens by counting bits (no atomic whose order matters), and the
 // expert's count.  A second launch turns the workgroups' counts into starting ranks and sums their partial
@@ -19,6 +21,9 @@
 namespace ggemm {
 namespace {
 
+#ifndef SPAN
+#define SPAN 128
+#endif
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -36,7 +41,7 @@ struct Shape {
 // Tokens a workgroup takes (a multiple of 32: whole words of the bit table).  Few tokens are spread over
 // the compute units, many take longer spans, which makes the tables of the second launch shorter.
 Shape shape_of(int tokens) {
-  const int span = tokens <= 32768 ? 64 : 256;
+  const int span = tokens <= 65536 ? 64 : SPAN;
   return Shape{span, tokens > 0 ? ceil_div(tokens, span) : 1};
 }
 
@@ -46,23 +51,43 @@ RouteWs carve(void* ws, const Shape& sh, int experts) {
   return RouteWs{reinterpret_cast<int*>(p), reinterpret_cast<float*>(p + table), reinterpret_cast<int*>(p + 2 * table)};
 }
 
-// A key that orders like x: 0 for -inf, above every other for NaN; x + 0 makes -0 equal to +0.
-__device__ __forceinline__ uint32_t key_of(float x) {
-  x += 0.0f;
-  const uint32_t b = __float_as_uint(x);
+// Keys that order like the logits: 0 for -inf, all ones for NaN, -0 as +0.
+__device__ __forceinline__ uint32_t key32(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
   if (x != x) return 0xffffffffu;
   if (b == 0xff800000u) return 0u;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float of_key(uint32_t k) {
+__device__ __forceinline__ float of_key32(uint32_t k) {
   return k == 0xffffffffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
+template <int D>
+__device__ __forceinline__ uint32_t key16(float x) {   // x: a value of the 16-bit type
+  const uint32_t b = __builtin_bit_cast(unsigned short, (typename Elem<D>::T)(x + 0.0f));
+  if (x != x) return 0xffffu;
+  if (x == -__builtin_inff()) return 0u;
+  return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+}
+template <int D>
+__device__ __forceinline__ float of_key16(uint32_t k) {
+  const unsigned short b = (unsigned short)(k & 0x8000u ? k ^ 0x8000u : ~k);
+  return k == 0xffffu ? __uint_as_float(0x7fc00000u) : (float)__builtin_bit_cast(typename Elem<D>::T, b);
+}
 
-// Reductions over the L lanes of a token; every lane gets the result.
+// Reductions over the L lanes of a token; every lane gets the result.  Up to 16 lanes the exchanges are part of the
+// vector instructions: neighbours, pairs, then (quads being alike) mirrored within 8 and 16.
+template <int CTRL, class T>
+__device__ __forceinline__ T other(T x) {
+  return __builtin_bit_cast(T, dpp<CTRL>(__builtin_bit_cast(uint32_t, x)));
+}
 template <int L, class T, class F>
 __device__ __forceinline__ T over_lanes(T x, F&& f) {
+  x = f(x, other<kDppXor1>(x));
+  x = f(x, other<kDppXor2>(x));
+  x = f(x, other<kDppHalfMirror>(x));
+  if constexpr (L >= 16) x = f(x, other<kDppMirror>(x));
 #pragma unroll
-  for (int d = 1; d < L; d *= 2) x = f(x, __shfl_xor(x, d));
+  for (int d = 16; d < L; d *= 2) x = f(x, __shfl_xor(x, d));
   return x;
 }
 template <int L>
@@ -73,14 +98,51 @@ template <int L>
 __device__ __forceinline__ uint32_t max_lanes(uint32_t x) {
   return over_lanes<L>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
+template <int L>
+__device__ __forceinline__ uint32_t min_lanes(uint32_t x) {
+  return over_lanes<L>(x, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
 
-// The lane's V logits of token t (experts lane V ...; -inf past the last expert).
+// V values side by side, in pieces of at most 16 bytes (kVec: aligned to them).
 template <int D, int V>
-__device__ __forceinline__ void load_logits(const ggemm_router_t& r, int t, int e0, float (&x)[V]) {
+struct Piece {
   using T = typename Elem<D>::T;
-  const T* p = static_cast<const T*>(r.logits) + (int64_t)t * r.ld + e0;
+  static constexpr int N = V * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : V;
+  struct alignas(N * sizeof(T)) Type { T x[N]; };
+};
+// The lane's V logits of token t (experts e0 ...; -inf past the last expert).
+template <int D, int V, bool kVec>
+__device__ __forceinline__ void load_logits(const ggemm_router_t& r, int t, int e0, float (&x)[V]) {
+  using P = Piece<D, V>;
+  const auto* p = static_cast<const typename P::T*>(r.logits) + (int64_t)t * r.ld + e0;
+  if (kVec && e0 + V <= r.experts) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) x[v] = e0 + v < r.experts ? (float)p[v] : -__builtin_inff();
+    for (int i = 0; i < V; i += P::N) {
+      const typename P::Type w = *reinterpret_cast<const typename P::Type*>(p + i);
+#pragma unroll
+      for (int j = 0; j < P::N; ++j) x[i + j] = (float)w.x[j];
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = e0 + v < r.experts ? (float)p[v] : -__builtin_inff();
+  }
+}
+template <int D, int V, bool kVec>
+__device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, int experts, const float (&g)[V]) {
+  using P = Piece<D, V>;
+  if (kVec && e0 + V <= experts) {
+#pragma unroll
+    for (int i = 0; i < V; i += P::N) {
+      typename P::Type w;
+#pragma unroll
+      for (int j = 0; j < P::N; ++j) w.x[j] = (typename P::T)g[i + j];
+      *reinterpret_cast<typename P::Type*>(p + e0 + i) = w;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (e0 + v < experts) p[e0 + v] = (typename P::T)g[v];
+  }
 }
 
 // p[v] = exp(x[v] - max) for a token's lanes, and the reciprocal of the sum.  m: the largest logit.
@@ -143,7 +205,7 @@ __device__ __forceinline__ void scan_offsets(const int* counts, int experts, int
 
 // First launch: choices, gates, ranks within the workgroup's tokens (into pos), counts and softmax sums
 // per workgroup.  kOne: the only workgroup, which finishes the call.
-template <int D, int L, int V, bool kOne>
+template <int D, int L, int V, bool kOne, bool kVec>
 __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, RouteWs ws, int span) {
   constexpr int kRows = 64 / L, kPar = 4 * kRows;   // tokens a wave and a workgroup hold at a time
   extern __shared__ uint32_t lds[];
@@ -162,67 +224,78 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
   int used = 0;
   for (int tb = t0; tb < t1; tb += kPar) {
     const int t = tb + slot;
-    const bool on = t < t1 && !masked(r, t);
+    const bool in = t < t1;
     float x[V], p[V];
     uint32_t key[V];
-    if (on) {
-      load_logits<D, V>(r, t, e0, x);
+    if (in && !masked(r, t)) {
+      load_logits<D, V, kVec>(r, t, e0, x);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v) x[v] = -__builtin_inff();
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
-    float inv = 0.0f, chosen = 0.0f, m = 0.0f;
-    float mine = 0.0f;   // gate of place `sub` (+ L, ...) is stored as it is found; kept for renormalising
-    bool live = false;
+    for (int v = 0; v < V; ++v) {
+      if constexpr (D == GGEMM_F32) {
+        key[v] = key32(x[v]);
+      } else {
+        const uint32_t k = key16<D>(x[v]);
+        key[v] = k ? k << 16 | (0xffffu - (e0 + v)) : 0u;
+      }
+    }
+    // the largest key of the token, 0: none left; every lane gets it, its logit and its expert
+    auto take = [&](float& logit, int& expert) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) best = max(best, key[v]);
+      best = max_lanes<L>(best);
+      if constexpr (D == GGEMM_F32) {
+        uint32_t e = 0xffffffffu;
+#pragma unroll
+        for (int v = V - 1; v >= 0; --v) e = key[v] == best ? e0 + v : e;
+        expert = (int)min_lanes<L>(e);
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = expert == e0 + v ? 0u : key[v];
+        logit = of_key32(best);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = key[v] == best ? 0u : key[v];
+        expert = 0xffff - (int)(best & 0xffffu);
+        logit = of_key16<D>(best >> 16);
+      }
+      return best != 0;
+    };
+    float m;
+    int e;
+    bool more = take(m, e);
+    const bool live = more;
+    const float inv = exps<L, V>(x, m, p);
+    float logit = m, chosen = 0.0f, gate = 0.0f;
+    int id = -1;
+    int64_t out = (int64_t)t * K + sub;   // lane `sub` stores places sub, sub + L, ...
     for (int j = 0; j < K; ++j) {
-      uint32_t top = key[0];
-#pragma unroll
-      for (int v = 1; v < V; ++v) top = max(top, key[v]);
-      const uint32_t best = max_lanes<L>(top);
-      if (j == 0) {
-        live = best != 0;
-        m = of_key(best);
-        inv = exps<L, V>(x, m, p);
+      if (j) more = take(logit, e);
+      const float g = more ? __builtin_amdgcn_exp2f((logit - m) * kLog2e) * inv : 0.0f;
+      chosen += g;
+      if ((j & (L - 1)) == sub) {
+        gate = g;
+        id = more ? e : -1;
       }
-      // the lowest lane of the token that holds it
-      const uint64_t holds = __ballot(top == best) >> (lane & ~(L - 1));
-      const bool here = best != 0 && __builtin_ctzll(holds) == sub;
-      float g = 0.0f;
-      if (here) {
-        int at = 0;
-#pragma unroll
-        for (int v = V - 1; v >= 0; --v)
-          if (key[v] == best) at = v;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v == at) {
-            key[v] = 0;
-            g = p[v] * inv;
-          }
-        const int e = e0 + at;
-        r.ids[(int64_t)t * K + j] = e;
-        r.gates[(int64_t)t * K + j] = g;
-        atomicOr(&bits[e * words + ((t - t0) >> 5)], 1u << ((t - t0) & 31));
+      if ((j & (L - 1)) == L - 1 || j == K - 1) {
+        if (in && sub <= (j & (L - 1))) {
+          r.ids[out] = id;
+          r.gates[out] = r.renormalize && K <= L && id >= 0 ? gate / chosen : gate;
+          if (id >= 0) atomicOr(&bits[id * words + ((t - t0) >> 5)], 1u << ((t - t0) & 31));
+        }
+        out += L;
       }
-      if (best == 0 && t < t1 && sub == 0) {
-        r.ids[(int64_t)t * K + j] = -1;
-        r.gates[(int64_t)t * K + j] = 0.0f;
-      }
-      mine += g;
     }
     if (live) {
       used += sub == 0;
 #pragma unroll
       for (int v = 0; v < V; ++v) acc[v] += p[v] * inv;
-    }
-    if (r.renormalize) {
-      chosen = sum_lanes<L>(mine);
-      __threadfence_block();   // the gates were stored by the lanes that held them
-      for (int j = sub; j < K && live; j += L) {
-        float* g = r.gates + (int64_t)t * K + j;
-        if (r.ids[(int64_t)t * K + j] >= 0) *g = *g / chosen;
+      if (r.renormalize && K > L) {   // the sum came after the first places were stored, by the same lanes
+        for (int64_t i = (int64_t)t * K + sub; i < (int64_t)(t + 1) * K; i += L)
+          if (r.ids[i] >= 0) r.gates[i] = r.gates[i] / chosen;
       }
     }
   }
@@ -283,16 +356,18 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
   }
 }
 
-// Second launch: a workgroup per 16 experts, 16 threads along the workgroups of the first launch each
+// Second launch: a workgroup per 16 experts, 64 threads along the workgroups of the first launch each
 // taking a run of them: sums per run, then starting ranks.
-__global__ void __launch_bounds__(kThreads) route_scan_kernel(ggemm_router_t r, RouteWs ws, int groups) {
-  __shared__ int s_cnt[16][17], s_use[16];
-  __shared__ float s_p[16][17];
+constexpr int kRuns = 64;
+__global__ void __launch_bounds__(16 * kRuns) route_scan_kernel(ggemm_router_t r, RouteWs ws, int groups) {
+  __shared__ int s_cnt[kRuns][17], s_use[16];
+  __shared__ float s_p[kRuns][17];
   const int i = threadIdx.x & 15, c = threadIdx.x >> 4, e = blockIdx.x * 16 + i, E = r.experts;
-  const int run = ceil_div(groups, 16), g0 = min(c * run, groups), g1 = min(g0 + run, groups);
+  const int run = ceil_div(groups, kRuns), g0 = min(c * run, groups), g1 = min(g0 + run, groups);
   int cnt = 0;
   float ps = 0.0f;
   if (e < E) {
+#pragma unroll 8
     for (int g = g0; g < g1; ++g) {
       cnt += ws.hist[(int64_t)g * E + e];
       ps += ws.psum[(int64_t)g * E + e];
@@ -301,20 +376,25 @@ __global__ void __launch_bounds__(kThreads) route_scan_kernel(ggemm_router_t r, 
   s_cnt[c][i] = cnt;
   s_p[c][i] = ps;
   int use = 0;
-  for (int g = threadIdx.x; g < groups; g += kThreads) use += ws.used[g];
+  for (int g = threadIdx.x; g < groups; g += 16 * kRuns) use += ws.used[g];
   use = over_lanes<64>(use, [](int a, int b) { return a + b; });
   if ((threadIdx.x & 63) == 0) s_use[threadIdx.x >> 6] = use;
   __syncthreads();
-  use = s_use[0] + s_use[1] + s_use[2] + s_use[3];
+  use = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) use += s_use[w];
   int at = 0;
+#pragma unroll 8
   for (int q = 0; q < c; ++q) at += s_cnt[q][i];
   if (e < E) {
-    if (c == 15) r.counts[e] = at + cnt;
+    if (c == kRuns - 1) r.counts[e] = at + cnt;
     if (c == 0) {
       float sum = 0.0f;
-      for (int q = 0; q < 16; ++q) sum += s_p[q][i];
+#pragma unroll 8
+      for (int q = 0; q < kRuns; ++q) sum += s_p[q][i];
       r.probs[e] = use ? sum / (float)use : 0.0f;
     }
+#pragma unroll 8
     for (int g = g0; g < g1; ++g) {
       int* h = ws.hist + (int64_t)g * E + e;
       const int n = *h;
@@ -354,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) route_place_kernel(ggemm_router_t r,
 // Gradient: dx = p (s - <p, s>) + c, with s_e = d_loss coef E counts_e / (topk used^2) and, for the chosen
 // places, c_j = g_j (dg_j - <g, dg>) when the gates are renormalised; else s_e takes dg_j too and c = 0.
 // The token's dg (or c) by expert goes through a row of LDS that is zero outside the chosen places.
-template <int D, int L, int V>
+template <int D, int L, int V, bool kVec>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t r, const float* __restrict__ d_gates,
                                                                   const float* __restrict__ d_loss, void* d_logits,
                                                                   int64_t ld_d, int per) {
@@ -379,16 +459,16 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     const bool in = t < t1, on = in && !masked(r, t);
     float x[V], p[V], d[V];
     if (on) {
-      load_logits<D, V>(r, t, e0, x);
+      load_logits<D, V, kVec>(r, t, e0, x);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v) x[v] = -__builtin_inff();
     }
     uint32_t top = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) top = max(top, key_of(x[v]));
+    for (int v = 0; v < V; ++v) top = max(top, key32(x[v]));
     top = max_lanes<L>(top);
-    const float inv = exps<L, V>(x, of_key(top), p);
+    const float inv = exps<L, V>(x, of_key32(top), p);
     const bool live = on && top != 0;
     float dot = 0.0f;
     if (r.renormalize && d_gates) {
@@ -416,13 +496,14 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     for (int v = 0; v < V; ++v) row[e0 + v] = 0.0f;
     __threadfence_block();
     if (in) {
-      T* out = static_cast<T*>(d_logits) + (int64_t)t * ld_d + e0;
+      float g[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float g = p[v] * (d[v] - ps) + (r.renormalize ? c[v] : 0.0f);
+        g[v] = p[v] * (d[v] - ps) + (r.renormalize ? c[v] : 0.0f);
         // a barred expert has p = 0 and no place, but 0 times a NaN sum is not 0
-        if (e0 + v < E) out[v] = (T)(live && x[v] != -__builtin_inff() ? g : 0.0f);
+        g[v] = live && x[v] != -__builtin_inff() ? g[v] : 0.0f;
       }
+      store_gradient<D, V, kVec>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, g);
     }
   }
 }
@@ -476,14 +557,19 @@ int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
     with_lanes(r->experts, [&](auto l, auto v) {
       constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
       const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + 4 * L * V * 4;
-      if (sh.groups == 1)
-        route_kernel<D, L, V, true><<<1, kThreads, lds, s>>>(*r, w, sh.span);
-      else
-        route_kernel<D, L, V, false><<<sh.groups, kThreads, lds, s>>>(*r, w, sh.span);
+      constexpr int A = sizeof(typename Piece<D, V>::Type);
+      auto go = [&](auto one, auto vec) {
+        route_kernel<D, L, V, decltype(one)::value, decltype(vec)::value><<<sh.groups, kThreads, lds, s>>>(*r, w, sh.span);
+      };
+      using std::true_type;
+      using std::false_type;
+      const bool vec = aligned(r->logits, A) && r->ld * elem_bytes(D) % A == 0;
+      if (sh.groups == 1) vec ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
+      else vec ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
     });
   });
   if (sh.groups > 1) {
-    route_scan_kernel<<<ceil_div(r->experts, 16), kThreads, 0, s>>>(*r, w, sh.groups);
+    route_scan_kernel<<<ceil_div(r->experts, 16), 16 * kRuns, 0, s>>>(*r, w, sh.groups);
     route_place_kernel<<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
   }
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
@@ -499,7 +585,15 @@ int route_backward(const ggemm_router_t* r, const float* d_gates, const float* d
       constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
       constexpr int kPar = 256 / L;
       const int per = std::max(kPar, (int)align_up((size_t)ceil_div(r->tokens, 2048), kPar));
-      route_backward_kernel<D, L, V><<<ceil_div(r->tokens, per), kThreads, 0, s>>>(*r, d_gates, d_loss, d_logits, ld_d, per);
+      constexpr int A = sizeof(typename Piece<D, V>::Type);
+      auto go = [&](auto vec) {
+        route_backward_kernel<D, L, V, decltype(vec)::value>
+            <<<ceil_div(r->tokens, per), kThreads, 0, s>>>(*r, d_gates, d_loss, d_logits, ld_d, per);
+      };
+      if (aligned(r->logits, A) && aligned(d_logits, A) && r->ld * elem_bytes(D) % A == 0 && ld_d * elem_bytes(D) % A == 0)
+        go(std::true_type{});
+      else
+        go(std::false_type{});
     });
   });
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;

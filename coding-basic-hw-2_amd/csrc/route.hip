@@ -3,9 +3,11 @@
 // A token's logits lie in L lanes of one wave, V consecutive experts to a lane (L V >= experts, L a power
 // of two, 64 / L tokens a wave), in registers from the load to the last use.  Selection works on
 // integer keys that order like the logits (NaN highest, barred experts 0): per place a maximum over the
-// lane's keys and then over the L lanes, whose holder is struck out.  16-bit logits have the expert's number,
-// inverted, in the key's low half, so that a key is unique and tells the expert to all lanes; 32-bit ones
-// take a second reduction, the least expert that holds the maximum.  Softmax is the usual exp2((x - max)
+// lane's keys and then over the L lanes.  16-bit logits have the expert's number, inverted, in the key's low
+// half, so that a key is unique and tells the expert to all lanes, and the next place is the largest of
+// key - best mod 2^32 (a key below `best` differs by 2^32 - best or more, one above by less): nothing is struck
+// out.  32-bit logits take a second reduction, the least expert that holds the maximum, which is struck out.
+// Softmax is the usual exp2((x - max)
 // log2 e) over its sum, the maximum being the first choice; its sums are 32-bit.
 // Counting: a workgroup takes `span` consecutive tokens.  One bit per (expert, token) in LDS gives each pair
 // its rank among the workgroup's tokens by counting bits (no atomic whose order matters), and the
@@ -61,16 +63,25 @@ __device__ __forceinline__ uint32_t key32(float x) {
 __device__ __forceinline__ float of_key32(uint32_t k) {
   return k == 0xffffffffu ? __uint_as_float(0x7fc00000u) : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
+// Two 16-bit logits a word: sign and magnitude to an unsigned order with -0 = +0, then down by what -inf got.  A
+// NaN of either sign has to be put right after.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
 template <int D>
-__device__ __forceinline__ uint32_t key16(float x) {   // x: a value of the 16-bit type
-  const uint32_t b = __builtin_bit_cast(unsigned short, (typename Elem<D>::T)(x + 0.0f));
-  if (x != x) return 0xffffu;
-  if (x == -__builtin_inff()) return 0u;
-  return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+struct Half {
+  static constexpr uint32_t kInf = D == GGEMM_BF16 ? 0x7f80u : 0x7c00u, kLow = 0x7fffu - kInf + 1;
+};
+template <int D>
+__device__ __forceinline__ uint32_t order16(uint32_t w) {
+  const i16x2 s = __builtin_bit_cast(i16x2, w) >> (short)15;
+  const uint32_t o = w ^ (__builtin_bit_cast(uint32_t, s) | 0x80008000u);
+  const u16x2 up = __builtin_bit_cast(u16x2, o) - __builtin_bit_cast(u16x2, s);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(up, u16x2{Half<D>::kLow, Half<D>::kLow}));
 }
 template <int D>
-__device__ __forceinline__ float of_key16(uint32_t k) {
-  const unsigned short b = (unsigned short)(k & 0x8000u ? k ^ 0x8000u : ~k);
+__device__ __forceinline__ float of_order16(uint32_t k) {
+  const uint32_t o = k + Half<D>::kLow;
+  const unsigned short b = (unsigned short)(o >= 0x8000u ? o ^ 0x8000u : ~(o - 1u));
   return k == 0xffffu ? __uint_as_float(0x7fc00000u) : (float)__builtin_bit_cast(typename Elem<D>::T, b);
 }
 
@@ -110,23 +121,31 @@ struct Piece {
   static constexpr int N = V * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : V;
   struct alignas(N * sizeof(T)) Type { T x[N]; };
 };
-// The lane's V logits of token t (experts e0 ...; -inf past the last expert).
-template <int D, int V, bool kVec>
-__device__ __forceinline__ void load_logits(const ggemm_router_t& r, int t, int e0, float (&x)[V]) {
+// The lane's V logits of token t (experts e0 ...; -inf past the last expert), as they lie in memory: a wave has the
+// next tokens' on the way while it works on these (131072 x 256 bf16, forward %%F%%, backward %%B%% us).  Those of a token
+// that is left out are read and not used.
+template <int D, int V>
+struct Logits {
   using P = Piece<D, V>;
-  const auto* p = static_cast<const typename P::T*>(r.logits) + (int64_t)t * r.ld + e0;
-  if (kVec && e0 + V <= r.experts) {
+  typename P::Type w[V / P::N];
+  unsigned char mask;
+  template <bool kVec>
+  __device__ __forceinline__ void load(const ggemm_router_t& r, int t, int t1, int e0) {
+    using T = typename P::T;
+    if (t >= t1) return;
+    mask = r.mask ? r.mask[t] : 1;
+    const T* p = static_cast<const T*>(r.logits) + (int64_t)t * r.ld + e0;
+    if (kVec && e0 + V <= r.experts) {
 #pragma unroll
-    for (int i = 0; i < V; i += P::N) {
-      const typename P::Type w = *reinterpret_cast<const typename P::Type*>(p + i);
+      for (int i = 0; i < V / P::N; ++i) w[i] = *reinterpret_cast<const typename P::Type*>(p + i * P::N);
+    } else {
 #pragma unroll
-      for (int j = 0; j < P::N; ++j) x[i + j] = (float)w.x[j];
+      for (int v = 0; v < V; ++v) w[v / P::N].x[v % P::N] = e0 + v < r.experts ? p[v] : (T)-__builtin_inff();
     }
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = e0 + v < r.experts ? (float)p[v] : -__builtin_inff();
   }
-}
+  __device__ __forceinline__ bool on(int t, int t1) const { return t < t1 && mask; }   // the token takes part
+  __device__ __forceinline__ typename P::T at(int v) const { return w[v / P::N].x[v % P::N]; }
+};
 template <int D, int V, bool kVec>
 __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, int experts, const float (&g)[V]) {
   using P = Piece<D, V>;
@@ -145,19 +164,26 @@ __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, i
   }
 }
 
-// p[v] = exp(x[v] - max) for a token's lanes, and the reciprocal of the sum.  m: the largest logit.
+// exp(x - m).  The difference first: m log2 e alone overflows for logits of the type's lowest value.
+__device__ __forceinline__ float exp_below(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
+// p[v] = exp(x[v] - max) for a token's lanes, and the reciprocal of the sum.  m: the largest logit; -inf gives 0.
+// Where no token of the wave has so large a maximum, one fma: the rounding of m log2 e is the same for all of a
+// token's values and leaves with the sum.
 template <int L, int V>
 __device__ __forceinline__ float exps(const float (&x)[V], float m, float (&p)[V]) {
   float sum = 0.0f;
+  if (__ballot(fabsf(m) > 1e30f) == 0) {
+    const float c = m * kLog2e;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    p[v] = x[v] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((x[v] - m) * kLog2e);
-    sum += p[v];
+    for (int v = 0; v < V; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], kLog2e, -c));
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = exp_below(x[v], m);
   }
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum += p[v];
   return 1.0f / sum_lanes<L>(sum);
 }
-
-__device__ __forceinline__ bool masked(const ggemm_router_t& r, int t) { return r.mask && r.mask[t] == 0; }
 
 // Rows of order that belong to no pair: expert e's padding, and what follows the last expert.
 __device__ __forceinline__ void pad_order(const ggemm_router_t& r, int from, int to, int lane, int lanes) {
@@ -222,71 +248,92 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
   int used = 0;
+  Logits<D, V> ahead;
+  ahead.template load<kVec>(r, t0 + slot, t1, e0);
   for (int tb = t0; tb < t1; tb += kPar) {
     const int t = tb + slot;
     const bool in = t < t1;
+    const bool on = ahead.on(t, t1);
     float x[V], p[V];
     uint32_t key[V];
-    if (in && !masked(r, t)) {
-      load_logits<D, V, kVec>(r, t, e0, x);
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = (float)ahead.at(v);
+    // 16-bit keys: order, then a number that falls with the expert's: within the lane here, the lane's later
+    constexpr uint32_t kIn = V - 1;
+    const uint32_t lane_part = 0xffffu - e0 - kIn;
+    if constexpr (D == GGEMM_F32) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) key[v] = key32(x[v]);
     } else {
+      typedef typename Elem<D>::T pair __attribute__((ext_vector_type(2)));
+      uint32_t worst = 0;   // the largest magnitudes: a NaN among them?
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = -__builtin_inff();
-    }
+      for (int v = 0; v < V; v += 2) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, pair{ahead.at(v), ahead.at(v + 1 < V ? v + 1 : v)});
+        worst = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, worst), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+        const uint32_t o = order16<D>(w);
+        key[v] = o << 16 | (kIn - v);
+        if (v + 1 < V) key[v + 1] = (o & 0xffff0000u) | (kIn - v - 1);
+      }
+      if (__ballot(max(worst & 0xffffu, worst >> 16) > Half<D>::kInf)) {
+        asm volatile("");   // a branch, not a select per value
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if constexpr (D == GGEMM_F32) {
-        key[v] = key32(x[v]);
-      } else {
-        const uint32_t k = key16<D>(x[v]);
-        key[v] = k ? k << 16 | (0xffffu - (e0 + v)) : 0u;
+        for (int v = 0; v < V; ++v) key[v] = x[v] != x[v] ? key[v] | 0xffff0000u : key[v];
       }
     }
-    // the largest key of the token, 0: none left; every lane gets it, its logit and its expert
-    auto take = [&](float& logit, int& expert) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int v = 1; v < V; ++v) best = max(best, key[v]);
-      best = max_lanes<L>(best);
+    ahead.template load<kVec>(r, t + kPar, t1, e0);
+    // the largest key of the token below the last one taken (32-bit: of those not struck out), and its expert
+    uint32_t best = 0;
+    int expert = 0;
+    auto take = [&]() {
       if constexpr (D == GGEMM_F32) {
+        uint32_t top = key[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) top = max(top, key[v]);
+        best = max_lanes<L>(top);
         uint32_t e = 0xffffffffu;
 #pragma unroll
         for (int v = V - 1; v >= 0; --v) e = key[v] == best ? e0 + v : e;
         expert = (int)min_lanes<L>(e);
 #pragma unroll
         for (int v = 0; v < V; ++v) key[v] = expert == e0 + v ? 0u : key[v];
-        logit = of_key32(best);
       } else {
+        const uint32_t from = best - lane_part;
+        uint32_t top = key[0] - from;
 #pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = key[v] == best ? 0u : key[v];
-        expert = 0xffff - (int)(best & 0xffffu);
-        logit = of_key16<D>(best >> 16);
+        for (int v = 1; v < V; ++v) top = max(top, key[v] - from);
+        best += max_lanes<L>(top);
       }
-      return best != 0;
     };
-    float m;
-    int e;
-    bool more = take(m, e);
-    const bool live = more;
+    auto logit_of = [&](uint32_t k) {
+      if constexpr (D == GGEMM_F32) return of_key32(k);
+      else return of_order16<D>(k >> 16);
+    };
+    auto expert_of = [&](uint32_t k, int e) { return D == GGEMM_F32 ? e : 0xffff - (int)(k & 0xffffu); };
+    auto any = [&](uint32_t k) { return D == GGEMM_F32 ? k != 0 : k >> 16 != 0; };   // not a barred expert's
+    take();
+    const float m = logit_of(best);
+    const bool live = on && any(best);
     const float inv = exps<L, V>(x, m, p);
-    float logit = m, chosen = 0.0f, gate = 0.0f;
-    int id = -1;
-    int64_t out = (int64_t)t * K + sub;   // lane `sub` stores places sub, sub + L, ...
-    for (int j = 0; j < K; ++j) {
-      if (j) more = take(logit, e);
-      const float g = more ? __builtin_amdgcn_exp2f((logit - m) * kLog2e) * inv : 0.0f;
-      chosen += g;
-      if ((j & (L - 1)) == sub) {
-        gate = g;
-        id = more ? e : -1;
+    float chosen = 0.0f;
+    for (int j0 = 0; j0 < K; j0 += L) {   // lane `sub` keeps place j0 + sub
+      uint32_t mine = best;
+      int mine_e = expert;
+      const int n = min(L, K - j0);
+      for (int j = j0 ? 0 : 1; j < n; ++j) {
+        take();
+        mine = j == sub ? best : mine;
+        if constexpr (D == GGEMM_F32) mine_e = j == sub ? expert : mine_e;
       }
-      if ((j & (L - 1)) == L - 1 || j == K - 1) {
-        if (in && sub <= (j & (L - 1))) {
-          r.ids[out] = id;
-          r.gates[out] = r.renormalize && K <= L && id >= 0 ? gate / chosen : gate;
-          if (id >= 0) atomicOr(&bits[id * words + ((t - t0) >> 5)], 1u << ((t - t0) & 31));
-        }
-        out += L;
+      const bool have = live && sub < n && any(mine);
+      const int id = have ? expert_of(mine, mine_e) : -1;
+      float g = have ? exp_below(logit_of(mine), m) * inv : 0.0f;
+      chosen += sum_lanes<L>(g);
+      if (r.renormalize && K <= L && have) g = g / chosen;
+      if (in && sub < n) {
+        r.ids[(int64_t)t * K + j0 + sub] = id;
+        r.gates[(int64_t)t * K + j0 + sub] = g;
+        if (have) atomicOr(&bits[id * words + ((t - t0) >> 5)], 1u << ((t - t0) & 31));
       }
     }
     if (live) {
@@ -454,57 +501,94 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     row[e0 + v] = 0.0f;
   }
   const int t0 = blockIdx.x * per, t1 = min(t0 + per, r.tokens);
+  // a place of a token: its expert (-1: none), gate and the gate's gradient
+  struct Choice {
+    int e;
+    float g, dg;
+  };
+  auto choice = [&](int t, int j) {
+    Choice c{-1, 0.0f, 0.0f};
+    if (t < t1 && j < K) {
+      const int64_t at = (int64_t)t * K + j;
+      c.e = r.ids[at];
+      if (d_gates) {
+        c.g = r.gates[at];
+        c.dg = d_gates[at];
+      }
+    }
+    return c;
+  };
+  Logits<D, V> ahead;
+  ahead.template load<kVec>(r, t0 + slot, t1, e0);
+  Choice next = choice(t0 + slot, sub);
   for (int tb = t0; tb < t1; tb += kPar) {
     const int t = tb + slot;
-    const bool in = t < t1, on = in && !masked(r, t);
-    float x[V], p[V], d[V];
-    if (on) {
-      load_logits<D, V, kVec>(r, t, e0, x);
-    } else {
+    const bool in = t < t1;
+    float x[V], p[V];
+    const bool on = ahead.on(t, t1);
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = -__builtin_inff();
-    }
-    uint32_t top = 0;
+    for (int v = 0; v < V; ++v) x[v] = (float)ahead.at(v);
+    const Choice mine = next;
+    ahead.template load<kVec>(r, t + kPar, t1, e0);
+    next = choice(t + kPar, sub);
+    float m = x[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v) top = max(top, key32(x[v]));
-    top = max_lanes<L>(top);
-    const float inv = exps<L, V>(x, of_key32(top), p);
-    const bool live = on && top != 0;
-    float dot = 0.0f;
-    if (r.renormalize && d_gates) {
-      for (int j = sub; j < K && live; j += L)
-        dot += r.gates[(int64_t)t * K + j] * (r.ids[(int64_t)t * K + j] >= 0 ? d_gates[(int64_t)t * K + j] : 0.0f);
-      dot = sum_lanes<L>(dot);
-    }
-    for (int j = sub; j < K && live && d_gates; j += L) {
-      const int e = r.ids[(int64_t)t * K + j];
-      const float dg = d_gates[(int64_t)t * K + j];
-      if (e >= 0 && e < E) row[e] = r.renormalize ? r.gates[(int64_t)t * K + j] * (dg - dot) : dg;
+    for (int v = 1; v < V; ++v) m = fmaxf(m, x[v]);
+    m = over_lanes<L>(m, [](float a, float b) { return fmaxf(a, b); });
+    const float inv = exps<L, V>(x, m, p);
+    // the first place is taken unless every expert is barred
+    const bool live = on && __shfl(mine.e, lane & ~(L - 1)) >= 0;
+    if (d_gates) {
+      float dot = 0.0f;
+      if (r.renormalize) {
+        for (int j = sub; j < K; j += L) {
+          const Choice c = j < L ? mine : choice(t, j);
+          dot += c.e >= 0 ? c.g * c.dg : 0.0f;
+        }
+        dot = sum_lanes<L>(dot);
+      }
+      for (int j = sub; j < K; j += L) {
+        const Choice c = j < L ? mine : choice(t, j);
+        if (live && c.e >= 0 && c.e < E) row[c.e] = r.renormalize ? c.g * (c.dg - dot) : c.dg;
+      }
     }
     __threadfence_block();
     float c[V], ps = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      c[v] = row[e0 + v];
-      p[v] = live ? p[v] * inv : 0.0f;
-      d[v] = r.renormalize ? s[v] : s[v] + c[v];
-      ps += p[v] * d[v];
+    for (int v = 0; v < V; ++v) c[v] = row[e0 + v];
+    if (!live) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[v] = 0.0f;
     }
-    ps = sum_lanes<L>(ps);
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] *= inv;
+    if (r.renormalize) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) ps += p[v] * s[v];
+      ps = sum_lanes<L>(ps);
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] += p[v] * (s[v] - ps);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        c[v] += s[v];
+        ps += p[v] * c[v];
+      }
+      ps = sum_lanes<L>(ps);
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] = p[v] * (c[v] - ps);
+    }
     __threadfence_block();
 #pragma unroll
     for (int v = 0; v < V; ++v) row[e0 + v] = 0.0f;
     __threadfence_block();
-    if (in) {
-      float g[V];
+    // 0 times a NaN or infinite sum is not the 0 of a barred expert or of a token left out
+    if (__ballot(!live || !(fabsf(ps) < 1e30f))) {
+      asm volatile("");   // a branch, not a select per value
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        g[v] = p[v] * (d[v] - ps) + (r.renormalize ? c[v] : 0.0f);
-        // a barred expert has p = 0 and no place, but 0 times a NaN sum is not 0
-        g[v] = live && x[v] != -__builtin_inff() ? g[v] : 0.0f;
-      }
-      store_gradient<D, V, kVec>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, g);
+      for (int v = 0; v < V; ++v) c[v] = live && x[v] != -__builtin_inff() ? c[v] : 0.0f;
     }
+    if (in) store_gradient<D, V, kVec>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, c);
   }
 }
 

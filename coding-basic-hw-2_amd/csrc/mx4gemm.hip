@@ -1,7 +1,14 @@
 // mx4gemm.hip -- grouped products of microscaled 4-bit matrices (include/ggemm_mx4.h).
 //
-// C = A B^T by v_mfma_scale_f32_32x32x64_f8f6f4: lane l holds 32 codes (one block, 16 bytes) of row
-// l % 32 at k block l / 32 and that block's scale byte; products of codes are exact, sums are 32-bit.
+// C = A B^T on the scaled matrix instructions.  v_mfma_scale_f32_32x32x64_f8f6f4: lane l holds 32 codes (one block, 16
+// bytes) of row l % 32 at block l / 32 of two, and that block's scale byte, one of the four bytes of a register
+// that the instruction names; products of codes are exact, sums are 32-bit.  The operands are given in the
+// order B, A, so that a lane gets four neighbouring columns of one row of C.
+// Rates, from registers only with random codes: 32x32x64 6.5 PFLOP/s, 16x16x128 5.8 (zeros: 9.6 and 7.3; the
+// card lowers its clock under the products' power), so the tiles use the former.
+// Bound: 256 x 256 tiles over a long inner dimension, that power (8192 x 8192 x 16384: 499 us, 4.4 PFLOP/s, at 1.85
+// GHz with the matrix cores busy 53 % of the cycles; all zeros 403 us at 2.46 GHz); over a short one, also the
+// stores of C (8192 x 8192 x 1024: 59 us); few rows, the bytes of B.
 #include <algorithm>
 #include <type_traits>
 
@@ -100,7 +107,7 @@ __device__ __forceinline__ void store_run(T* c, const float (&v)[N], const Out& 
 // barrier and the first reads of stage s + 1.
 // Scale bytes come in windows of 32 per row (four stages), two windows in LDS: the compute unit's line
 // requests bound this kernel, and 8 bytes of every row per stage took as many as the codes (256 x 256 tiles,
-// 8192 x 8192 x 16384: %%SCALE%%).
+// 8192 x 8192 x 16384: 541 us, with windows 525).
 // LDS: chunk c (16 bytes, one block's codes) of row r lies at position c ^ (r / 2) % 8 of the row, so that the 16
 // rows of a group of lanes reading one chunk hit all banks.  Step t of a stage takes block t of the
 // stage's first four from lanes 0-31 and block 4 + t from lanes 32-63 (any pairing will do as long as
@@ -312,24 +319,33 @@ __device__ __forceinline__ void tile_store(uint8_t* lds, const Out& o, typename 
         st[(lane & 31) * Q + ((8 * j + 2 * q + (lane >> 5)) ^ (lane & (Q - 1)))] =
             f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     if (i == 0) landed();
+    if constexpr (kVec) {
 #pragma unroll 2
-    for (int r = lane / LR; r < 32; r += RI) {
-      const int row = r0 + 32 * i + r;
-      float v[E];
+      for (int r = lane / LR; r < 32; r += RI) {
+        const int row = r0 + 32 * i + r;
+        float v[E];
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const f32x4 u = st[r * Q + (((lane % LR) * (E / 4) + e / 4) ^ (r & (Q - 1)))];
+        for (int e = 0; e < E; e += 4) {
+          const f32x4 u = st[r * Q + (((lane % LR) * (E / 4) + e / 4) ^ (r & (Q - 1)))];
 #pragma unroll
-        for (int z = 0; z < 4; ++z) v[e + z] = u[z];
+          for (int z = 0; z < 4; ++z) v[e + z] = u[z];
+        }
+        if (row >= m_rem) continue;
+        T* const out = c + (int64_t)row * o.ldc + c0;
+        if (c0 + E <= n_rem) {
+          store_run<T, E>(out, v, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (c0 + e < n_rem) store_one(out + e, v[e], o);
+        }
       }
-      if (row >= m_rem) continue;
-      T* const out = c + (int64_t)row * o.ldc + c0;
-      if (kVec && c0 + E <= n_rem) {
-        store_run<T, E>(out, v, o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (c0 + e < n_rem) store_one(out + e, v[e], o);
+    } else {   // rows of C that are not aligned: neighbouring lanes, neighbouring columns
+#pragma unroll 4
+      for (int x = lane; x < 32 * W; x += 64) {
+        const int r = x / W, col = x % W, row = r0 + 32 * i + r;
+        const float v = reinterpret_cast<const float*>(st + r * Q + ((col >> 2) ^ (r & (Q - 1))))[col & 3];
+        if (row < m_rem && wn * W + col < n_rem) store_one(c + (int64_t)row * o.ldc + wn * W + col, v, o);
       }
     }
   }
@@ -579,10 +595,11 @@ struct Way {
 //   group 4.2 / 6.5, 8 groups (256 tiles) 8.3 / 8.5, 16 groups 15.3 / 13.6
 //   32 x 128 or 128 x 128 tiles: up to 64 rows a group on average.  64 groups of 4096 x 2048: 64 rows each 66 /
 //   80, 128 rows 117 / 88
-//   256 x 256 tiles (one workgroup a compute unit) as soon as there is one for every compute unit.
-//   32768 rows: %%BIG%%
+//   128 x 128 or 256 x 256 tiles (one workgroup a compute unit): where the latter make two rounds, half a tile
+//   added for every group.  16 groups of n x 1024 weights: n = 2048, 8192 rows in all 18.3 / 17.7, 12288 rows 26 / 31,
+//   16384 rows 35 / 30; n = 4096, 8192 rows 33 / 31, 32768 rows 119 / 99
 //   parts of the inner dimension: fewer tiles than compute units, so that two tiles' worth per compute unit
-//   run, each part four stages or more.  64 rows, 1024 x 16384: 27 / %%SPLIT%%
+//   run, each part four stages or more.  64 rows, 1024 x 16384: 27 us whole, 15.5 in parts
 Way way_of(const ggemm_mx4_gemm_t& p) {
   const int64_t widest = std::max(std::max(p.lda, p.ldb), std::max(p.lda_scales, p.ldb_scales));
   const bool inner = p.form == GGEMM_MX4_INNER;
@@ -590,8 +607,9 @@ Way way_of(const ggemm_mx4_gemm_t& p) {
   if (widest > kMaxLd || (p.m <= 16 * groups && thin <= kCus)) return Way{16, 1, tiles_of(p, 16, 32)};
   Way w{32, 1, thin};
   if (p.m > 64 * groups) {
-    w = Way{256, 1, tiles_of(p, 256, 256)};
-    if (w.tiles < kCus) w = Way{128, 1, tiles_of(p, 128, 128)};
+    const int64_t big = tiles_of(p, 256, 256), nt = ceil_div(p.n, 256);
+    const int64_t likely = inner || !p.offsets ? big : (2 * (int64_t)p.m / 256 + p.groups) * nt / 2;
+    w = likely >= 2 * kCus ? Way{256, 1, big} : Way{128, 1, tiles_of(p, 128, 128)};
   }
   const int64_t runs = ceil_div(p.k, 256) / (inner ? p.groups : 1);
   if (w.tiles < kCus) w.splits = (int)std::max<int64_t>(1, std::min(2 * kCus / w.tiles, runs / 4));
@@ -600,9 +618,11 @@ Way way_of(const ggemm_mx4_gemm_t& p) {
 
 template <class C, int D, bool kInner, bool kVec>
 void launch_tiles(const ggemm_mx4_gemm_t& p, const Way& w, float* parts, hipStream_t s) {
-  if (w.splits > 1) {
-    gemm_tile_kernel<C, D, kInner, kVec, true><<<dim3((unsigned)w.tiles, w.splits), C::NT, 0, s>>>(p, (int)w.tiles, parts);
-    join_kernel<C, D, kInner><<<dim3((unsigned)w.tiles, C::BM / 8), 256, 0, s>>>(p, (int)w.tiles, w.splits, parts);
+  if (C::BM < 256 && w.splits > 1) {
+    if constexpr (C::BM < 256) {
+      gemm_tile_kernel<C, D, kInner, kVec, true><<<dim3((unsigned)w.tiles, w.splits), C::NT, 0, s>>>(p, (int)w.tiles, parts);
+      join_kernel<C, D, kInner><<<dim3((unsigned)w.tiles, C::BM / 8), 256, 0, s>>>(p, (int)w.tiles, w.splits, parts);
+    }
   } else {
     const int64_t at_once = (int64_t)kCus * 4 * C::WAVES / C::NW;
     gemm_tile_kernel<C, D, kInner, kVec, false>

@@ -1,10 +1,15 @@
 """What the 4-bit operators and the router refuse, and what they accept without work: all decided on the
 host before anything is launched (no GPU here; the pointers are never followed)."""
 import ctypes as C
+import sys
+from pathlib import Path
 
 import pytest
 
 import ggemm as G
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "coding-basic-hw-2_amd" / "apps"))
+import moe_mx4   # noqa: E402
 
 P = 0x7f0000000000      # an address, aligned to everything
 
@@ -118,3 +123,11 @@ def test_route_workspace():
     assert router("backward", tokens=0) == G.GGEMM_OK
     assert G.lib().ggemm_route(None, P, 1 << 30, None) == G.GGEMM_ERR_INVALID
     assert G.lib().ggemm_route_backward(None, P, P, P, 16, None) == G.GGEMM_ERR_INVALID
+
+
+@pytest.mark.parametrize("bad", [["--tokens", "0"], ["--topk", "17"], ["--topk", "0"], ["--d-model", "100"], ["--d-ff", "64"],
+                                 ["--experts", "2000"], ["--steps", "0"]])
+def test_app_refuses(bad, capsys):
+    with pytest.raises(SystemExit):
+        moe_mx4.parse_args(bad)
+    assert "error" in capsys.readouterr().err

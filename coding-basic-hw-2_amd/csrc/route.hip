@@ -23,9 +23,6 @@
 namespace ggemm {
 namespace {
 
-#ifndef SPAN
-#define SPAN 128
-#endif
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -37,13 +34,14 @@ struct RouteWs {
   int* used;     // groups
 };
 
+constexpr int kFewGroups = 128;   // workgroups of the first launch up to which there is no second one
 struct Shape {
   int span, groups;
 };
 // Tokens a workgroup takes (a multiple of 32: whole words of the bit table).  Few tokens are spread over
 // the compute units, many take longer spans, which makes the tables of the second launch shorter.
 Shape shape_of(int tokens) {
-  const int span = tokens <= 65536 ? 64 : SPAN;
+  const int span = tokens <= 64 ? 64 : tokens <= 4096 ? 32 : tokens <= 65536 ? 64 : 128;
   return Shape{span, tokens > 0 ? ceil_div(tokens, span) : 1};
 }
 
@@ -146,6 +144,11 @@ struct Logits {
   __device__ __forceinline__ bool on(int t, int t1) const { return t < t1 && mask; }   // the token takes part
   __device__ __forceinline__ typename P::T at(int v) const { return w[v / P::N].x[v % P::N]; }
 };
+template <class P>
+__device__ __forceinline__ void store_streaming(const P& w, void* p) {
+  typedef unsigned short half_words __attribute__((ext_vector_type(sizeof(P) / 2)));
+  __builtin_nontemporal_store(__builtin_bit_cast(half_words, w), static_cast<half_words*>(p));
+}
 template <int D, int V, bool kVec>
 __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, int experts, const float (&g)[V]) {
   using P = Piece<D, V>;
@@ -155,7 +158,7 @@ __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, i
       typename P::Type w;
 #pragma unroll
       for (int j = 0; j < P::N; ++j) w.x[j] = (typename P::T)g[i + j];
-      *reinterpret_cast<typename P::Type*>(p + e0 + i) = w;
+      store_streaming(w, p + e0 + i);
     }
   } else {
 #pragma unroll
@@ -200,8 +203,9 @@ __device__ __forceinline__ void write_loss(const ggemm_router_t& r, const int* c
 }
 
 // Exclusive sums over experts of the counts rounded up to row_align, into off[0 .. experts]; called by
-// the whole workgroup (at most 4 experts a thread), ends with a barrier.
+// the whole workgroup (its first kThreads threads, 4 experts each, do it), ends with a barrier.
 __device__ __forceinline__ void scan_offsets(const int* counts, int experts, int align, int* off, int* tmp) {
+  static_assert(GGEMM_ROUTE_MAX_EXPERTS == 4 * kThreads, "experts a thread");
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int c[4], sum = 0;
 #pragma unroll
@@ -216,33 +220,38 @@ __device__ __forceinline__ void scan_offsets(const int* counts, int experts, int
     const int up = __shfl_up(inc, d);
     inc += lane >= d ? up : 0;
   }
-  if (lane == 63) tmp[wave] = inc;
+  if (lane == 63 && tid < kThreads) tmp[wave] = inc;
   __syncthreads();
-  int at = inc - sum;
-  for (int w = 0; w < wave; ++w) at += tmp[w];
+  if (tid < kThreads) {
+    int at = inc - sum;
+    for (int w = 0; w < wave; ++w) at += tmp[w];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (4 * tid + i <= experts) off[4 * tid + i] = at;
-    at += c[i];
+    for (int i = 0; i < 4; ++i) {
+      if (4 * tid + i <= experts) off[4 * tid + i] = at;
+      at += c[i];
+    }
+    if (tid == kThreads - 1 && experts == 4 * kThreads) off[experts] = at;
   }
-  if (tid == kThreads - 1 && experts == 4 * kThreads) off[experts] = at;
   __syncthreads();
 }
 
 // First launch: choices, gates, ranks within the workgroup's tokens (into pos), counts and softmax sums
 // per workgroup.  kOne: the only workgroup, which finishes the call.
+// (kOne: 16 waves, as long as their sums fit, for the latency of one call)
+__host__ __device__ constexpr int first_threads(int experts, bool one) { return one && experts <= 256 ? 1024 : kThreads; }
 template <int D, int L, int V, bool kOne, bool kVec>
-__global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, RouteWs ws, int span) {
-  constexpr int kRows = 64 / L, kPar = 4 * kRows;   // tokens a wave and a workgroup hold at a time
+__global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm_router_t r, RouteWs ws, int span) {
+  constexpr int NT = first_threads(L * V, kOne), NW = NT / 64;
+  constexpr int kRows = 64 / L, kPar = NW * kRows;   // tokens a wave and a workgroup hold at a time
   extern __shared__ uint32_t lds[];
   const int words = span / 32, E = r.experts, K = r.topk;
   uint32_t* bits = lds;                                        // E x words
-  float* part = reinterpret_cast<float*>(lds + E * words);     // 4 x (L V): the waves' softmax sums
-  __shared__ int s_used[4];
+  float* part = reinterpret_cast<float*>(lds + E * words);     // NW x (L V): the waves' softmax sums
+  __shared__ int s_used[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = sub * V;
   const int t0 = blockIdx.x * span, t1 = min(t0 + span, r.tokens);
-  for (int i = tid; i < E * words; i += kThreads) bits[i] = 0;
+  for (int i = tid; i < E * words; i += NT) bits[i] = 0;
   __syncthreads();
   float acc[V];
 #pragma unroll
@@ -356,9 +365,11 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
   used = over_lanes<64>(used, [](int a, int b) { return a + b; });
   if (lane == 0) s_used[wave] = used;
   __syncthreads();
-  used = s_used[0] + s_used[1] + s_used[2] + s_used[3];
+  used = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) used += s_used[w];
   // ranks, counts
-  for (int i = tid; i < (t1 - t0) * K; i += kThreads) {
+  for (int i = tid; i < (t1 - t0) * K; i += NT) {
     const int64_t at = (int64_t)t0 * K + i;
     const int e = r.ids[at], t = i / K;
     int rank = -1;
@@ -369,10 +380,12 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
     r.pos[at] = rank;
   }
   __shared__ int s_off[kOne ? GGEMM_ROUTE_MAX_EXPERTS + 1 : 1], s_tmp[4];
-  for (int e = tid; e < E; e += kThreads) {
+  for (int e = tid; e < E; e += NT) {
     int c = 0;
     for (int w = 0; w < words; ++w) c += __popc(bits[e * words + w]);
-    const float ps = part[e] + part[L * V + e] + part[2 * L * V + e] + part[3 * L * V + e];
+    float ps = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) ps += part[w * L * V + e];
     if constexpr (kOne) {
       r.counts[e] = c;
       r.probs[e] = used ? ps / (float)used : 0.0f;
@@ -386,8 +399,8 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
   } else {
     __syncthreads();
     scan_offsets(r.counts, E, r.row_align, s_off, s_tmp);
-    for (int e = tid; e <= E; e += kThreads) r.offsets[e] = s_off[e];
-    for (int i = tid; i < r.tokens * K; i += kThreads) {
+    for (int e = tid; e <= E; e += NT) r.offsets[e] = s_off[e];
+    for (int i = tid; i < r.tokens * K; i += NT) {
       const int e = r.ids[i];
       if (e >= 0) {
         const int row = s_off[e] + r.pos[i];
@@ -395,9 +408,9 @@ __global__ void __launch_bounds__(kThreads) route_kernel(ggemm_router_t r, Route
         if (row < r.max_rows) r.order[row] = i / K;
       }
     }
-    for (int e = tid; e < E; e += kThreads)
+    for (int e = tid; e < E; e += NT)
       if (r.row_align > 1) pad_order(r, s_off[e] + r.counts[e], s_off[e + 1], 0, 1);
-    pad_order(r, s_off[E], r.max_rows, tid, kThreads);
+    pad_order(r, s_off[E], r.max_rows, tid, NT);
     if (tid == 0) r.used[0] = used;
     if (wave == 0) write_loss(r, r.counts, r.probs, used);
   }
@@ -453,28 +466,81 @@ __global__ void __launch_bounds__(16 * kRuns) route_scan_kernel(ggemm_router_t r
 }
 
 // Third launch: rows of the pairs, order, padding, loss.  Workgroup b takes the pairs of workgroup b of
-// the first launch.
+// the first launch.  kScan: there was no second launch; every workgroup sums the tables for itself (experts <=
+// kThreads), which few workgroups do faster than a launch of its own takes (4096 tokens, 16 experts: 2 us).
+template <bool kScan>
 __global__ void __launch_bounds__(kThreads) route_place_kernel(ggemm_router_t r, RouteWs ws, int span) {
   __shared__ int s_off[GGEMM_ROUTE_MAX_EXPERTS + 1], s_tmp[4];
+  __shared__ int s_cnt[kThreads], s_rank[kThreads];
+  __shared__ float s_p[kThreads];
   const int tid = threadIdx.x, E = r.experts, K = r.topk;
-  scan_offsets(r.counts, E, r.row_align, s_off, s_tmp);
+  const int* counts = r.counts;
+  const int* rank = ws.hist + (int64_t)blockIdx.x * E;
+  const float* probs = r.probs;
+  int used = 0;
+  if constexpr (kScan) {
+    int lanes = 1;   // threads along the experts, the others along the workgroups of the first launch
+    while (lanes < E) lanes *= 2;
+    const int e = tid & (lanes - 1), c = tid / lanes, runs = kThreads / lanes, groups = gridDim.x;
+    int cnt = 0, before = 0;
+    float ps = 0.0f;
+    if (e < E) {
+#pragma unroll 4
+      for (int g = c; g < groups; g += runs) {
+        const int n = ws.hist[(int64_t)g * E + e];
+        cnt += n;
+        before += g < (int)blockIdx.x ? n : 0;
+        ps += ws.psum[(int64_t)g * E + e];
+      }
+    }
+    for (int g = tid; g < groups; g += kThreads) used += ws.used[g];
+    used = over_lanes<64>(used, [](int a, int b) { return a + b; });
+    if ((tid & 63) == 0) s_tmp[tid >> 6] = used;
+    s_cnt[tid] = cnt;
+    s_rank[tid] = before;
+    s_p[tid] = ps;
+    __syncthreads();
+    used = s_tmp[0] + s_tmp[1] + s_tmp[2] + s_tmp[3];
+    if (tid < lanes) {
+      for (int q = 1; q < runs; ++q) {
+        cnt += s_cnt[q * lanes + tid];
+        before += s_rank[q * lanes + tid];
+        ps += s_p[q * lanes + tid];
+      }
+      s_cnt[tid] = cnt;
+      s_rank[tid] = before;
+      s_p[tid] = used ? ps / (float)used : 0.0f;
+    }
+    __syncthreads();
+    counts = s_cnt;
+    rank = s_rank;
+    probs = s_p;
+  }
+  scan_offsets(counts, E, r.row_align, s_off, s_tmp);
   const int t0 = blockIdx.x * span, t1 = min(t0 + span, r.tokens);
   for (int i = tid; i < (t1 - t0) * K; i += kThreads) {
     const int64_t at = (int64_t)t0 * K + i;
     const int e = r.ids[at];
     if (e >= 0) {
-      const int row = s_off[e] + ws.hist[(int64_t)blockIdx.x * E + e] + r.pos[at];
+      const int row = s_off[e] + rank[e] + r.pos[at];
       r.pos[at] = row;
       if (row < r.max_rows) r.order[row] = t0 + i / K;
     }
   }
   const int all = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
   if (r.row_align > 1)
-    for (int e = me; e < E; e += all) pad_order(r, s_off[e] + r.counts[e], s_off[e + 1], 0, 1);
+    for (int e = me; e < E; e += all) pad_order(r, s_off[e] + counts[e], s_off[e + 1], 0, 1);
   pad_order(r, s_off[E], r.max_rows, me, all);
   if (blockIdx.x == 0) {
     for (int e = tid; e <= E; e += kThreads) r.offsets[e] = s_off[e];
-    if (tid < 64) write_loss(r, r.counts, r.probs, r.used[0]);
+    if constexpr (kScan) {
+      if (tid < E) {
+        r.counts[tid] = counts[tid];
+        r.probs[tid] = probs[tid];
+      }
+      if (tid == 0) r.used[0] = used;
+    }
+    if (tid < 64) write_loss(r, counts, probs, kScan ? used : r.used[0]);
   }
 }
 
@@ -640,10 +706,11 @@ int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
   with_elem(r->dtype, [&](auto d) {
     with_lanes(r->experts, [&](auto l, auto v) {
       constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
-      const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + 4 * L * V * 4;
       constexpr int A = sizeof(typename Piece<D, V>::Type);
       auto go = [&](auto one, auto vec) {
-        route_kernel<D, L, V, decltype(one)::value, decltype(vec)::value><<<sh.groups, kThreads, lds, s>>>(*r, w, sh.span);
+        constexpr int NT = first_threads(L * V, decltype(one)::value);
+        const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + NT / 64 * L * V * 4;
+        route_kernel<D, L, V, decltype(one)::value, decltype(vec)::value><<<sh.groups, NT, lds, s>>>(*r, w, sh.span);
       };
       using std::true_type;
       using std::false_type;
@@ -653,8 +720,12 @@ int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
     });
   });
   if (sh.groups > 1) {
-    route_scan_kernel<<<ceil_div(r->experts, 16), 16 * kRuns, 0, s>>>(*r, w, sh.groups);
-    route_place_kernel<<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+    if (r->experts <= kThreads && sh.groups <= kFewGroups) {
+      route_place_kernel<true><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+    } else {
+      route_scan_kernel<<<ceil_div(r->experts, 16), 16 * kRuns, 0, s>>>(*r, w, sh.groups);
+      route_place_kernel<false><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+    }
   }
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
 }

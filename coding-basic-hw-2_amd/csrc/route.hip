@@ -1,7 +1,8 @@
 // route.hip -- the router of a mixture-of-experts layer (include/ggemm_route.h).
 //
-// A token's logits lie in L lanes of one wave, V consecutive experts to a lane (L V >= experts, L a power
-// of two, 64 / L tokens a wave), in registers from the load to the last use.  Selection works on
+// A token's logits lie in L lanes of one wave, V experts to a lane (L V >= experts, L a power of two, 64 / L tokens
+// a wave), in registers from the load to the last use: in pieces of up to 16 bytes, piece c of lane l at piece
+// c L + l of the row, so that the lanes of a load or store lie side by side.  Selection works on
 // integer keys that order like the logits (NaN highest, barred experts 0): per place a maximum over the
 // lane's keys and then over the L lanes.  16-bit logits have the expert's number, inverted, in the key's low
 // half, so that a key is unique and tells the expert to all lanes, and the next place is the largest of
@@ -118,11 +119,15 @@ struct Piece {
   using T = typename Elem<D>::T;
   static constexpr int N = V * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : V;
   struct alignas(N * sizeof(T)) Type { T x[N]; };
+  // the expert of a lane's value v, less that of its value 0; and that one
+  template <int L>
+  static __device__ __forceinline__ constexpr int step(int v) { return v / N * L * N + v % N; }
+  static __device__ __forceinline__ int first(int lane) { return lane * N; }
 };
-// The lane's V logits of token t (experts e0 ...; -inf past the last expert), as they lie in memory: a wave has the
+// The lane's V logits of token t (from expert e0 on; -inf past the last expert), as they lie in memory: a wave has the
 // next tokens' on the way while it works on these (131072 x 256 bf16, forward %%F%%, backward %%B%% us).  Those of a token
 // that is left out are read and not used.
-template <int D, int V>
+template <int D, int L, int V>
 struct Logits {
   using P = Piece<D, V>;
   typename P::Type w[V / P::N];
@@ -133,12 +138,16 @@ struct Logits {
     if (t >= t1) return;
     mask = r.mask ? r.mask[t] : 1;
     const T* p = static_cast<const T*>(r.logits) + (int64_t)t * r.ld + e0;
-    if (kVec && e0 + V <= r.experts) {
 #pragma unroll
-      for (int i = 0; i < V / P::N; ++i) w[i] = *reinterpret_cast<const typename P::Type*>(p + i * P::N);
-    } else {
+    for (int i = 0; i < V / P::N; ++i) {
+      constexpr int N = P::N;
+      const int at = i * L * N;
+      if (kVec && e0 + at + N <= r.experts) {
+        w[i] = *reinterpret_cast<const typename P::Type*>(p + at);
+      } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) w[v / P::N].x[v % P::N] = e0 + v < r.experts ? p[v] : (T)-__builtin_inff();
+        for (int j = 0; j < N; ++j) w[i].x[j] = e0 + at + j < r.experts ? p[at + j] : (T)-__builtin_inff();
+      }
     }
   }
   __device__ __forceinline__ bool on(int t, int t1) const { return t < t1 && mask; }   // the token takes part
@@ -149,21 +158,23 @@ __device__ __forceinline__ void store_streaming(const P& w, void* p) {
   typedef unsigned short half_words __attribute__((ext_vector_type(sizeof(P) / 2)));
   __builtin_nontemporal_store(__builtin_bit_cast(half_words, w), static_cast<half_words*>(p));
 }
-template <int D, int V, bool kVec>
+template <int D, int L, int V, bool kVec>
 __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, int experts, const float (&g)[V]) {
   using P = Piece<D, V>;
-  if (kVec && e0 + V <= experts) {
+  constexpr int N = P::N;
 #pragma unroll
-    for (int i = 0; i < V; i += P::N) {
-      typename P::Type w;
+  for (int i = 0; i < V / N; ++i) {
+    const int at = e0 + i * L * N;
+    typename P::Type w;
 #pragma unroll
-      for (int j = 0; j < P::N; ++j) w.x[j] = (typename P::T)g[i + j];
-      store_streaming(w, p + e0 + i);
+    for (int j = 0; j < N; ++j) w.x[j] = (typename P::T)g[i * N + j];
+    if (kVec && at + N <= experts) {
+      store_streaming(w, p + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (at + j < experts) p[at + j] = w.x[j];
     }
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (e0 + v < experts) p[e0 + v] = (typename P::T)g[v];
   }
 }
 
@@ -241,6 +252,7 @@ __device__ __forceinline__ void scan_offsets(const int* counts, int experts, int
 __host__ __device__ constexpr int first_threads(int experts, bool one) { return one && experts <= 256 ? 1024 : kThreads; }
 template <int D, int L, int V, bool kOne, bool kVec>
 __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm_router_t r, RouteWs ws, int span) {
+  using P = Piece<D, V>;
   constexpr int NT = first_threads(L * V, kOne), NW = NT / 64;
   constexpr int kRows = 64 / L, kPar = NW * kRows;   // tokens a wave and a workgroup hold at a time
   extern __shared__ uint32_t lds[];
@@ -249,7 +261,7 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
   float* part = reinterpret_cast<float*>(lds + E * words);     // NW x (L V): the waves' softmax sums
   __shared__ int s_used[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = sub * V;
+  const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = P::first(sub);
   const int t0 = blockIdx.x * span, t1 = min(t0 + span, r.tokens);
   for (int i = tid; i < E * words; i += NT) bits[i] = 0;
   __syncthreads();
@@ -257,7 +269,7 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
   int used = 0;
-  Logits<D, V> ahead;
+  Logits<D, L, V> ahead;
   ahead.template load<kVec>(r, t0 + slot, t1, e0);
   for (int tb = t0; tb < t1; tb += kPar) {
     const int t = tb + slot;
@@ -268,7 +280,7 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
 #pragma unroll
     for (int v = 0; v < V; ++v) x[v] = (float)ahead.at(v);
     // 16-bit keys: order, then a number that falls with the expert's: within the lane here, the lane's later
-    constexpr uint32_t kIn = V - 1;
+    constexpr uint32_t kIn = P::template step<L>(V - 1);
     const uint32_t lane_part = 0xffffu - e0 - kIn;
     if constexpr (D == GGEMM_F32) {
 #pragma unroll
@@ -281,8 +293,8 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
         const uint32_t w = __builtin_bit_cast(uint32_t, pair{ahead.at(v), ahead.at(v + 1 < V ? v + 1 : v)});
         worst = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, worst), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
         const uint32_t o = order16<D>(w);
-        key[v] = o << 16 | (kIn - v);
-        if (v + 1 < V) key[v + 1] = (o & 0xffff0000u) | (kIn - v - 1);
+        key[v] = o << 16 | (kIn - P::template step<L>(v));
+        if (v + 1 < V) key[v + 1] = (o & 0xffff0000u) | (kIn - P::template step<L>(v + 1));
       }
       if (__ballot(max(worst & 0xffffu, worst >> 16) > Half<D>::kInf)) {
         asm volatile("");   // a branch, not a select per value
@@ -302,10 +314,10 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
         best = max_lanes<L>(top);
         uint32_t e = 0xffffffffu;
 #pragma unroll
-        for (int v = V - 1; v >= 0; --v) e = key[v] == best ? e0 + v : e;
+        for (int v = V - 1; v >= 0; --v) e = key[v] == best ? e0 + P::template step<L>(v) : e;
         expert = (int)min_lanes<L>(e);
 #pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = expert == e0 + v ? 0u : key[v];
+        for (int v = 0; v < V; ++v) key[v] = expert == e0 + P::template step<L>(v) ? 0u : key[v];
       } else {
         const uint32_t from = best - lane_part;
         uint32_t top = key[0] - from;
@@ -360,7 +372,7 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
   for (int v = 0; v < V; ++v) {
 #pragma unroll
     for (int d = L; d < 64; d *= 2) acc[v] += __shfl_xor(acc[v], d);
-    if (lane < L) part[wave * L * V + e0 + v] = acc[v];
+    if (lane < L) part[wave * L * V + e0 + P::template step<L>(v)] = acc[v];
   }
   used = over_lanes<64>(used, [](int a, int b) { return a + b; });
   if (lane == 0) s_used[wave] = used;
@@ -552,10 +564,11 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
                                                                   const float* __restrict__ d_loss, void* d_logits,
                                                                   int64_t ld_d, int per) {
   using T = typename Elem<D>::T;
+  using P = Piece<D, V>;
   constexpr int kRows = 64 / L, kPar = 4 * kRows;
   __shared__ float s_row[kPar * L * V];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = sub * V, E = r.experts, K = r.topk;
+  const int sub = lane & (L - 1), slot = wave * kRows + lane / L, e0 = P::first(sub), E = r.experts, K = r.topk;
   float* row = s_row + slot * L * V;
   const int used = r.used[0];
   const float n = (float)used;
@@ -563,8 +576,9 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
   float s[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    s[v] = e0 + v < E ? f * (float)r.counts[e0 + v] : 0.0f;
-    row[e0 + v] = 0.0f;
+    const int e = e0 + P::template step<L>(v);
+    s[v] = e < E ? f * (float)r.counts[e] : 0.0f;
+    row[e] = 0.0f;
   }
   const int t0 = blockIdx.x * per, t1 = min(t0 + per, r.tokens);
   // a place of a token: its expert (-1: none), gate and the gate's gradient
@@ -584,7 +598,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     }
     return c;
   };
-  Logits<D, V> ahead;
+  Logits<D, L, V> ahead;
   ahead.template load<kVec>(r, t0 + slot, t1, e0);
   Choice next = choice(t0 + slot, sub);
   for (int tb = t0; tb < t1; tb += kPar) {
@@ -621,7 +635,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     __threadfence_block();
     float c[V], ps = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) c[v] = row[e0 + v];
+    for (int v = 0; v < V; ++v) c[v] = row[e0 + P::template step<L>(v)];
     if (!live) {
 #pragma unroll
       for (int v = 0; v < V; ++v) p[v] = 0.0f;
@@ -646,7 +660,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     }
     __threadfence_block();
 #pragma unroll
-    for (int v = 0; v < V; ++v) row[e0 + v] = 0.0f;
+    for (int v = 0; v < V; ++v) row[e0 + P::template step<L>(v)] = 0.0f;
     __threadfence_block();
     // 0 times a NaN or infinite sum is not the 0 of a barred expert or of a token left out
     if (__ballot(!live || !(fabsf(ps) < 1e30f))) {
@@ -654,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
 #pragma unroll
       for (int v = 0; v < V; ++v) c[v] = live && x[v] != -__builtin_inff() ? c[v] : 0.0f;
     }
-    if (in) store_gradient<D, V, kVec>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, c);
+    if (in) store_gradient<D, L, V, kVec>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, c);
   }
 }
 

@@ -35,6 +35,40 @@ inline void with_elem(int dtype, F&& f) {
   else f(std::integral_constant<int, GGEMM_F16>{});
 }
 
+// N values of type T side by side, loaded or stored as one vector at any address that suits one of them: the memory
+// instructions take that, so that rows of odd length need no path of their own (results of a product, 20993 x 4062 bf16: 123 us value by
+// value, 72 this way).
+template <class T, int N>
+struct Run {
+  typedef uint32_t words __attribute__((ext_vector_type(N * sizeof(T) / 4)));
+  typedef words at_any __attribute__((aligned(sizeof(T))));
+  T x[N];
+  static __device__ __forceinline__ Run load(const T* p) {
+    return __builtin_bit_cast(Run, (words)*reinterpret_cast<const at_any*>(p));
+  }
+  // kStream: non-temporally
+  template <bool kStream>
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kStream) __builtin_nontemporal_store(__builtin_bit_cast(words, *this), reinterpret_cast<at_any*>(p));
+    else *reinterpret_cast<at_any*>(p) = __builtin_bit_cast(words, *this);
+  }
+};
+// one 16-bit value
+template <>
+struct Run<__bf16, 1> {
+  __bf16 x[1];
+  static __device__ __forceinline__ Run load(const __bf16* p) { return Run{{*p}}; }
+  template <bool>
+  __device__ __forceinline__ void store(__bf16* p) const { *p = x[0]; }
+};
+template <>
+struct Run<_Float16, 1> {
+  _Float16 x[1];
+  static __device__ __forceinline__ Run load(const _Float16* p) { return Run{{*p}}; }
+  template <bool>
+  __device__ __forceinline__ void store(_Float16* p) const { *p = x[0]; }
+};
+
 // The scale byte s as a number: 2^(s - 127), exact (s = 0 is the subnormal 2^-127); s < 255.
 __device__ __forceinline__ float mx4_scale(uint32_t s) { return __uint_as_float(s ? s << 23 : 1u << 22); }
 

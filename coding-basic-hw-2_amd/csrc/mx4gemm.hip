@@ -79,23 +79,24 @@ __device__ __forceinline__ void store_one(T* c, float v, const Out& o) {
   if (o.beta != 0.0f) v += o.beta * (float)*c;
   *c = (T)v;
 }
-// N = 16 / sizeof(T) (or half of it) values side by side, c aligned to them.  The stores are non-temporal: C is not
-// read here again and would push the operands out of L2 (32 groups of 2048 x 4096 x 4096: 701 -> 623 us).
-template <class T, int N>
+// N values side by side.  kStream: non-temporal stores, for a C of more than the 256 MB of the last-level cache whose rows begin at a multiple
+// of 64 bytes: they leave the operands in the caches (32 groups of 2048 x 4096, 32-bit results, 1 GB, inner 32768 in
+// all: 358 -> 257 us), but a smaller C is stored faster into the cache (8192 x 8192 bf16, k = 1024: 52 / 55), and a
+// line stored in parts has to be read first (20993 x 4062 bf16: 72 / 109).
+template <bool kStream, class T, int N>
 __device__ __forceinline__ void store_run(T* c, const float (&v)[N], const Out& o) {
-  typedef uint32_t words __attribute__((ext_vector_type(N * sizeof(T) / 4)));
-  struct alignas(N * sizeof(T)) Run { T x[N]; } w;
+  Run<T, N> w;
   float u[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) u[e] = o.alpha * v[e];
   if (o.beta != 0.0f) {
-    w = *reinterpret_cast<const Run*>(c);
+    w = Run<T, N>::load(c);
 #pragma unroll
     for (int e = 0; e < N; ++e) u[e] += o.beta * (float)w.x[e];
   }
 #pragma unroll
   for (int e = 0; e < N; ++e) w.x[e] = (T)u[e];
-  __builtin_nontemporal_store(__builtin_bit_cast(words, w), reinterpret_cast<words*>(c));
+  w.template store<kStream>(c);
 }
 
 // ---------------------------------------------------------------- tiles through LDS
@@ -300,7 +301,7 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, const Source<C>& src
 // 16-byte piece q of row r lies at q ^ r % (pieces of a row), which spreads both the writes and the reads over
 // the banks), then stores whole 16-byte pieces along C's rows.
 // Before the first store it waits for the transfers in flight, the next tile's first stage.
-template <class C, int D, bool kVec>
+template <class C, int D, bool kStream>
 __device__ __forceinline__ void tile_store(uint8_t* lds, const Out& o, typename Elem<D>::T* c, int m_rem, int n_rem,
                                            const f32x16 (&acc)[C::FM][C::FN]) {
   using T = typename Elem<D>::T;
@@ -319,33 +320,24 @@ __device__ __forceinline__ void tile_store(uint8_t* lds, const Out& o, typename 
         st[(lane & 31) * Q + ((8 * j + 2 * q + (lane >> 5)) ^ (lane & (Q - 1)))] =
             f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     if (i == 0) landed();
-    if constexpr (kVec) {
 #pragma unroll 2
-      for (int r = lane / LR; r < 32; r += RI) {
-        const int row = r0 + 32 * i + r;
-        float v[E];
+    for (int r = lane / LR; r < 32; r += RI) {
+      const int row = r0 + 32 * i + r;
+      float v[E];
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const f32x4 u = st[r * Q + (((lane % LR) * (E / 4) + e / 4) ^ (r & (Q - 1)))];
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 u = st[r * Q + (((lane % LR) * (E / 4) + e / 4) ^ (r & (Q - 1)))];
 #pragma unroll
-          for (int z = 0; z < 4; ++z) v[e + z] = u[z];
-        }
-        if (row >= m_rem) continue;
-        T* const out = c + (int64_t)row * o.ldc + c0;
-        if (c0 + E <= n_rem) {
-          store_run<T, E>(out, v, o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (c0 + e < n_rem) store_one(out + e, v[e], o);
-        }
+        for (int z = 0; z < 4; ++z) v[e + z] = u[z];
       }
-    } else {   // rows of C that are not aligned: neighbouring lanes, neighbouring columns
-#pragma unroll 4
-      for (int x = lane; x < 32 * W; x += 64) {
-        const int r = x / W, col = x % W, row = r0 + 32 * i + r;
-        const float v = reinterpret_cast<const float*>(st + r * Q + ((col >> 2) ^ (r & (Q - 1))))[col & 3];
-        if (row < m_rem && wn * W + col < n_rem) store_one(c + (int64_t)row * o.ldc + wn * W + col, v, o);
+      if (row >= m_rem) continue;
+      T* const out = c + (int64_t)row * o.ldc + c0;
+      if (c0 + E <= n_rem) {
+        store_run<kStream>(out, v, o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (c0 + e < n_rem) store_one(out + e, v[e], o);
       }
     }
   }
@@ -400,7 +392,7 @@ __device__ __forceinline__ void take_part(int& b0, int& b1, int s, int S) {
 // Workgroup b takes tiles b, b + grid, ... of `total` (some past the last of a ragged rows form).  The next
 // tile's first stage is on its way while this one's results are stored.  kSplit: blockIdx.y is one of gridDim.y parts
 // of the inner dimension; its sums go to `parts`, tile after tile, for join_kernel.
-template <class C, int D, bool kInner, bool kVec, bool kSplit>
+template <class C, int D, bool kInner, bool kSplit, bool kStream>
 __global__ void __launch_bounds__(C::NT, C::WAVES) gemm_tile_kernel(ggemm_mx4_gemm_t p, int total, float* parts) {
   __shared__ __attribute__((aligned(128))) uint8_t tile_lds[C::SMEM];
   using T = typename Elem<D>::T;
@@ -440,10 +432,10 @@ __global__ void __launch_bounds__(C::NT, C::WAVES) gemm_tile_kernel(ggemm_mx4_ge
     }
     if constexpr (kSplit) {
       float* const c = parts + ((int64_t)blockIdx.y * total + done) * C::BM * C::BN;
-      tile_store<C, GGEMM_F32, true>(tile_lds, Out{1.0f, 0.0f, C::BN}, c, C::BM, C::BN, acc);
+      tile_store<C, GGEMM_F32, false>(tile_lds, Out{1.0f, 0.0f, C::BN}, c, C::BM, C::BN, acc);
     } else {
       T* const c = static_cast<T*>(p.c) + (kInner ? cur.g * p.c_stride : 0) + (int64_t)cur.m0 * p.ldc + cur.n0;
-      tile_store<C, D, kVec>(tile_lds, o, c, cur.m_end - cur.m0, p.n - cur.n0, acc);
+      tile_store<C, D, kStream>(tile_lds, o, c, cur.m_end - cur.m0, p.n - cur.n0, acc);
     }
     if (nxt.g < 0) return;
     cur = nxt;
@@ -480,7 +472,7 @@ __global__ void __launch_bounds__(256) join_kernel(ggemm_mx4_gemm_t p, int total
 struct FewTile {
   static constexpr int BM = 16, BN = 32;
 };
-template <int D, bool kInner, bool kVec, int NW>
+template <int D, bool kInner, int NW>
 __global__ void __launch_bounds__(64 * NW, 4) gemm_few_kernel(ggemm_mx4_gemm_t p) {
   using T = typename Elem<D>::T;
   __shared__ f32x4 sums[NW][2][64];
@@ -542,8 +534,8 @@ __global__ void __launch_bounds__(64 * NW, 4) gemm_few_kernel(ggemm_mx4_gemm_t p
   const Out o{p.alpha, p.beta, p.ldc};
   T* const c = static_cast<T*>(p.c) + (kInner ? t.g * p.c_stride : 0) + (int64_t)i * p.ldc + j;
   const float u[4] = {v[0], v[1], v[2], v[3]};
-  if (kVec && j + 4 <= p.n) {
-    store_run<T, 4>(c, u, o);
+  if (j + 4 <= p.n) {
+    store_run<false>(c, u, o);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -616,17 +608,25 @@ Way way_of(const ggemm_mx4_gemm_t& p) {
   return w;
 }
 
-template <class C, int D, bool kInner, bool kVec>
+template <class C, int D, bool kInner>
 void launch_tiles(const ggemm_mx4_gemm_t& p, const Way& w, float* parts, hipStream_t s) {
   if (C::BM < 256 && w.splits > 1) {
     if constexpr (C::BM < 256) {
-      gemm_tile_kernel<C, D, kInner, kVec, true><<<dim3((unsigned)w.tiles, w.splits), C::NT, 0, s>>>(p, (int)w.tiles, parts);
+      gemm_tile_kernel<C, D, kInner, true, false><<<dim3((unsigned)w.tiles, w.splits), C::NT, 0, s>>>(p, (int)w.tiles, parts);
       join_kernel<C, D, kInner><<<dim3((unsigned)w.tiles, C::BM / 8), 256, 0, s>>>(p, (int)w.tiles, w.splits, parts);
     }
   } else {
-    const int64_t at_once = (int64_t)kCus * 4 * C::WAVES / C::NW;
-    gemm_tile_kernel<C, D, kInner, kVec, false>
-        <<<(unsigned)std::min(w.tiles, at_once), C::NT, 0, s>>>(p, (int)w.tiles, nullptr);
+    const int es = elem_bytes(p.dtype);
+    const int64_t bytes = (int64_t)p.m * p.n * es * (kInner ? p.groups : 1);
+    const bool stream = bytes > ((int64_t)256 << 20) && aligned(p.c, 64) && p.ldc * es % 64 == 0 && p.c_stride * es % 64 == 0;
+    const unsigned grid = (unsigned)std::min(w.tiles, (int64_t)kCus * 4 * C::WAVES / C::NW);
+    if constexpr (C::BM == 256) {   // a C of that size has so many tiles unless it is very narrow
+      if (stream) {
+        gemm_tile_kernel<C, D, kInner, false, true><<<grid, C::NT, 0, s>>>(p, (int)w.tiles, nullptr);
+        return;
+      }
+    }
+    gemm_tile_kernel<C, D, kInner, false, false><<<grid, C::NT, 0, s>>>(p, (int)w.tiles, nullptr);
   }
 }
 
@@ -646,23 +646,19 @@ int mx4_gemm(const ggemm_mx4_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s
   if (need && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
   const Way w = way_of(*p);
   if (w.tiles >= (1 << 23)) return GGEMM_ERR_INVALID;   // 512 threads each: a grid of 2^32
-  const size_t es = elem_bytes(p->dtype);
-  const bool vec = aligned(p->c, 16) && p->ldc * es % 16 == 0 && p->c_stride * es % 16 == 0;
   with_elem(p->dtype, [&](auto d) {
-    auto go = [&](auto inner, auto v) {
+    auto go = [&](auto inner) {
       constexpr int D = decltype(d)::value;
-      constexpr bool I = decltype(inner)::value, V = decltype(v)::value;
+      constexpr bool I = decltype(inner)::value;
       float* const parts = static_cast<float*>(ws);
-      if (w.tile == 256) launch_tiles<Tile256, D, I, V>(*p, w, parts, s);
-      else if (w.tile == 32) launch_tiles<Tile32, D, I, V>(*p, w, parts, s);
-      else if (w.tile == 128) launch_tiles<Tile128, D, I, V>(*p, w, parts, s);
-      else if (w.tiles < kCus && p->k >= 4096) gemm_few_kernel<D, I, V, 16><<<(unsigned)w.tiles, 1024, 0, s>>>(*p);
-      else gemm_few_kernel<D, I, V, 4><<<(unsigned)w.tiles, 256, 0, s>>>(*p);
+      if (w.tile == 256) launch_tiles<Tile256, D, I>(*p, w, parts, s);
+      else if (w.tile == 128) launch_tiles<Tile128, D, I>(*p, w, parts, s);
+      else if (w.tile == 32) launch_tiles<Tile32, D, I>(*p, w, parts, s);
+      else if (w.tiles < kCus && p->k >= 4096) gemm_few_kernel<D, I, 16><<<(unsigned)w.tiles, 1024, 0, s>>>(*p);
+      else gemm_few_kernel<D, I, 4><<<(unsigned)w.tiles, 256, 0, s>>>(*p);
     };
-    using std::true_type;
-    using std::false_type;
-    if (p->form == GGEMM_MX4_INNER) vec ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
-    else vec ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
+    if (p->form == GGEMM_MX4_INNER) go(std::true_type{});
+    else go(std::false_type{});
   });
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
 }

@@ -19,14 +19,18 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Results are stored non-temporally: they would push what is still to be read out of L2.  32768 x 4096 bf16: along
-// the rows 63 -> 49 us, down the columns 90 -> 69, back to values 117 -> 51.
-template <class V>
+// kStream: non-temporal stores, which leave what is still to be read in the caches.  32768 x 4096 bf16: along the rows 64
+// -> 51 us, down the columns 72 -> 62, both 88 -> 76, back to values 72 -> 51 (f32 138 -> 99).  Where rows end inside a
+// line the parts of a line come one by one and each has to be read first (30001 x 1000 f32, both: 28 us by way of the
+// caches, 34; 32768 x 1001 back to bf16: 15, 18), so the rows have to be whole lines of 128 bytes (codes turned through
+// LDS) or 64 (values); along the rows a wave's 256 bytes are mostly whole whatever the rows' length.
+template <bool kStream, class V>
 __device__ __forceinline__ void put(V v, void* p) {
-  __builtin_nontemporal_store(v, static_cast<V*>(p));
+  if constexpr (kStream) __builtin_nontemporal_store(v, static_cast<V*>(p));
+  else *static_cast<V*>(p) = v;
 }
 
-// Eight consecutive values: two words of four, or four words of two.
+// Eight consecutive values: two vectors of four, or one.
 template <int D>
 struct Oct {
   typename Elem<D>::T v[8];
@@ -97,14 +101,20 @@ __device__ __forceinline__ int64_t source_row(const ggemm_mx4_quant_t& q, int ro
 }
 
 // Columns 8 chunk .. of a row (zeros past its end and for a row that does not exist).
-template <int D, bool kVec>
+template <int D>
 __device__ __forceinline__ Oct<D> load_chunk(const ggemm_mx4_quant_t& q, int64_t src, int chunk) {
   using T = typename Elem<D>::T;
+  constexpr int N = 16 / (int)sizeof(T);
   const int c0 = 8 * chunk;
   const T* p = static_cast<const T*>(q.x) + src * q.ld + c0;
   Oct<D> o;
-  if (kVec && src >= 0 && c0 + 8 <= q.cols) {
-    o = *reinterpret_cast<const Oct<D>*>(__builtin_assume_aligned(p, 16));
+  if (src >= 0 && c0 + 8 <= q.cols) {
+#pragma unroll
+    for (int i = 0; i < 8; i += N) {
+      const Run<T, N> w = Run<T, N>::load(p + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) o.v[i + j] = w.x[j];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.v[i] = src >= 0 && c0 + i < q.cols ? p[i] : (T)0.0f;
@@ -124,13 +134,13 @@ template <int D>
 __device__ __forceinline__ void store_chunk(const ggemm_mx4_quant_t& q, int64_t row, int chunk, const Oct<D>& o) {
   uint32_t s;
   const uint32_t w = code_chunk<D>(o, s);
-  put(w, q.codes + row * q.ld_codes + 4 * chunk);
-  if ((chunk & 3) == 0) put((uint8_t)s, q.scales + row * q.ld_scales + (chunk >> 2));
+  put<true>(w, q.codes + row * q.ld_codes + 4 * chunk);
+  if ((chunk & 3) == 0) put<true>((uint8_t)s, q.scales + row * q.ld_scales + (chunk >> 2));
 }
 
 // Blocks along the rows.  A workgroup of 256 lanes covers cx chunks of 8 columns (cx a power of two)
 // of 256 / cx rows.
-template <int D, bool kVec>
+template <int D>
 __global__ void __launch_bounds__(kThreads) quant_rows_kernel(ggemm_mx4_quant_t q, int log_cx) {
   const int chunks = 4 * ceil_div(q.cols, 32);
   const int chunk = (blockIdx.y << log_cx) + (threadIdx.x & ((1 << log_cx) - 1));
@@ -139,11 +149,11 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(ggemm_mx4_quant_t 
   int64_t row = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx);
   for (; row + step < q.rows; row += 2 * step) {   // two rows' loads before their stores
     const int64_t s0 = source_row(q, (int)row), s1 = source_row(q, (int)(row + step));
-    const Oct<D> a = load_chunk<D, kVec>(q, s0, chunk), b = load_chunk<D, kVec>(q, s1, chunk);
+    const Oct<D> a = load_chunk<D>(q, s0, chunk), b = load_chunk<D>(q, s1, chunk);
     store_chunk<D>(q, row, chunk, a);
     store_chunk<D>(q, row + step, chunk, b);
   }
-  if (row < q.rows) store_chunk<D>(q, row, chunk, load_chunk<D, kVec>(q, source_row(q, (int)row), chunk));
+  if (row < q.rows) store_chunk<D>(q, row, chunk, load_chunk<D>(q, source_row(q, (int)row), chunk));
 }
 
 // Blocks down the columns, and along the rows too with kAlong: a workgroup takes a tile of kRows rows (a
@@ -159,7 +169,7 @@ struct Turn {
   static constexpr int kLanes = kCols / 8;   // lanes of a row
   static constexpr int kBlocks = kRows / 32, kRowBytes = kCols * (int)sizeof(typename Elem<D>::T);
 };
-template <int D, bool kVec, bool kAlong>
+template <int D, bool kAlong, bool kStream>
 __global__ void __launch_bounds__(Turn<D>::kThreads, 4) quant_turn_kernel(ggemm_mx4_quant_t q) {
   using T = typename Elem<D>::T;
   using U = Turn<D>;
@@ -183,7 +193,7 @@ __global__ void __launch_bounds__(Turn<D>::kThreads, 4) quant_turn_kernel(ggemm_
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
         const int r = i * kStep + lane_row;
-        o[i] = load_chunk<D, kVec>(q, r < rows_left ? source_row(q, (int)(r0 + r)) : -1, c0 / 8 + lane_chunk);
+        o[i] = load_chunk<D>(q, r < rows_left ? source_row(q, (int)(r0 + r)) : -1, c0 / 8 + lane_chunk);
       }
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
@@ -254,26 +264,24 @@ __global__ void __launch_bounds__(Turn<D>::kThreads, 4) quant_turn_kernel(ggemm_
     auto put_scales = [&](const uint8_t* from, uint8_t* to, int left, auto stream) {
       if (left < 4) {
         for (int i = 0; i < left; ++i) to[i] = from[i];
-      } else if (decltype(stream)::value) {
-        put(*reinterpret_cast<const uint32_t*>(from), to);
       } else {
-        *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+        put<decltype(stream)::value>(*reinterpret_cast<const uint32_t*>(from), to);
       }
     };
     const int blocks_down = ceil_div(rows_left, 32), blocks_along = ceil_div(cols_left, 32);
     for (int i = tid; i < U::kCols * B; i += U::kThreads) {
       const int c = i / B, b = i % B;
-      if (c < cols_left && b < blocks_down) put(*reinterpret_cast<const u32x4*>(place(c, b)), q.codes_t + (int64_t)(c0 + c) * q.ld_codes_t + r0 / 2 + 16 * b);
+      if (c < cols_left && b < blocks_down) put<kStream>(*reinterpret_cast<const u32x4*>(place(c, b)), q.codes_t + (int64_t)(c0 + c) * q.ld_codes_t + r0 / 2 + 16 * b);
     }
     for (int i = tid; i < U::kCols * B / 4; i += U::kThreads) {
       const int c = i / (B / 4), b = i % (B / 4) * 4;
-      if (c < cols_left) put_scales(&down_scale[c][b], q.scales_t + (int64_t)(c0 + c) * q.ld_scales_t + r0 / 32 + b, blocks_down - b, std::true_type{});
+      if (c < cols_left) put_scales(&down_scale[c][b], q.scales_t + (int64_t)(c0 + c) * q.ld_scales_t + r0 / 32 + b, blocks_down - b, std::bool_constant<kStream>{});
     }
     if constexpr (kAlong) {
       for (int i = tid; i < U::kRows * 4; i += U::kThreads) {
         const int r = i / 4, b = i % 4;
         if (r < rows_left && b < blocks_along)
-          put(*reinterpret_cast<const u32x4*>(tile + kAlongCodes + 16 * i), q.codes + (r0 + r) * q.ld_codes + c0 / 2 + 16 * b);
+          put<kStream>(*reinterpret_cast<const u32x4*>(tile + kAlongCodes + 16 * i), q.codes + (r0 + r) * q.ld_codes + c0 / 2 + 16 * b);
       }
       for (int r = tid; r < rows_left; r += U::kThreads) put_scales(along_scale[r], q.scales + (r0 + r) * q.ld_scales + c0 / 32, blocks_along, std::false_type{});
     }
@@ -321,21 +329,21 @@ __device__ __forceinline__ void load_codes(const ggemm_mx4_dequant_t& d, int64_t
   w = *reinterpret_cast<const typename Sixteen<D>::Codes*>(d.codes + row * d.ld_codes + chunk * (N / 2));
   s = d.scales[row * d.ld_scales + chunk / (32 / N)];
 }
-template <int D, bool kVec>
+template <int D, bool kStream>
 __device__ __forceinline__ void store_values(const ggemm_mx4_dequant_t& d, int64_t row, int chunk, uint32_t w, uint32_t s) {
   constexpr int N = Sixteen<D>::N;
   const Sixteen<D> o = values_of<D>(w, s);
   const int c0 = N * chunk;
   auto* p = static_cast<typename Elem<D>::T*>(d.y) + row * d.ld + c0;
-  if (kVec && c0 + N <= d.cols) {
-    put(__builtin_bit_cast(u32x4, o), p);
+  if (c0 + N <= d.cols) {
+    __builtin_bit_cast(Run<typename Elem<D>::T, N>, o).template store<kStream>(p);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (c0 + i < d.cols) p[i] = o.v[i];
   }
 }
-template <int D, bool kVec>
+template <int D, bool kStream>
 __global__ void __launch_bounds__(kThreads) dequant_kernel(ggemm_mx4_dequant_t d, int log_cx) {
   const int chunks = ceil_div(d.cols, Sixteen<D>::N);
   const int chunk = (blockIdx.y << log_cx) + (threadIdx.x & ((1 << log_cx) - 1));
@@ -347,12 +355,12 @@ __global__ void __launch_bounds__(kThreads) dequant_kernel(ggemm_mx4_dequant_t d
 #pragma unroll
     for (int i = 0; i < 4; ++i) load_codes<D>(d, row + i * step, chunk, w[i], s[i]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_values<D, kVec>(d, row + i * step, chunk, w[i], s[i]);
+    for (int i = 0; i < 4; ++i) store_values<D, kStream>(d, row + i * step, chunk, w[i], s[i]);
   }
   for (; row < d.rows; row += step) {
     uint32_t w, s;
     load_codes<D>(d, row, chunk, w, s);
-    store_values<D, kVec>(d, row, chunk, w, s);
+    store_values<D, kStream>(d, row, chunk, w, s);
   }
 }
 
@@ -393,22 +401,21 @@ int mx4_quantize(const ggemm_mx4_quant_t* q, hipStream_t s) {
   if (down && !codes_ok(q->codes_t, q->ld_codes_t, q->scales_t, q->ld_scales_t, q->rows)) return GGEMM_ERR_INVALID;
   with_elem(q->dtype, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const bool vec = aligned(q->x, 16) && q->ld * elem_bytes(D) % 16 == 0;
     if (down) {
       const int64_t tiles = (int64_t)ceil_div(q->rows, Turn<D>::kRows) * ceil_div(q->cols, Turn<D>::kCols);
       const unsigned grid = (unsigned)std::min<int64_t>(tiles, 1 << 20);
-      auto go = [&](auto v, auto a) {
-        quant_turn_kernel<D, decltype(v)::value, decltype(a)::value><<<grid, Turn<D>::kThreads, 0, s>>>(*q);
+      auto lines = [](const uint8_t* p, int64_t ld) { return aligned(p, 128) && ld % 128 == 0; };
+      const bool stream = lines(q->codes_t, q->ld_codes_t) && (!along || lines(q->codes, q->ld_codes));
+      auto go = [&](auto a, auto st) {
+        quant_turn_kernel<D, decltype(a)::value, decltype(st)::value><<<grid, Turn<D>::kThreads, 0, s>>>(*q);
       };
       using std::true_type;
       using std::false_type;
-      if (vec) along ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
-      else along ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
+      if (along) stream ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
+      else stream ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
     } else {
       const int chunks = 4 * ceil_div(q->cols, 32), l = log_lanes(chunks);
-      const dim3 grid = row_grid(q->rows, chunks, l);
-      if (vec) quant_rows_kernel<D, true><<<grid, kThreads, 0, s>>>(*q, l);
-      else quant_rows_kernel<D, false><<<grid, kThreads, 0, s>>>(*q, l);
+      quant_rows_kernel<D><<<row_grid(q->rows, chunks, l), kThreads, 0, s>>>(*q, l);
     }
   });
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
@@ -424,10 +431,8 @@ int mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t s) {
     constexpr int D = decltype(t)::value;
     const int chunks = ceil_div(d->cols, Sixteen<D>::N), l = log_lanes(chunks);
     const dim3 grid = row_grid(d->rows, chunks, l);
-    if (aligned(d->y, 16) && d->ld * elem_bytes(D) % 16 == 0)
-      dequant_kernel<D, true><<<grid, kThreads, 0, s>>>(*d, l);
-    else
-      dequant_kernel<D, false><<<grid, kThreads, 0, s>>>(*d, l);
+    if (aligned(d->y, 64) && d->ld * elem_bytes(D) % 64 == 0) dequant_kernel<D, true><<<grid, kThreads, 0, s>>>(*d, l);
+    else dequant_kernel<D, false><<<grid, kThreads, 0, s>>>(*d, l);
   });
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
 }

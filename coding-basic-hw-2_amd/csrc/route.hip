@@ -113,12 +113,12 @@ __device__ __forceinline__ uint32_t min_lanes(uint32_t x) {
   return over_lanes<L>(x, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
 
-// V values side by side, in pieces of at most 16 bytes (kVec: aligned to them).
+// A lane's V values in pieces of N side by side, at most 16 bytes.
 template <int D, int V>
 struct Piece {
   using T = typename Elem<D>::T;
   static constexpr int N = V * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : V;
-  struct alignas(N * sizeof(T)) Type { T x[N]; };
+  using Type = Run<T, N>;
   // the expert of a lane's value v, less that of its value 0; and that one
   template <int L>
   static __device__ __forceinline__ constexpr int step(int v) { return v / N * L * N + v % N; }
@@ -132,7 +132,6 @@ struct Logits {
   using P = Piece<D, V>;
   typename P::Type w[V / P::N];
   unsigned char mask;
-  template <bool kVec>
   __device__ __forceinline__ void load(const ggemm_router_t& r, int t, int t1, int e0) {
     using T = typename P::T;
     if (t >= t1) return;
@@ -142,8 +141,8 @@ struct Logits {
     for (int i = 0; i < V / P::N; ++i) {
       constexpr int N = P::N;
       const int at = i * L * N;
-      if (kVec && e0 + at + N <= r.experts) {
-        w[i] = *reinterpret_cast<const typename P::Type*>(p + at);
+      if (e0 + at + N <= r.experts) {
+        w[i] = P::Type::load(p + at);
       } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) w[i].x[j] = e0 + at + j < r.experts ? p[at + j] : (T)-__builtin_inff();
@@ -153,12 +152,7 @@ struct Logits {
   __device__ __forceinline__ bool on(int t, int t1) const { return t < t1 && mask; }   // the token takes part
   __device__ __forceinline__ typename P::T at(int v) const { return w[v / P::N].x[v % P::N]; }
 };
-template <class P>
-__device__ __forceinline__ void store_streaming(const P& w, void* p) {
-  typedef unsigned short half_words __attribute__((ext_vector_type(sizeof(P) / 2)));
-  __builtin_nontemporal_store(__builtin_bit_cast(half_words, w), static_cast<half_words*>(p));
-}
-template <int D, int L, int V, bool kVec>
+template <int D, int L, int V>
 __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, int experts, const float (&g)[V]) {
   using P = Piece<D, V>;
   constexpr int N = P::N;
@@ -168,8 +162,8 @@ __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, i
     typename P::Type w;
 #pragma unroll
     for (int j = 0; j < N; ++j) w.x[j] = (typename P::T)g[i * N + j];
-    if (kVec && at + N <= experts) {
-      store_streaming(w, p + at);
+    if (at + N <= experts) {
+      w.template store<true>(p + at);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
@@ -250,7 +244,7 @@ __device__ __forceinline__ void scan_offsets(const int* counts, int experts, int
 // per workgroup.  kOne: the only workgroup, which finishes the call.
 // (kOne: 16 waves, as long as their sums fit, for the latency of one call)
 __host__ __device__ constexpr int first_threads(int experts, bool one) { return one && experts <= 256 ? 1024 : kThreads; }
-template <int D, int L, int V, bool kOne, bool kVec>
+template <int D, int L, int V, bool kOne>
 __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm_router_t r, RouteWs ws, int span) {
   using P = Piece<D, V>;
   constexpr int NT = first_threads(L * V, kOne), NW = NT / 64;
@@ -270,7 +264,7 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
   int used = 0;
   Logits<D, L, V> ahead;
-  ahead.template load<kVec>(r, t0 + slot, t1, e0);
+  ahead.load(r, t0 + slot, t1, e0);
   for (int tb = t0; tb < t1; tb += kPar) {
     const int t = tb + slot;
     const bool in = t < t1;
@@ -302,7 +296,7 @@ __global__ void __launch_bounds__(first_threads(L * V, kOne)) route_kernel(ggemm
         for (int v = 0; v < V; ++v) key[v] = x[v] != x[v] ? key[v] | 0xffff0000u : key[v];
       }
     }
-    ahead.template load<kVec>(r, t + kPar, t1, e0);
+    ahead.load(r, t + kPar, t1, e0);
     // the largest key of the token below the last one taken (32-bit: of those not struck out), and its expert
     uint32_t best = 0;
     int expert = 0;
@@ -559,7 +553,7 @@ __global__ void __launch_bounds__(kThreads) route_place_kernel(ggemm_router_t r,
 // Gradient: dx = p (s - <p, s>) + c, with s_e = d_loss coef E counts_e / (topk used^2) and, for the chosen
 // places, c_j = g_j (dg_j - <g, dg>) when the gates are renormalised; else s_e takes dg_j too and c = 0.
 // The token's dg (or c) by expert goes through a row of LDS that is zero outside the chosen places.
-template <int D, int L, int V, bool kVec>
+template <int D, int L, int V>
 __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t r, const float* __restrict__ d_gates,
                                                                   const float* __restrict__ d_loss, void* d_logits,
                                                                   int64_t ld_d, int per) {
@@ -599,7 +593,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
     return c;
   };
   Logits<D, L, V> ahead;
-  ahead.template load<kVec>(r, t0 + slot, t1, e0);
+  ahead.load(r, t0 + slot, t1, e0);
   Choice next = choice(t0 + slot, sub);
   for (int tb = t0; tb < t1; tb += kPar) {
     const int t = tb + slot;
@@ -609,7 +603,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
 #pragma unroll
     for (int v = 0; v < V; ++v) x[v] = (float)ahead.at(v);
     const Choice mine = next;
-    ahead.template load<kVec>(r, t + kPar, t1, e0);
+    ahead.load(r, t + kPar, t1, e0);
     next = choice(t + kPar, sub);
     float m = x[0];
 #pragma unroll
@@ -668,7 +662,7 @@ __global__ void __launch_bounds__(kThreads) route_backward_kernel(ggemm_router_t
 #pragma unroll
       for (int v = 0; v < V; ++v) c[v] = live && x[v] != -__builtin_inff() ? c[v] : 0.0f;
     }
-    if (in) store_gradient<D, L, V, kVec>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, c);
+    if (in) store_gradient<D, L, V>(static_cast<T*>(d_logits) + (int64_t)t * ld_d, e0, E, c);
   }
 }
 
@@ -720,17 +714,13 @@ int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
   with_elem(r->dtype, [&](auto d) {
     with_lanes(r->experts, [&](auto l, auto v) {
       constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
-      constexpr int A = sizeof(typename Piece<D, V>::Type);
-      auto go = [&](auto one, auto vec) {
+      auto go = [&](auto one) {
         constexpr int NT = first_threads(L * V, decltype(one)::value);
         const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + NT / 64 * L * V * 4;
-        route_kernel<D, L, V, decltype(one)::value, decltype(vec)::value><<<sh.groups, NT, lds, s>>>(*r, w, sh.span);
+        route_kernel<D, L, V, decltype(one)::value><<<sh.groups, NT, lds, s>>>(*r, w, sh.span);
       };
-      using std::true_type;
-      using std::false_type;
-      const bool vec = aligned(r->logits, A) && r->ld * elem_bytes(D) % A == 0;
-      if (sh.groups == 1) vec ? go(true_type{}, true_type{}) : go(true_type{}, false_type{});
-      else vec ? go(false_type{}, true_type{}) : go(false_type{}, false_type{});
+      if (sh.groups == 1) go(std::true_type{});
+      else go(std::false_type{});
     });
   });
   if (sh.groups > 1) {
@@ -754,15 +744,7 @@ int route_backward(const ggemm_router_t* r, const float* d_gates, const float* d
       constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
       constexpr int kPar = 256 / L;
       const int per = std::max(kPar, (int)align_up((size_t)ceil_div(r->tokens, 2048), kPar));
-      constexpr int A = sizeof(typename Piece<D, V>::Type);
-      auto go = [&](auto vec) {
-        route_backward_kernel<D, L, V, decltype(vec)::value>
-            <<<ceil_div(r->tokens, per), kThreads, 0, s>>>(*r, d_gates, d_loss, d_logits, ld_d, per);
-      };
-      if (aligned(r->logits, A) && aligned(d_logits, A) && r->ld * elem_bytes(D) % A == 0 && ld_d * elem_bytes(D) % A == 0)
-        go(std::true_type{});
-      else
-        go(std::false_type{});
+      route_backward_kernel<D, L, V><<<ceil_div(r->tokens, per), kThreads, 0, s>>>(*r, d_gates, d_loss, d_logits, ld_d, per);
     });
   });
   return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;

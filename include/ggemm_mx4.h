@@ -73,7 +73,7 @@ int ggemm_mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t stream);
  * results but no access out of bounds.  alpha == 0 still multiplies; with beta == 0 C is not read.  k = 0 (or
  * an empty K_g) gives beta C.  C must not overlap the inputs.
  * Alignment: a, b and their ld and stride multiples of 16 bytes; scales, their ld and stride of 4 bytes.  C needs
- * its type's alignment only (16 bytes, with ldc and c_stride, is faster).  Results are the same bits every time.
+ * its type's alignment only.  Results are the same bits every time.
  * Products of 2^23 or more tiles (16 x 32 to 256 x 256 of C) are refused. */
 #define GGEMM_MX4_ROWS  0
 #define GGEMM_MX4_INNER 1

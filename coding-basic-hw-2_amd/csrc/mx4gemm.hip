@@ -8,7 +8,7 @@
 // card lowers its clock under the products' power), so the tiles use the former.
 // Bound: 256 x 256 tiles over a long inner dimension, that power (8192 x 8192 x 16384: 499 us, 4.4 PFLOP/s, at 1.85
 // GHz with the matrix cores busy 53 % of the cycles; all zeros 403 us at 2.46 GHz); over a short one, also the
-// stores of C (8192 x 8192 x 1024: 59 us); few rows, the bytes of B.
+// stores of C (8192 x 8192 x 1024: 56 us); few rows, the bytes of B.
 #include <algorithm>
 #include <type_traits>
 

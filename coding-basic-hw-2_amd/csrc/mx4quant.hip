@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(ggemm_mx4_quant_t 
 // memory line of codes of every column; half of one for 32-bit values) and 128 columns through 64 KB of LDS.
 // Codes and scales of both kinds go back through LDS and leave as 16 and 4 bytes a lane, runs of 128 (64)
 // bytes.  A tile has 4 scale bytes of a row; runs of tiles side by side go to one XCD and these bytes are stored
-// the ordinary way, so that its L2 makes lines of them (32768 x 4096 bf16, both kinds: 127 us as they come, 104;
-// the two kinds one after the other 118).  Half the tile and twice the workgroups per compute unit is slower
+// the ordinary way, so that its L2 makes lines of them (32768 x 4096 bf16, both kinds: 127 us as they come, 104
+// this way; 76 with the present loads, the two kinds one after the other 114).  Half the tile and twice the workgroups per compute unit is slower
 // by 5 to 20 %.
 template <int D>
 struct Turn {

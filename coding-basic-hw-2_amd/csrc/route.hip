@@ -8,13 +8,12 @@
 // half, so that a key is unique and tells the expert to all lanes, and the next place is the largest of
 // key - best mod 2^32 (a key below `best` differs by 2^32 - best or more, one above by less): nothing is struck
 // out.  32-bit logits take a second reduction, the least expert that holds the maximum, which is struck out.
-// Softmax is the usual exp2((x - max)
-// log2 e) over its sum, the maximum being the first choice; its sums are 32-bit.
+// Softmax is the usual exp2((x - max) log2 e) over its sum, the maximum being the first choice; its sums are 32-bit.
 // Counting: a workgroup takes `span` consecutive tokens.  One bit per (expert, token) in LDS gives each pair
 // its rank among the workgroup's tokens by counting bits (no atomic whose order matters), and the
 // expert's count.  A second launch turns the workgroups' counts into starting ranks and sums their partial
-// softmax sums in a fixed order; a third one writes rows, order and loss.  A call of one workgroup does
-// all of it in the first launch.
+// softmax sums in a fixed order; a third one writes rows, order and loss, and does the second one's work too
+// while the tables are small.  A call of one workgroup does all of it in the first launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,14 +34,15 @@ struct RouteWs {
   int* used;     // groups
 };
 
-constexpr int kFewGroups = 128;   // workgroups of the first launch up to which there is no second one
+constexpr int kFewCounts = 8192;   // entries of the count table up to which there is no second launch
 struct Shape {
   int span, groups;
 };
 // Tokens a workgroup takes (a multiple of 32: whole words of the bit table).  Few tokens are spread over
-// the compute units, many take longer spans, which makes the tables of the second launch shorter.
+// the compute units, many take longer spans, which makes the tables of the second launch shorter (16384 x 128:
+// 16.5 us with 32, 18 with 64; 32768 x 64: 20.4 and 19.4; 131072 x 256: 78, 68, and 63 with 128).
 Shape shape_of(int tokens) {
-  const int span = tokens <= 64 ? 64 : tokens <= 4096 ? 32 : tokens <= 65536 ? 64 : 128;
+  const int span = tokens <= 64 ? 64 : tokens <= 16384 ? 32 : tokens <= 65536 ? 64 : 128;
   return Shape{span, tokens > 0 ? ceil_div(tokens, span) : 1};
 }
 
@@ -125,7 +125,7 @@ struct Piece {
   static __device__ __forceinline__ int first(int lane) { return lane * N; }
 };
 // The lane's V logits of token t (from expert e0 on; -inf past the last expert), as they lie in memory: a wave has the
-// next tokens' on the way while it works on these (131072 x 256 bf16, forward %%F%%, backward %%B%% us).  Those of a token
+// next tokens' on the way while it works on these (131072 x 256 bf16: gradient 48 -> 44 us).  Those of a token
 // that is left out are read and not used.
 template <int D, int L, int V>
 struct Logits {
@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(16 * kRuns) route_scan_kernel(ggemm_router_t r
 
 // Third launch: rows of the pairs, order, padding, loss.  Workgroup b takes the pairs of workgroup b of
 // the first launch.  kScan: there was no second launch; every workgroup sums the tables for itself (experts <=
-// kThreads), which few workgroups do faster than a launch of its own takes (4096 tokens, 16 experts: 2 us).
+// kThreads), which is faster than a launch while the tables are small (4096 x 16: 9.4 us for the call and 11;
+// 4096 x 256: 24 and 17.5).
 template <bool kScan>
 __global__ void __launch_bounds__(kThreads) route_place_kernel(ggemm_router_t r, RouteWs ws, int span) {
   __shared__ int s_off[GGEMM_ROUTE_MAX_EXPERTS + 1], s_tmp[4];
@@ -724,7 +725,7 @@ int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
     });
   });
   if (sh.groups > 1) {
-    if (r->experts <= kThreads && sh.groups <= kFewGroups) {
+    if (r->experts <= kThreads && (int64_t)sh.groups * r->experts <= kFewCounts) {
       route_place_kernel<true><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
     } else {
       route_scan_kernel<<<ceil_div(r->experts, 16), 16 * kRuns, 0, s>>>(*r, w, sh.groups);

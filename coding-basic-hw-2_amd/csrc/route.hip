@@ -172,22 +172,16 @@ __device__ __forceinline__ void store_gradient(typename Elem<D>::T* p, int e0, i
   }
 }
 
-// exp(x - m).  The difference first: m log2 e alone overflows for logits of the type's lowest value.
+// exp(x - m).  The difference first: it is exact for logits near the maximum, however large they are.
 __device__ __forceinline__ float exp_below(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kLog2e); }
-// p[v] = exp(x[v] - max) for a token's lanes, and the reciprocal of the sum.  m: the largest logit; -inf gives 0.
-// Where no token of the wave has so large a maximum, one fma: the rounding of m log2 e is the same for all of a
-// token's values and leaves with the sum.
+// p[v] = exp(x[v] - max) for a token's lanes, and the reciprocal of the sum.  m: the largest logit;
+// a logit of -inf gives 0 unless m is -inf too, where nothing uses p.
+// (One fma of x log2 e and -m log2 e was no faster, and its error grows with m.)
 template <int L, int V>
 __device__ __forceinline__ float exps(const float (&x)[V], float m, float (&p)[V]) {
   float sum = 0.0f;
-  if (__ballot(fabsf(m) > 1e30f) == 0) {
-    const float c = m * kLog2e;
 #pragma unroll
-    for (int v = 0; v < V; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v], kLog2e, -c));
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) p[v] = exp_below(x[v], m);
-  }
+  for (int v = 0; v < V; ++v) p[v] = exp_below(x[v], m);
 #pragma unroll
   for (int v = 0; v < V; ++v) sum += p[v];
   return 1.0f / sum_lanes<L>(sum);

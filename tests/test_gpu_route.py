@@ -211,3 +211,31 @@ def test_graph_replay():
         _compare(o, w, ("replay", i))
         grad, mag = R.route_gradient(w, k, True, 0.1, dg.double().cpu().numpy(), 1.0)
         assert (np.abs(out.double().cpu().numpy() - grad) <= 3 * REL * mag + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_logits_far_from_zero(dtype):
+    """Softmax depends on differences only: rows of large logits that differ by a few units or of the type's spacings, alone
+    and beside ordinary rows; gates as they are, sums and gradients.  Differences stay exact in 32 bits."""
+    say(f"route far from zero {dtype}")
+    rng = np.random.default_rng(8)
+    E, k = 40, 4
+    centres = [20.0, -40.0, 90.0, 1e3, -1e3, 3e4] + ([] if dtype == "f16" else [1e6, 1e10, -1e10, 1e25, -3e29, 2e30])
+    x = rng.standard_normal((40 * len(centres), E)) * 2
+    for i, c in enumerate(centres):
+        spacing = 2.0 ** np.floor(np.log2(abs(c))) * 2 * R.UNIT[dtype]
+        rows = x[40 * i:40 * i + 30]
+        rows[:] = c + (np.round(rows / spacing) if spacing < 0.5 else np.round(rows)) * spacing
+    x = torch.from_numpy(x).to(R.TORCH[dtype])
+    T = x.shape[0]
+    dg, dl = rng.standard_normal((T, k)).astype(np.float32), np.float32(0.6)
+    xd, dgd, dld = x.cuda(), R.dev(dg), torch.full((1,), float(dl), device="cuda")
+    for renorm in (False, True):
+        w = R.route(x.double().numpy(), None, k, 1, renorm, 0.3)
+        r, o, _ = R.gpu_route(xd, None, k, 1, renorm, 0.3)
+        _compare(o, w, (dtype, renorm))
+        grad, mag = R.route_gradient(w, k, renorm, 0.3, dg.astype(np.float64), float(dl))
+        out = torch.full((T, E), 9.0, dtype=R.TORCH[dtype], device="cuda")
+        assert G.lib().ggemm_route_backward(C.byref(r), dgd.data_ptr(), dld.data_ptr(), out.data_ptr(), E, R.stream()) == 0
+        tol = 3 * REL * mag + R.UNIT[dtype] * np.abs(grad) + R.TINY[dtype]
+        assert (np.abs(out.double().cpu().numpy() - grad) <= tol).all(), (dtype, renorm)

@@ -127,3 +127,9 @@ def test_long_rows():
     R.gemm(G.MX4_ROWS, (wide, a[1]), b, m, n, k, out)
     w = bv.t().contiguous()
     _check(out, av @ w, av.abs() @ w.abs(), k, "f32", "long rows")
+
+
+def test_inner_order_of_groups():
+    """More than two runs of 64 groups of different lengths, empty ones among them."""
+    test_inner(130, 200, 6400, 150)
+    test_inner(300, 260, 3200, 64)

@@ -1,3 +1,4 @@
+import os
 import sys
 from pathlib import Path
 
@@ -7,9 +8,24 @@ HERE = Path(__file__).resolve().parent
 sys.path.insert(0, str(HERE))
 sys.path.insert(0, str(HERE.parent / "coding-basic-hw-2_amd"))
 
+# Tests of what the host refuses: their pointers are addresses of nothing, which a card would follow if a call were
+# accepted (two calls of test_gemm_workspace_and_empty are).
+HOST_ONLY = ("test_mx4_args.py", "test_mx4_limits.py")
+
+
+def card_present():
+    return os.path.exists("/dev/kfd")
+
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (gfx950) GPU and the built HIP library")
+
+
+def pytest_collection_modifyitems(config, items):
+    if card_present():
+        for item in items:
+            if Path(str(item.fspath)).name in HOST_ONLY:
+                item.add_marker(pytest.mark.skip(reason="made-up addresses: run where no card can follow them"))
 
 
 @pytest.fixture(scope="session", autouse=True)

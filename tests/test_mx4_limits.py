@@ -1,0 +1,27 @@
+"""Workspaces and limits of the 4-bit operators and the router, as the host decides them.  Every call here is refused:
+the pointers are addresses of nothing."""
+import ctypes as C
+
+import pytest
+
+import ggemm as G
+
+P = 0x7f0000000000
+
+
+def product(**kw):
+    """A product whose inner dimension is computed in parts: it needs a workspace."""
+    f = dict(form=G.MX4_ROWS, groups=1, m=64, n=1024, k=16384, dtype=G.F32, alpha=1.0, beta=0.0, a=P, lda=8192, a_scales=P,
+             lda_scales=512, b=P, ldb=8192, b_stride=0, b_scales=P, ldb_scales=512, b_scales_stride=0, offsets=None, c=P,
+             ldc=1024, c_stride=0)
+    f.update(kw)
+    return G.Mx4Gemm(**f)
+
+
+def test_product_workspace_refusals():
+    p = product()
+    size = G.lib().ggemm_mx4_gemm_workspace(C.byref(p))
+    assert size > 0 and size % 16 == 0
+    for ws, n, rc in ((P, size - 1, G.GGEMM_ERR_WORKSPACE), (P, 0, G.GGEMM_ERR_WORKSPACE), (None, 0, G.GGEMM_ERR_WORKSPACE),
+                      (None, size, G.GGEMM_ERR_INVALID), (P + 4, size, G.GGEMM_ERR_INVALID)):
+        assert G.lib().ggemm_mx4_gemm(C.byref(p), ws, n, None) == rc, (ws, n)

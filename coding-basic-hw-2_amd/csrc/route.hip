@@ -38,6 +38,8 @@ constexpr int kFewCounts = 8192;   // entries of the count table up to which the
 struct Shape {
   int span, groups;
 };
+// GGEMM_ROUTE_MAX_TOKENS keeps a token's number plus a workgroup's tokens within 31 bits, and the grids (two threads
+// a token at most, where there are many) within 2^32.
 // Tokens a workgroup takes (a multiple of 32: whole words of the bit table).  Few tokens are spread over
 // the compute units, many take longer spans, which makes the tables of the second launch shorter (16384 x 128:
 // 16.5 us with 32, 18 with 64; 32768 x 64: 20.4 and 19.4; 131072 x 256: 78, 68, and 63 with 128).
@@ -187,9 +189,10 @@ __device__ __forceinline__ float exps(const float (&x)[V], float m, float (&p)[V
   return 1.0f / sum_lanes<L>(sum);
 }
 
-// Rows of order that belong to no pair: expert e's padding, and what follows the last expert.
-__device__ __forceinline__ void pad_order(const ggemm_router_t& r, int from, int to, int lane, int lanes) {
-  for (int i = from + lane; i < to; i += lanes) r.order[i] = -1;
+// Rows of order that belong to no pair: expert e's padding, and what follows the last expert.  64-bit: the rows and the
+// lanes of a large grid (twice the tokens) together pass 2^31.
+__device__ __forceinline__ void pad_order(const ggemm_router_t& r, int from, int to, int64_t lane, int64_t lanes) {
+  for (int64_t i = from + lane; i < to; i += lanes) r.order[i] = -1;
 }
 
 // The balance loss from counts, probs and the tokens used: one wave, fixed order.
@@ -528,9 +531,9 @@ __global__ void __launch_bounds__(kThreads) route_place_kernel(ggemm_router_t r,
       if (row < r.max_rows) r.order[row] = t0 + i / K;
     }
   }
-  const int all = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
+  const int64_t all = (int64_t)gridDim.x * kThreads, me = (int64_t)blockIdx.x * kThreads + tid;
   if (r.row_align > 1)
-    for (int e = me; e < E; e += all) pad_order(r, s_off[e] + counts[e], s_off[e + 1], 0, 1);
+    for (int64_t e = me; e < E; e += all) pad_order(r, s_off[e] + counts[e], s_off[e + 1], 0, 1);
   pad_order(r, s_off[E], r.max_rows, me, all);
   if (blockIdx.x == 0) {
     for (int e = tid; e <= E; e += kThreads) r.offsets[e] = s_off[e];
@@ -677,7 +680,7 @@ void with_lanes(int experts, F&& f) {
 }
 
 bool sizes_ok(int tokens, int experts, int topk) {
-  return tokens >= 0 && experts >= 1 && experts <= GGEMM_ROUTE_MAX_EXPERTS && topk >= 1 &&
+  return tokens >= 0 && tokens <= GGEMM_ROUTE_MAX_TOKENS && experts >= 1 && experts <= GGEMM_ROUTE_MAX_EXPERTS && topk >= 1 &&
          topk <= GGEMM_ROUTE_MAX_TOPK && topk <= experts && (int64_t)tokens * topk <= 0x7fffffff;
 }
 

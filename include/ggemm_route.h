@@ -34,6 +34,7 @@
 extern "C" {
 #endif
 
+#define GGEMM_ROUTE_MAX_TOKENS (1 << 30)   /* and tokens topk + experts (row_align - 1) < 2^31 */
 #define GGEMM_ROUTE_MAX_EXPERTS 1024
 #define GGEMM_ROUTE_MAX_TOPK 64
 #define GGEMM_ROUTE_MAX_ALIGN 1024

@@ -25,3 +25,11 @@ def test_product_workspace_refusals():
     for ws, n, rc in ((P, size - 1, G.GGEMM_ERR_WORKSPACE), (P, 0, G.GGEMM_ERR_WORKSPACE), (None, 0, G.GGEMM_ERR_WORKSPACE),
                       (None, size, G.GGEMM_ERR_INVALID), (P + 4, size, G.GGEMM_ERR_INVALID)):
         assert G.lib().ggemm_mx4_gemm(C.byref(p), ws, n, None) == rc, (ws, n)
+
+
+def test_router_token_limit():
+    T = G.ROUTE_MAX_TOKENS
+    assert T == 2 ** 30 and G.lib().ggemm_route_workspace(T, 1, 1) > 0 and G.lib().ggemm_route_workspace(T + 1, 1, 1) == 0
+    r = G.Router(T + 1, 2, 1, 1, G.BF16, 0, 0.0, T + 1, P, 2, None, P, P, P, P, P, P, P, P, P)
+    assert G.lib().ggemm_route(C.byref(r), P, 1 << 40, None) == G.GGEMM_ERR_INVALID
+    assert G.lib().ggemm_route_backward(C.byref(r), P, P, P, 2, None) == G.GGEMM_ERR_INVALID

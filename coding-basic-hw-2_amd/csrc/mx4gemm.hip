@@ -571,27 +571,34 @@ __global__ void __launch_bounds__(64 * NW, 4) gemm_few_kernel(ggemm_mx4_gemm_t p
   }
 }
 
-bool gemm_ok(const ggemm_mx4_gemm_t* p) {
+// Sizes, leading dimensions and strides.
+bool shape_ok(const ggemm_mx4_gemm_t* p) {
   if (!p || (p->form != GGEMM_MX4_ROWS && p->form != GGEMM_MX4_INNER) || p->groups < 1 ||
-      p->groups > GGEMM_MX4_MAX_GROUPS || p->m < 0 || p->n < 0 || p->k < 0 || !elem_known(p->dtype) ||
-      (!p->offsets && p->groups != 1))
+      p->groups > GGEMM_MX4_MAX_GROUPS || p->m < 0 || p->n < 0 || p->k < 0 || !elem_known(p->dtype))
     return false;
   if (p->m == 0 || p->n == 0) return true;
   const bool inner = p->form == GGEMM_MX4_INNER;
-  if (!p->c || !aligned(p->c, elem_bytes(p->dtype)) || p->ldc < p->n || !aligned(p->offsets, 4)) return false;
+  if (p->ldc < p->n) return false;
   if (inner && p->groups > 1 && (p->c_stride < 0 || p->c_stride < (int64_t)(p->m - 1) * p->ldc + p->n)) return false;
   if (p->k == 0) return true;
   const int64_t nb = ceil_div(p->k, 32);
-  auto operand = [&](const uint8_t* x, int64_t ld, const uint8_t* s, int64_t lds) {
-    return x && s && aligned(x, 16) && aligned(s, 4) && ld % 16 == 0 && ld >= 16 * nb && lds % 4 == 0 && lds >= nb;
-  };
-  return operand(p->a, p->lda, p->a_scales, p->lda_scales) && operand(p->b, p->ldb, p->b_scales, p->ldb_scales) &&
+  auto operand = [&](int64_t ld, int64_t lds) { return ld % 16 == 0 && ld >= 16 * nb && lds % 4 == 0 && lds >= nb; };
+  return operand(p->lda, p->lda_scales) && operand(p->ldb, p->ldb_scales) &&
          (inner || p->groups == 1 || (p->b_stride % 16 == 0 && p->b_scales_stride % 4 == 0));
 }
 
-// Row tiles of TM rows that the groups can have at most: sum ceil(m_g / TM) <= m / TM + groups with rows.
+bool gemm_ok(const ggemm_mx4_gemm_t* p) {
+  if (!shape_ok(p) || (!p->offsets && p->groups != 1)) return false;
+  if (p->m == 0 || p->n == 0) return true;
+  if (!p->c || !aligned(p->c, elem_bytes(p->dtype)) || !aligned(p->offsets, 4)) return false;
+  auto operand = [](const uint8_t* x, const uint8_t* s) { return x && s && aligned(x, 16) && aligned(s, 4); };
+  return p->k == 0 || (operand(p->a, p->a_scales) && operand(p->b, p->b_scales));
+}
+
+// Row tiles of TM rows that the groups can have at most: sum ceil(m_g / TM) <= m / TM + groups with rows.  (Not by
+// whether there are offsets: a workspace may be asked for before they exist.)
 int64_t row_tiles(const ggemm_mx4_gemm_t& p, int tm) {
-  return p.offsets ? (int64_t)p.m / tm + std::min(p.groups, p.m) : ceil_div(p.m, tm);
+  return p.groups > 1 ? (int64_t)p.m / tm + std::min(p.groups, p.m) : ceil_div(p.m, tm);
 }
 
 using Tile256 = Tile<256, 256, 2, 4>;
@@ -628,7 +635,7 @@ Way way_of(const ggemm_mx4_gemm_t& p) {
   Way w{32, 1, thin};
   if (p.m > 64 * groups) {
     const int64_t big = tiles_of(p, 256, 256), nt = ceil_div(p.n, 256);
-    const int64_t likely = inner || !p.offsets ? big : (2 * (int64_t)p.m / 256 + p.groups) * nt / 2;
+    const int64_t likely = inner || p.groups == 1 ? big : (2 * (int64_t)p.m / 256 + p.groups) * nt / 2;
     w = likely >= 2 * kCus ? Way{256, 1, big} : Way{128, 1, tiles_of(p, 128, 128)};
   }
   const int64_t runs = ceil_div(p.k, 256) / (inner ? p.groups : 1);
@@ -661,7 +668,7 @@ void launch_tiles(const ggemm_mx4_gemm_t& p, const Way& w, float* parts, hipStre
 }  // namespace
 
 size_t mx4_gemm_workspace(const ggemm_mx4_gemm_t* p) {
-  if (!gemm_ok(p) || p->m == 0 || p->n == 0) return 0;
+  if (!shape_ok(p) || p->m == 0 || p->n == 0) return 0;
   const Way w = way_of(*p);
   return w.splits > 1 ? (size_t)w.tiles * w.splits * w.tile * 128 * sizeof(float) : 0;
 }

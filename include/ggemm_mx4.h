@@ -89,7 +89,8 @@ typedef struct {
   const int32_t* offsets;
   void* c; int64_t ldc; int64_t c_stride;
 } ggemm_mx4_gemm_t;
-/* Bytes of workspace (16-byte aligned) that a call with these sizes needs; 0 for invalid ones. */
+/* Bytes of workspace (16-byte aligned) that a call with these sizes, leading dimensions and strides needs: often 0, and
+ * 0 for invalid ones.  Pointers are not looked at: they may still be NULL. */
 size_t ggemm_mx4_gemm_workspace(const ggemm_mx4_gemm_t* p);
 /* Too small a workspace: GGEMM_ERR_WORKSPACE.  Its contents need not be kept or cleared between calls;
  * calls that may overlap need one each. */

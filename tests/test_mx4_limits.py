@@ -33,3 +33,20 @@ def test_router_token_limit():
     r = G.Router(T + 1, 2, 1, 1, G.BF16, 0, 0.0, T + 1, P, 2, None, P, P, P, P, P, P, P, P, P)
     assert G.lib().ggemm_route(C.byref(r), P, 1 << 40, None) == G.GGEMM_ERR_INVALID
     assert G.lib().ggemm_route_backward(C.byref(r), P, P, P, 2, None) == G.GGEMM_ERR_INVALID
+
+
+@pytest.mark.parametrize("form", [G.MX4_ROWS, G.MX4_INNER])
+@pytest.mark.parametrize("groups,m", [(1, 64), (1, 256), (2, 100)])
+def test_product_workspace_by_sizes(form, groups, m):
+    """The same before the operands and the offsets exist as with them."""
+    kw = dict(form=form, groups=groups, m=m, b_stride=8192 * 1024, b_scales_stride=512 * 1024, c_stride=m * 1024)
+    full = product(offsets=P, **kw)
+    none = product(a=None, a_scales=None, b=None, b_scales=None, c=None, offsets=None, **kw)
+    size = G.lib().ggemm_mx4_gemm_workspace(C.byref(full))
+    assert size > 0 and G.lib().ggemm_mx4_gemm_workspace(C.byref(none)) == size
+    if groups == 1:
+        assert G.lib().ggemm_mx4_gemm_workspace(C.byref(product(**kw))) == size      # one group without offsets
+    assert G.lib().ggemm_mx4_gemm(C.byref(none), P, size, None) == G.GGEMM_ERR_INVALID
+    assert G.lib().ggemm_mx4_gemm(C.byref(full), P, size - 1, None) == G.GGEMM_ERR_WORKSPACE
+    for bad in (dict(lda=16), dict(ldb=8184), dict(lda_scales=511), dict(ldc=1023), dict(dtype=9), dict(k=-1), dict(form=2)):
+        assert G.lib().ggemm_mx4_gemm_workspace(C.byref(product(**{**kw, **bad}))) == 0, bad

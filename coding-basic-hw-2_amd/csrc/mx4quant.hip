@@ -395,7 +395,8 @@ int mx4_quantize(const ggemm_mx4_quant_t* q, hipStream_t s) {
   if (!along && !down) return GGEMM_ERR_INVALID;
   if (q->cols > kMaxCols || (down && q->rows > kMaxCols)) return GGEMM_ERR_INVALID;
   if (q->rows == 0 || q->cols == 0) return GGEMM_OK;
-  if (!q->x || q->ld < q->cols || !aligned(q->x, elem_bytes(q->dtype)) || (q->index && (q->x_rows < 0 || !aligned(q->index, 4))))
+  const bool no_rows = q->index && q->x_rows == 0;   // an index that picks from nothing: x is not read
+  if ((!q->x && !no_rows) || q->ld < q->cols || !aligned(q->x, elem_bytes(q->dtype)) || (q->index && (q->x_rows < 0 || !aligned(q->index, 4))))
     return GGEMM_ERR_INVALID;
   if (along && !codes_ok(q->codes, q->ld_codes, q->scales, q->ld_scales, q->cols)) return GGEMM_ERR_INVALID;
   if (down && !codes_ok(q->codes_t, q->ld_codes_t, q->scales_t, q->ld_scales_t, q->rows)) return GGEMM_ERR_INVALID;

@@ -30,7 +30,7 @@ extern "C" {
 #define GGEMM_MX4_MAX_GROUPS 4096
 
 /* Quantisation of a rows x cols matrix: row i is x[i], or with an index x[index[i]], and zeros where
- * index[i] lies outside [0, x_rows) (rows that pad a group).  Per block of 32 values v, with
+ * index[i] lies outside [0, x_rows) (rows that pad a group; x may be NULL if x_rows is 0).  Per block of 32 values v, with
  * a = max |v|: s = clamp(floor(log2 a) - 2, -127, 127) + 127 (all zeros: 0), codes = v / 2^(s - 127)
  * rounded to the nearest magnitude, ties to the even code, beyond 6 to 6.  A block that holds a NaN
  * or an Inf gets s = 255 and zero codes: every value of it is NaN.

@@ -50,3 +50,15 @@ def test_product_workspace_by_sizes(form, groups, m):
     assert G.lib().ggemm_mx4_gemm(C.byref(full), P, size - 1, None) == G.GGEMM_ERR_WORKSPACE
     for bad in (dict(lda=16), dict(ldb=8184), dict(lda_scales=511), dict(ldc=1023), dict(dtype=9), dict(k=-1), dict(form=2)):
         assert G.lib().ggemm_mx4_gemm_workspace(C.byref(product(**{**kw, **bad}))) == 0, bad
+
+
+def quant(**kw):
+    f = dict(rows=4, cols=64, dtype=G.BF16, x_rows=4, x=P, ld=64, index=P, codes=P, ld_codes=32, scales=P, ld_scales=4)
+    f.update(kw)
+    return G.lib().ggemm_mx4_quantize(C.byref(G.Mx4Quant(**f)), None)
+
+
+def test_quantise_without_a_matrix():
+    """x may be NULL only where an index picks from no rows."""
+    assert quant(x=None) == quant(x=None, index=None, x_rows=0) == quant(x=None, x_rows=1) == G.GGEMM_ERR_INVALID
+    assert quant(x=None, x_rows=0, ld=63) == quant(x=None, x_rows=0, codes=None) == G.GGEMM_ERR_INVALID

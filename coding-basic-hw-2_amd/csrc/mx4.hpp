@@ -35,6 +35,14 @@ inline void with_elem(int dtype, F&& f) {
   else f(std::integral_constant<int, GGEMM_F16>{});
 }
 
+// The status of the launches that f makes.  An error that an earlier call of the program left behind is not theirs.
+template <class F>
+inline int launch(F&& f) {
+  (void)hipGetLastError();
+  f();
+  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+}
+
 // N values of type T side by side, loaded or stored as one vector at any address that suits one of them: the memory
 // instructions take that, so that rows of odd length need no path of their own (results of a product, 20993 x 4062 bf16: 123 us value by
 // value, 72 this way).

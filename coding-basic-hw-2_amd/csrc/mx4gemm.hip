@@ -681,7 +681,7 @@ int mx4_gemm(const ggemm_mx4_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s
   if (need && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
   const Way w = way_of(*p);
   if (w.tiles >= (1 << 23)) return GGEMM_ERR_INVALID;   // 512 threads each: a grid of 2^32
-  with_elem(p->dtype, [&](auto d) {
+  return launch([&] { with_elem(p->dtype, [&](auto d) {
     auto go = [&](auto inner) {
       constexpr int D = decltype(d)::value;
       constexpr bool I = decltype(inner)::value;
@@ -694,8 +694,7 @@ int mx4_gemm(const ggemm_mx4_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s
     };
     if (p->form == GGEMM_MX4_INNER) go(std::true_type{});
     else go(std::false_type{});
-  });
-  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+  }); });
 }
 
 }  // namespace ggemm

@@ -400,7 +400,7 @@ int mx4_quantize(const ggemm_mx4_quant_t* q, hipStream_t s) {
     return GGEMM_ERR_INVALID;
   if (along && !codes_ok(q->codes, q->ld_codes, q->scales, q->ld_scales, q->cols)) return GGEMM_ERR_INVALID;
   if (down && !codes_ok(q->codes_t, q->ld_codes_t, q->scales_t, q->ld_scales_t, q->rows)) return GGEMM_ERR_INVALID;
-  with_elem(q->dtype, [&](auto d) {
+  return launch([&] { with_elem(q->dtype, [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (down) {
       const int64_t tiles = (int64_t)ceil_div(q->rows, Turn<D>::kRows) * ceil_div(q->cols, Turn<D>::kCols);
@@ -418,8 +418,7 @@ int mx4_quantize(const ggemm_mx4_quant_t* q, hipStream_t s) {
       const int chunks = 4 * ceil_div(q->cols, 32), l = log_lanes(chunks);
       quant_rows_kernel<D><<<row_grid(q->rows, chunks, l), kThreads, 0, s>>>(*q, l);
     }
-  });
-  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+  }); });
 }
 
 int mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t s) {
@@ -428,14 +427,13 @@ int mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t s) {
   if (!codes_ok(d->codes, d->ld_codes, d->scales, d->ld_scales, d->cols) || !d->y || d->ld < d->cols ||
       !aligned(d->y, elem_bytes(d->dtype)))
     return GGEMM_ERR_INVALID;
-  with_elem(d->dtype, [&](auto t) {
+  return launch([&] { with_elem(d->dtype, [&](auto t) {
     constexpr int D = decltype(t)::value;
     const int chunks = ceil_div(d->cols, Sixteen<D>::N), l = log_lanes(chunks);
     const dim3 grid = row_grid(d->rows, chunks, l);
     if (aligned(d->y, 64) && d->ld * elem_bytes(D) % 64 == 0) dequant_kernel<D, true><<<grid, kThreads, 0, s>>>(*d, l);
     else dequant_kernel<D, false><<<grid, kThreads, 0, s>>>(*d, l);
-  });
-  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+  }); });
 }
 
 }  // namespace ggemm

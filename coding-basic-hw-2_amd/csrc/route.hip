@@ -709,27 +709,28 @@ int route(const ggemm_router_t* r, void* ws, size_t ws_bytes, hipStream_t s) {
   if (!ws || !aligned(ws, 16)) return GGEMM_ERR_INVALID;
   const Shape sh = shape_of(r->tokens);
   const RouteWs w = carve(ws, sh, r->experts);
-  with_elem(r->dtype, [&](auto d) {
-    with_lanes(r->experts, [&](auto l, auto v) {
-      constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
-      auto go = [&](auto one) {
-        constexpr int NT = first_threads(L * V, decltype(one)::value);
-        const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + NT / 64 * L * V * 4;
-        route_kernel<D, L, V, decltype(one)::value><<<sh.groups, NT, lds, s>>>(*r, w, sh.span);
-      };
-      if (sh.groups == 1) go(std::true_type{});
-      else go(std::false_type{});
+  return launch([&] {
+    with_elem(r->dtype, [&](auto d) {
+      with_lanes(r->experts, [&](auto l, auto v) {
+        constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
+        auto go = [&](auto one) {
+          constexpr int NT = first_threads(L * V, decltype(one)::value);
+          const size_t lds = (size_t)r->experts * (sh.span / 32) * 4 + NT / 64 * L * V * 4;
+          route_kernel<D, L, V, decltype(one)::value><<<sh.groups, NT, lds, s>>>(*r, w, sh.span);
+        };
+        if (sh.groups == 1) go(std::true_type{});
+        else go(std::false_type{});
+      });
     });
-  });
-  if (sh.groups > 1) {
-    if (r->experts <= kThreads && (int64_t)sh.groups * r->experts <= kFewCounts) {
-      route_place_kernel<true><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
-    } else {
-      route_scan_kernel<<<ceil_div(r->experts, 16), 16 * kRuns, 0, s>>>(*r, w, sh.groups);
-      route_place_kernel<false><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+    if (sh.groups > 1) {
+      if (r->experts <= kThreads && (int64_t)sh.groups * r->experts <= kFewCounts) {
+        route_place_kernel<true><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+      } else {
+        route_scan_kernel<<<ceil_div(r->experts, 16), 16 * kRuns, 0, s>>>(*r, w, sh.groups);
+        route_place_kernel<false><<<sh.groups, kThreads, 0, s>>>(*r, w, sh.span);
+      }
     }
-  }
-  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+  });
 }
 
 int route_backward(const ggemm_router_t* r, const float* d_gates, const float* d_loss, void* d_logits, int64_t ld_d,
@@ -737,15 +738,14 @@ int route_backward(const ggemm_router_t* r, const float* d_gates, const float* d
   if (!route_ok(r)) return GGEMM_ERR_INVALID;
   if (r->tokens == 0) return GGEMM_OK;
   if (!d_logits || !aligned(d_logits, elem_bytes(r->dtype)) || ld_d < r->experts) return GGEMM_ERR_INVALID;
-  with_elem(r->dtype, [&](auto d) {
+  return launch([&] { with_elem(r->dtype, [&](auto d) {
     with_lanes(r->experts, [&](auto l, auto v) {
       constexpr int D = decltype(d)::value, L = decltype(l)::value, V = decltype(v)::value;
       constexpr int kPar = 256 / L;
       const int per = std::max(kPar, (int)align_up((size_t)ceil_div(r->tokens, 2048), kPar));
       route_backward_kernel<D, L, V><<<ceil_div(r->tokens, per), kThreads, 0, s>>>(*r, d_gates, d_loss, d_logits, ld_d, per);
     });
-  });
-  return hipGetLastError() == hipSuccess ? GGEMM_OK : GGEMM_ERR_CUDA;
+  }); });
 }
 
 }  // namespace ggemm

@@ -38,3 +38,35 @@ def test_layer_without_tokens(dtype):
     assert bool((out == 5.0).all())
     out = R.gemm(G.MX4_INNER, at, at, d, d, rows, torch.full((E, d, d), 5.0, device="cuda"), o["offsets"], E, c_stride=d * d)
     assert bool((out == 0.0).all())
+
+
+def test_older_error_is_not_the_calls():
+    """An error that an earlier call of the program left behind (here: a device that does not exist) is not reported as a
+    failed launch."""
+    say("older error")
+    hip = C.CDLL("libamdhip64.so")
+    x = torch.randn(70, 96, device="cuda")
+    y = torch.zeros(70, 96, device="cuda")
+    c, s = torch.zeros(70, 48, dtype=torch.uint8, device="cuda"), torch.zeros(70, 4, dtype=torch.uint8, device="cuda")
+    out = torch.zeros(70, 70, device="cuda")
+    q = G.Mx4Quant(70, 96, G.F32, 70, x.data_ptr(), 96, None, c.data_ptr(), 48, s.data_ptr(), 4, None, 0, None, 0)
+    d = G.Mx4Dequant(70, 96, G.F32, c.data_ptr(), 48, s.data_ptr(), 4, y.data_ptr(), 96)
+    p = G.Mx4Gemm(G.MX4_ROWS, 1, 70, 70, 96, G.F32, 1.0, 0.0, c.data_ptr(), 48, s.data_ptr(), 4, c.data_ptr(), 48, 0,
+                  s.data_ptr(), 4, 0, None, out.data_ptr(), 70, 0)
+    ws = torch.zeros(max(16, G.lib().ggemm_mx4_gemm_workspace(C.byref(p))), dtype=torch.uint8, device="cuda")
+    r, o, rws = R.gpu_route(x, None, 2, 1, True, 0.1)
+    dx = torch.zeros(70, 96, device="cuda")
+    calls = {"quantize": lambda: G.lib().ggemm_mx4_quantize(C.byref(q), R.stream()),
+             "dequantize": lambda: G.lib().ggemm_mx4_dequantize(C.byref(d), R.stream()),
+             "gemm": lambda: G.lib().ggemm_mx4_gemm(C.byref(p), ws.data_ptr(), ws.numel(), R.stream()),
+             "route": lambda: G.lib().ggemm_route(C.byref(r), rws.data_ptr(), rws.numel(), R.stream()),
+             "route_backward": lambda: G.lib().ggemm_route_backward(C.byref(r), None, None, dx.data_ptr(), 96, R.stream())}
+    torch.cuda.synchronize()
+    rc = {}
+    for name, call in calls.items():
+        assert hip.hipSetDevice(9999) != 0
+        rc[name] = call()
+        hip.hipGetLastError()
+    torch.cuda.synchronize()
+    assert rc == {name: G.GGEMM_OK for name in calls}
+    assert bool(((y - x).abs() <= 0.5 * x.abs().amax(1, keepdim=True)).all()) and bool(out.any())

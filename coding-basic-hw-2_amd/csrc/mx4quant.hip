@@ -379,7 +379,8 @@ dim3 row_grid(int rows, int chunks, int log_cx) {
   return dim3((unsigned)std::min(ceil_div(rows, per), std::max(1, 2048 / y)), (unsigned)y);
 }
 
-constexpr int kMaxCols = 1 << 25;   // 4 columns a lane or more, 256 lanes a workgroup: at most 32768 workgroups along a row
+// 4 columns a lane or more, 256 lanes a workgroup: at most 32768 workgroups along a row.
+constexpr int kMaxCols = GGEMM_MX4_MAX_COLS;
 
 bool codes_ok(const uint8_t* codes, int64_t ld_codes, const uint8_t* scales, int64_t ld_scales, int cols) {
   const int64_t nb = ceil_div(cols, 32);

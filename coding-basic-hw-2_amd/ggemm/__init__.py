@@ -105,7 +105,7 @@ class ReuseBytes(C.Structure):
 F32, BF16, F16 = 0, 1, 2
 DTYPES = {"f32": F32, "bf16": BF16, "f16": F16}
 MX4_ROWS, MX4_INNER = 0, 1
-MX4_BLOCK, MX4_MAX_GROUPS = 32, 4096
+MX4_BLOCK, MX4_MAX_COLS, MX4_MAX_GROUPS = 32, 1 << 25, 4096
 ROUTE_MAX_TOKENS, ROUTE_MAX_EXPERTS, ROUTE_MAX_TOPK, ROUTE_MAX_ALIGN = 1 << 30, 1024, 64, 1024
 
 

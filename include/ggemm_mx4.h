@@ -27,6 +27,7 @@ extern "C" {
 #define GGEMM_F16  2
 
 #define GGEMM_MX4_BLOCK 32
+#define GGEMM_MX4_MAX_COLS (1 << 25)   /* a quantised row; quantisation and back */
 #define GGEMM_MX4_MAX_GROUPS 4096
 
 /* Quantisation of a rows x cols matrix: row i is x[i], or with an index x[index[i]], and zeros where
@@ -37,7 +38,8 @@ extern "C" {
  *   codes / scales     blocks along the rows:      rows x round_up(cols, 32) / 2 and / 32 bytes
  *   codes_t / scales_t blocks down the columns, stored transposed: cols x round_up(rows, 32) / 2, / 32
  * Either pair may be NULL, not both.  codes 16-byte aligned with ld_codes a multiple of 16; ld of
- * scales a multiple of 4, scales 4-byte aligned; bytes of a scale row past its blocks are not written. */
+ * scales a multiple of 4, scales 4-byte aligned; bytes of a scale row past its blocks are not written.
+ * cols (with codes_t: and rows) up to GGEMM_MX4_MAX_COLS. */
 typedef struct {
   int rows, cols;
   int dtype;                     /* of x: GGEMM_F32, GGEMM_BF16, GGEMM_F16 */
@@ -51,7 +53,8 @@ typedef struct {
 } ggemm_mx4_quant_t;
 int ggemm_mx4_quantize(const ggemm_mx4_quant_t* q, hipStream_t stream);
 
-/* y[i, j] = the value that code and scale stand for, rounded once to y's type (only f16 rounds). */
+/* y[i, j] = the value that code and scale stand for, rounded once to y's type (only f16 rounds).  cols up to
+ * GGEMM_MX4_MAX_COLS; codes and scales aligned as the quantisation's. */
 typedef struct {
   int rows, cols;
   int dtype;                     /* of y */
@@ -61,7 +64,7 @@ typedef struct {
 } ggemm_mx4_dequant_t;
 int ggemm_mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t stream);
 
-/* Grouped products of quantised matrices, sums in 32 bits, one rounding to C's type.  offsets: device
+/* Grouped products of quantised matrices, sums in 32 bits (subnormals kept), one rounding to C's type.  offsets: device
  * array of groups + 1 ascending values, or NULL for one group that spans everything.
  *   GGEMM_MX4_ROWS   C[r, :] = alpha A[r, :] B_g^T + beta C[r, :] for offsets[g] <= r < offsets[g + 1]
  *                    A m x k, B_g n x k (b_stride / b_scales_stride bytes apart), C m x n.  Rows of C
@@ -72,8 +75,8 @@ int ggemm_mx4_dequantize(const ggemm_mx4_dequant_t* d, hipStream_t stream);
  * Offsets are read on the device; they are clamped to [0, m] or [0, k], so wrong ones give wrong
  * results but no access out of bounds.  alpha == 0 still multiplies; with beta == 0 C is not read.  k = 0 (or
  * an empty K_g) gives beta C.  C must not overlap the inputs.
- * Alignment: a, b and their ld and stride multiples of 16 bytes; scales, their ld and stride of 4 bytes.  C needs
- * its type's alignment only.  Results are the same bits every time.
+ * Alignment: a, b and their ld and stride multiples of 16 bytes; scales, their ld and stride of 4 bytes: expert e's part
+ * of a transposed quantisation, columns k e on, can be B_e if k is a multiple of 128.  C needs its type's alignment only.  Results are the same bits every time.
  * Products of 2^23 or more tiles (16 x 32 to 256 x 256 of C) are refused. */
 #define GGEMM_MX4_ROWS  0
 #define GGEMM_MX4_INNER 1

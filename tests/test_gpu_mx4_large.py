@@ -70,3 +70,24 @@ def test_older_error_is_not_the_calls():
     torch.cuda.synchronize()
     assert rc == {name: G.GGEMM_OK for name in calls}
     assert bool(((y - x).abs() <= 0.5 * x.abs().amax(1, keepdim=True)).all()) and bool(out.any())
+
+
+@pytest.mark.parametrize("m", [3, 100, 9000])
+def test_products_of_subnormal_size(m):
+    """A single product of 1.5 2^e, and two that leave 2^(e - 1), down to e = -152: exact where a 32-bit number holds it
+    (multiples of 2^-149), rounded there below."""
+    say(f"subnormal products {m}")
+    n, k = 64, 64
+    e = np.arange(-152, -152 + n)
+    ac = torch.zeros(m, 32, dtype=torch.uint8, device="cuda")
+    asc = torch.full((m, 4), 127 - 60, dtype=torch.uint8, device="cuda")
+    bsc = R.dev(np.repeat((e + 60 + 127).astype(np.uint8)[:, None], 4, 1))
+    for a0, b0, want in ((0x02, 0x03, np.ldexp(1.5, e)), (0x22, 0xA3, np.ldexp(0.5, e))):      # 1, 1.5;  1 1, 1.5 -1
+        ac[:, 0] = a0
+        bc = torch.zeros(n, 32, dtype=torch.uint8, device="cuda")
+        bc[:, 0] = b0
+        out = R.gemm(G.MX4_ROWS, (ac, asc), (bc, bsc), m, n, k, torch.zeros(m, n, device="cuda"))
+        got = out.double().cpu().numpy()
+        held = np.ldexp(np.round(np.ldexp(want, 149)), -149) == want
+        assert (got[:, held] == want[held]).all() and held.sum() >= 60
+        assert (np.abs(got - want) <= 2.0 ** -149).all()

@@ -62,3 +62,14 @@ def test_quantise_without_a_matrix():
     """x may be NULL only where an index picks from no rows."""
     assert quant(x=None) == quant(x=None, index=None, x_rows=0) == quant(x=None, x_rows=1) == G.GGEMM_ERR_INVALID
     assert quant(x=None, x_rows=0, ld=63) == quant(x=None, x_rows=0, codes=None) == G.GGEMM_ERR_INVALID
+
+
+def test_quantised_row_limit():
+    """One column more than a quantised row can have, along the rows, down the columns and back to values."""
+    n = G.MX4_MAX_COLS + 1
+    long = dict(ld_codes=2 ** 25, ld_scales=2 ** 21)
+    assert G.MX4_MAX_COLS == 2 ** 25
+    assert quant(cols=n, ld=n, **long) == G.GGEMM_ERR_INVALID
+    assert quant(rows=n, codes_t=P, scales_t=P, ld_codes_t=2 ** 25, ld_scales_t=2 ** 21) == G.GGEMM_ERR_INVALID
+    d = G.Mx4Dequant(4, n, G.BF16, P, 2 ** 25, P, 2 ** 21, P, n)
+    assert G.lib().ggemm_mx4_dequantize(C.byref(d), None) == G.GGEMM_ERR_INVALID

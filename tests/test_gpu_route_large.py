@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import ggemm as G
+import mx4_gpu_ref as M
 import mx4_ref as R
 from gpu_util import say
 
@@ -106,3 +107,57 @@ def test_most_tokens():
         # the formula's terms are below 2 |s|; one rounding to 16 bits
         assert bool(((d[t:t + step].double() - want).abs() <= 1e-4 * max(s) + R.UNIT["bf16"] * want.abs()).all())
     assert bool((o["order"][T - n1:first] == -1).all()) and bool((o["order"][first + n1:] == -1).all())
+
+
+def _case(T, E, dtype, seed, masked=0.1, barred=0.05):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    x = torch.randn(T, E, device="cuda", generator=gen) * 2
+    x[torch.rand(T, E, device="cuda", generator=gen) < barred] = -torch.inf
+    mask = (torch.rand(T, device="cuda", generator=gen) >= masked).to(torch.uint8) if masked else None
+    return x.to(R.TORCH[dtype]), mask, gen
+
+
+# Sums of probabilities: at most 128 tokens in 4 or more chains, 4 to 64 partial sums, 9 workgroups a chain and 64 chains:
+# 109 additions of positive terms, 109 2^-24 < 7e-6, beside the entries' own 9e-6; together below the 2e-5 that the
+# smaller calls have.
+REL = 2e-5
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,E,k,align,renorm", [(70001, 200, 8, 32, True), (66000, 1000, 10, 1, False), (90000, 5, 2, 16, False),
+                                                (131072, 64, 6, 128, True), (33001, 129, 3, 1, True), (68000, 24, 12, 4, False)])
+def test_forward_long_spans(dtype, T, E, k, align, renorm):
+    """Spans of 64 and 128 tokens, with tokens left out and experts barred; choices, ranks and order exactly."""
+    say(f"route long spans {dtype} {T} {E} {k}")
+    x, mask, _ = _case(T, E, dtype, T + E)
+    w = M.route(x, mask, k, align, renorm, 0.01)
+    _, o, _ = R.gpu_route(x, mask, k, align, renorm, 0.01)
+    for n in ("ids", "counts", "offsets", "pos", "order"):
+        assert torch.equal(o[n].long(), w[n]), n
+    assert int(o["used"]) == w["used"]
+    for n in ("gates", "probs"):
+        assert bool(((o[n] - w[n]).abs() <= REL * w[n] + 1e-30).all()), n
+    assert abs(float(o["loss"]) - w["loss"]) <= 2 * REL * w["loss"]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k", [(70000, 24, 3), (140001, 7, 2), (40000, 200, 8), (9001, 700, 20), (70, 32, 20), (50, 33, 33), (17, 8, 8),
+                                   (33000, 60, 17), (300, 1024, 64)])
+def test_backward_long_and_many_places(dtype, renorm, T, E, k):
+    """More tokens than the grid covers at once, and more places than a token has lanes."""
+    say(f"route backward long {dtype} {T} {E} {k} {renorm}")
+    x, mask, gen = _case(T, E, dtype, T + E + k)
+    w = M.route(x, mask, k, 1, renorm, 0.3)
+    r, o, _ = R.gpu_route(x, mask, k, 1, renorm, 0.3)
+    assert torch.equal(o["ids"].long(), w["ids"])
+    dg, dl = torch.randn(T, k, device="cuda", generator=gen), torch.full((1,), 1.75, device="cuda")
+    for gates, loss in ((True, True), (True, False), (False, True)):
+        grad, mag = M.route_gradient(w, k, renorm, 0.3, dg.double() * gates, 1.75 * loss)
+        out = torch.full((T, E + 1), 9.0, dtype=R.TORCH[dtype], device="cuda")
+        assert G.lib().ggemm_route_backward(C.byref(r), dg.data_ptr() if gates else None, dl.data_ptr() if loss else None,
+                                            out.data_ptr(), E + 1, R.stream()) == G.GGEMM_OK
+        got = out[:, :E].double()
+        assert bool(((got - grad).abs() <= 3 * REL * mag + R.UNIT[dtype] * grad.abs() + R.TINY[dtype]).all()), (gates, loss)
+        assert bool((got[x == -torch.inf] == 0).all()) and bool((got[~w["on"]] == 0).all()) and bool((out[:, E] == 9.0).all())

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import ggemm as G
+import mx4_gpu_ref as M
 import mx4_ref as R
 from gpu_util import say
 
@@ -91,3 +92,220 @@ def test_products_of_subnormal_size(m):
         held = np.ldexp(np.round(np.ldexp(want, 149)), -149) == want
         assert (got[:, held] == want[held]).all() and held.sum() >= 60
         assert (np.abs(got - want) <= 2.0 ** -149).all()
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _quantised(x, index=None, along=True, down=False, spare=0):
+    """The kernel's codes and scales on the GPU; rows as long as the format needs and `spare` 128-byte lines more."""
+    rows, cols = (x.shape[0] if index is None else index.shape[0]), x.shape[1]
+    bufs, put = [], []
+    for on, r, k in ((along, rows, cols), (down, cols, rows)):
+        for n in (R.up(k, 32) // 2 + 128 * spare, R.up(k, 128) // 32 + 4 * spare):
+            t = torch.full((r, n), 0xA5, dtype=torch.uint8, device="cuda") if on else None
+            bufs.append(t)
+            put += [R.ptr(t), n if on else 0]
+    dt = {v: k for k, v in R.TORCH.items()}[x.dtype]
+    q = G.Mx4Quant(rows, cols, G.DTYPES[dt], x.shape[0], x.data_ptr(), x.stride(0), R.ptr(index), *put)
+    assert G.lib().ggemm_mx4_quantize(C.byref(q), R.stream()) == G.GGEMM_OK
+    return bufs
+
+
+def _same(got, x):
+    """Codes and scales of x's rows, and nothing written past a row's blocks."""
+    codes, scales = got
+    nb = R.up(x.shape[1], 32) // 32
+    step = max(1, 2 ** 23 // x.shape[1])
+    for r in range(0, x.shape[0], step):
+        c, s = M.quantise(x[r:r + step])
+        assert torch.equal(codes[r:r + step, :16 * nb], c) and torch.equal(scales[r:r + step, :nb], s), r
+    assert bool((codes[:, 16 * nb:] == 0xA5).all()) and bool((scales[:, nb:] == 0xA5).all())
+
+
+# rows, cols, spare lines at a row's end.  Along the rows the grid covers 4096 (1024 columns) or 2048 rows at once; down the
+# columns 256 tiles of 256 (f32: 128) x 128 and more are dealt to the dies in runs; rows of whole 128-byte lines are stored
+# past the caches.
+QUANT = [(20000, 1024, 0), (20001, 1003, 0), (8192, 2048, 0), (8192, 2048, 1), (8191, 2047, 0), (16640, 1280, 0), (65537, 96, 0), (300, 40000, 0)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,spare", QUANT)
+def test_quantise_large(dtype, rows, cols, spare):
+    say(f"quantise large {dtype} {rows}x{cols}+{spare}")
+    gen = _gen(rows + cols)
+    x = torch.randn(rows, cols, device="cuda", generator=gen) * torch.exp(torch.randn(rows, 1, device="cuda", generator=gen))
+    x = x.to(R.TORCH[dtype])
+    xt = x.t().contiguous()
+    c, s, ct, st = _quantised(x, down=True, spare=spare)
+    _same((c, s), x)
+    _same((ct, st), xt)
+    c, s, _, _ = _quantised(x, spare=spare)
+    _same((c, s), x)
+    _, _, ct, st = _quantised(x, along=False, down=True, spare=spare)
+    _same((ct, st), xt)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(8192, 1024), (30000, 520)])
+def test_quantise_gather_large(dtype, rows, cols):
+    say(f"quantise gather large {dtype} {rows}x{cols}")
+    gen = _gen(rows)
+    x = torch.randn(rows // 2, cols, device="cuda", generator=gen).to(R.TORCH[dtype])
+    index = torch.randint(-1, rows // 2, (rows,), device="cuda", generator=gen, dtype=torch.int32)
+    picked = torch.where((index >= 0)[:, None], x[index.clamp(min=0).long()], torch.zeros((), dtype=x.dtype, device="cuda"))
+    c, s, ct, st = _quantised(x, index, down=True)
+    _same((c, s), picked)
+    _same((ct, st), picked.t().contiguous())
+    c, s, _, _ = _quantised(x, index)
+    _same((c, s), picked)
+
+
+def test_quantise_past_31_bits():
+    """2.8e9 values: rows at both ends, around the 2^31st value and in the middle; columns at both ends."""
+    rows, cols = 70000, 40000
+    say("quantise past 31 bits")
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    gen = _gen(4)
+    for r in range(0, rows, 4096):
+        x[r:r + 4096] = torch.randn(min(4096, rows - r), cols, device="cuda", generator=gen)
+    c, s, ct, st = _quantised(x, down=True)
+    c2, s2, _, _ = _quantised(x)
+    assert torch.equal(c, c2) and torch.equal(s[:, :cols // 32], s2[:, :cols // 32])
+    torch.cuda.synchronize()
+    say("quantise past 31 bits: compared")
+    for r in (0, 31000, 2 ** 31 // cols - 100, rows - 200):
+        wc, ws = M.quantise(x[r:r + 200])
+        assert torch.equal(c[r:r + 200], wc) and torch.equal(s[r:r + 200, :cols // 32], ws), r
+    nr = R.up(rows, 32) // 32
+    for k in (0, 20000, cols - 100):
+        wc, ws = M.quantise(x[:, k:k + 100].t().contiguous())
+        assert torch.equal(ct[k:k + 100, :16 * nr], wc) and torch.equal(st[k:k + 100, :nr], ws), k
+    y = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    d = G.Mx4Dequant(rows, cols, G.BF16, c.data_ptr(), c.shape[1], s.data_ptr(), s.shape[1], y.data_ptr(), cols)
+    assert G.lib().ggemm_mx4_dequantize(C.byref(d), R.stream()) == G.GGEMM_OK
+    for r in (0, 2 ** 31 // cols - 100, rows - 200):
+        assert torch.equal(y[r:r + 200].double(), M.values(c[r:r + 200], s[r:r + 200], cols)), r
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,ld", [(20000, 1024, 1024), (20001, 1003, 1003), (20000, 1000, 1024), (9000, 4096, 4096), (33000, 40, 64)])
+def test_dequantise_large(dtype, rows, cols, ld):
+    say(f"dequantise large {dtype} {rows}x{cols}")
+    gen = _gen(cols)
+    codes, scales = M.operand(gen, rows, cols, 100, 150)      # 16-bit values: subnormal ones and some beyond the largest
+    scales[::7, 0] = 255
+    y = torch.full((rows, ld), 7.0, dtype=R.TORCH[dtype], device="cuda")
+    d = G.Mx4Dequant(rows, cols, G.DTYPES[dtype], codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1],
+                     y.data_ptr(), ld)
+    assert G.lib().ggemm_mx4_dequantize(C.byref(d), R.stream()) == G.GGEMM_OK
+    want = M.values(codes, scales, cols).to(R.TORCH[dtype])
+    assert torch.equal(torch.nan_to_num(y[:, :cols].float(), nan=12345.0), torch.nan_to_num(want.float(), nan=12345.0))
+    assert bool((y[:, cols:] == 7.0).all())
+
+
+def _near(got, want, mass, k, dtype, what):
+    """Each of k additions off by one 32-bit truncation of at most the sum of magnitudes; the output's rounding."""
+    tol = (k + 4) * 2.0 ** -23 * mass + 2 * R.UNIT[dtype] * want.abs() + R.TINY[dtype]
+    assert bool(((got.double() - want).abs() <= tol).all()), what
+
+
+def _rows_case(gen, m, n, k, off, dtype, ldc, beta, lo=123, hi=132):
+    groups = len(off) - 1
+    a, b = M.operand(gen, m, k, lo, hi), M.operand(gen, groups * n, k, lo, hi)
+    out = torch.empty(m, ldc, dtype=R.TORCH[dtype], device="cuda")
+    for r in range(0, m, 4096):
+        out[r:r + 4096] = torch.randn(min(4096, m - r), ldc, device="cuda", generator=gen)
+    before = out.clone() if beta or ldc > n else None
+    R.gemm(G.MX4_ROWS, a, b, m, n, k, out, R.dev(np.array(off, dtype=np.int32)), groups, beta=beta,
+           b_strides=(n * b[0].shape[1], n * b[1].shape[1]), ldc=ldc)
+    torch.cuda.synchronize()
+    for g in range(groups):
+        w = M.values(b[0][g * n:(g + 1) * n], b[1][g * n:(g + 1) * n], k).t().contiguous()
+        for r in range(off[g], off[g + 1], 2048):
+            e = min(r + 2048, off[g + 1])
+            av = M.values(a[0][r:e], a[1][r:e], k)
+            want, mass = av @ w, av.abs() @ w.abs()
+            if beta:
+                want, mass = want + beta * before[r:e, :n].double(), mass + abs(beta) * before[r:e, :n].double().abs()
+            _near(out[r:e, :n], want, mass, k, dtype, (g, r))
+    if ldc > n:
+        assert torch.equal(out[:, n:], before[:, n:])
+
+
+@pytest.mark.parametrize("dtype,m,n,k,off,ldc,beta", [
+    ("f32", 9000, 8192, 300, (0, 3000, 3001, 9000), 8192, 0.0),
+    ("f32", 8300, 8200, 320, (0, 8300), 8208, -0.5),
+    ("bf16", 17000, 8192, 256, (0, 5, 9000, 9000, 17000), 8192, 0.0),
+    ("bf16", 17000, 8010, 96, (0, 8500, 17000), 8032, 1.0),
+    ("f16", 17000, 8192, 288, (0, 17000), 8192, 0.0),
+])
+def test_rows_stored_past_the_caches(dtype, m, n, k, off, ldc, beta):
+    """C of more than 256 MB with rows at multiples of 64 bytes."""
+    say(f"rows streamed {dtype} {m} {n} {k}")
+    assert m * n * (4 if dtype == "f32" else 2) > 2 ** 28 and ldc * (4 if dtype == "f32" else 2) % 64 == 0
+    _rows_case(_gen(m + n + k), m, n, k, off, dtype, ldc, beta, *((115, 123) if dtype == "f16" else (123, 132)))
+
+
+def test_rows_results_past_31_bits():
+    """2.3e9 results."""
+    say("rows results past 31 bits")
+    _rows_case(_gen(1), 70000, 32800, 64, (0, 100, 69000, 70000), "bf16", 32800, 0.0)
+
+
+def test_rows_weights_past_32_bits():
+    """4.6e9 bytes of codes in the weights of 70 groups, a few rows each."""
+    say("rows weights past 32 bits")
+    off = [9 * g for g in range(71)]
+    _rows_case(_gen(2), 630, 8192, 16000, off, "f32", 8192, 0.0)
+
+
+@pytest.mark.parametrize("dtype,groups,m,n,k,pad,beta", [
+    ("f32", 3, 4100, 6000, 3200, 0, 0.0), ("f32", 5, 4096, 4096, 4000, 16, 1.0), ("bf16", 9, 4096, 4096, 5000, 0, 0.0),
+    ("f16", 9, 4000, 4112, 5000, 16, 0.0),                       # more than 256 MB
+    ("f16", 2, 2048, 4096, 2000, 0, 0.0), ("f16", 3, 1000, 700, 2500, 1, 0.5), ("f16", 5, 20, 500, 3000, 0, 0.0),
+    ("f16", 1, 16, 33, 640, 0, 0.0), ("f16", 1, 128, 130, 30000, 0, 0.0), ("f16", 70, 64, 64, 2000, 3, 0.0),
+])
+def test_inner_large_and_f16(dtype, groups, m, n, k, pad, beta):
+    say(f"inner {dtype} {groups} {m} {n} {k}")
+    gen = _gen(m + n + k)
+    lo, hi = (113, 121) if dtype == "f16" else (123, 132)
+    a, b = M.operand(gen, m, k, lo, hi), M.operand(gen, n, k, lo, hi)
+    cut = np.sort(np.random.default_rng(k).integers(0, k // 32 + 1, groups - 1)) * 32
+    off, ldc = np.concatenate([[0], cut, [k]]).astype(np.int32), n + pad
+    out = torch.randn(groups, m, ldc, device="cuda", generator=gen).to(R.TORCH[dtype])
+    before = out.clone()
+    R.gemm(G.MX4_INNER, a, b, m, n, k, out, R.dev(off), groups, ldc=ldc, c_stride=m * ldc, beta=beta)
+    av, bv = M.values(*a, k), M.values(*b, k)
+    for g in range(groups):
+        s = slice(int(off[g]), int(off[g + 1]))
+        w = bv[:, s].t().contiguous()
+        want, mass = av[:, s] @ w, av[:, s].abs() @ w.abs()
+        if beta:
+            want, mass = want + beta * before[g, :, :n].double(), mass + beta * before[g, :, :n].double().abs()
+        _near(out[g, :, :n], want, mass, k, dtype, g)
+        assert torch.equal(out[g, :, n:], before[g, :, n:])
+
+
+@pytest.mark.parametrize("E,n,k,m", [(5, 128, 100, 77), (3, 384, 257, 1000), (40, 256, 1000, 60), (2, 2048, 1024, 6000), (16, 128, 32, 3)])
+def test_input_gradient_on_transposed_weights(E, n, k, m):
+    """dX[r] = dH[r] W_e by ROWS on the columns n e .. of the stacked weights' transposed quantisation, whose rows hold all
+    experts; accumulated too."""
+    say(f"input gradient {E} {n} {k} {m}")
+    gen = _gen(E + n + k)
+    W = torch.randn(E * n, k, device="cuda", generator=gen)
+    _, _, wt, wts = _quantised(W, along=False, down=True)
+    a = M.operand(gen, m, n)
+    off = np.concatenate([[0], np.sort(np.random.default_rng(m).integers(0, m + 1, E - 1)), [m]]).astype(np.int32)
+    first = R.gemm(G.MX4_ROWS, a, (wt, wts), m, k, n, torch.zeros(m, k, device="cuda"), R.dev(off), E, b_strides=(n // 2, n // 32))
+    again = R.gemm(G.MX4_ROWS, a, (wt, wts), m, k, n, first.clone(), R.dev(off), E, b_strides=(n // 2, n // 32), beta=1.0)
+    av, wv = M.values(*a, n), M.values(wt, wts, E * n)
+    for g in range(E):
+        s = slice(int(off[g]), int(off[g + 1]))
+        w = wv[:, g * n:(g + 1) * n].t().contiguous()
+        want, mass = av[s] @ w, av[s].abs() @ w.abs()
+        _near(first[s], want, mass, n, "f32", g)
+        _near(again[s], want + first[s].double(), mass + first[s].double().abs(), n, "f32", g)

@@ -309,3 +309,48 @@ def test_input_gradient_on_transposed_weights(E, n, k, m):
         want, mass = av[s] @ w, av[s].abs() @ w.abs()
         _near(first[s], want, mass, n, "f32", g)
         _near(again[s], want + first[s].double(), mass + first[s].double().abs(), n, "f32", g)
+
+
+def _at(t, skip, spare):
+    """t's rows in a buffer that begins `skip` bytes late and has `spare` more bytes a row, all of them 255."""
+    rows, n = t.shape
+    buf = torch.full((skip + rows * (n + spare),), 255, dtype=torch.uint8, device="cuda")
+    v = buf[skip:].view(rows, n + spare)
+    v[:, :n] = t
+    return v
+
+
+@pytest.mark.parametrize("m,n,k,groups", [(5, 70, 3000, 2), (40, 300, 1500, 3), (700, 500, 1300, 4), (300, 260, 20000, 1),
+                                          (9000, 4100, 1200, 3), (2000, 515, 2050, 9)])
+def test_products_at_least_alignment(m, n, k, groups):
+    """Codes at odd multiples of 16 bytes and scales at odd multiples of 4, rows and weights further apart than they are
+    long; every tile shape, with whole and ragged windows of scales."""
+    say(f"least alignment {m} {n} {k} {groups}")
+    gen = _gen(m + n + k)
+    a, b = M.operand(gen, m, k), M.operand(gen, groups * n, k)
+    av, bv = M.values(*a, k), M.values(*b, k)
+    off = np.concatenate([[0], np.sort(np.random.default_rng(n).integers(0, m + 1, groups - 1)), [m]]).astype(np.int32)
+    a2, b2 = (_at(a[0], 16, 48), _at(a[1], 4, 4)), (_at(b[0], 48, 16), _at(b[1], 12, 20))
+    assert a2[0].data_ptr() % 32 == 16 and a2[1].data_ptr() % 8 == 4 and b2[1].data_ptr() % 8 == 4
+    for dtype, skip in (("f32", 1), ("bf16", 3), ("f16", 1)):
+        ldc = n + 3
+        out = torch.full((m * ldc + skip,), 5.0, dtype=R.TORCH[dtype], device="cuda")
+        c = out[skip:].view(m, ldc)
+        R.gemm(G.MX4_ROWS, a2, b2, m, n, k, c, R.dev(off), groups, b_strides=(n * b2[0].stride(0), n * b2[1].stride(0)), ldc=ldc,
+               alpha=2.0 ** -9 if dtype == "f16" else 1.0)
+        for g in range(groups):
+            s, w = slice(int(off[g]), int(off[g + 1])), bv[g * n:(g + 1) * n].t().contiguous()
+            want, mass = av[s] @ w, av[s].abs() @ w.abs()
+            f = 2.0 ** -9 if dtype == "f16" else 1.0
+            _near(c[s, :n], f * want, f * mass, k, dtype, (dtype, g))
+        assert bool((c[:, n:] == 5.0).all())
+    if groups * m * n < 2 ** 25:       # the same operands' columns cut into groups
+        b3 = (b2[0][:n], b2[1][:n])
+        cut = np.concatenate([[0], np.sort(np.random.default_rng(m).integers(0, k // 32 + 1, groups - 1)) * 32, [k]]).astype(np.int32)
+        out = torch.full((groups, m, n + 1), 5.0, device="cuda")
+        R.gemm(G.MX4_INNER, a2, b3, m, n, k, out, R.dev(cut), groups, ldc=n + 1, c_stride=m * (n + 1))
+        for g in range(groups):
+            s = slice(int(cut[g]), int(cut[g + 1]))
+            w = bv[:n, s].t().contiguous()
+            _near(out[g, :, :n], av[:, s] @ w, av[:, s].abs() @ w.abs(), k, "f32", ("inner", g))
+        assert bool((out[..., n:] == 5.0).all())

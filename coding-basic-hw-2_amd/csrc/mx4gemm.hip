@@ -4,11 +4,12 @@
 // bytes) of row l % 32 at block l / 32 of two, and that block's scale byte, one of the four bytes of a register
 // that the instruction names; products of codes are exact, sums are 32-bit.  The operands are given in the
 // order B, A, so that a lane gets four neighbouring columns of one row of C.
-// Rates, from registers only with random codes: 32x32x64 6.5 PFLOP/s, 16x16x128 5.8 (zeros: 9.6 and 7.3; the
+// Rates, from registers only with random codes: 32x32x64 6.6 PFLOP/s, 16x16x128 5.8 (zeros: 9.4 and 7.1; the
 // card lowers its clock under the products' power), so the tiles use the former.
-// Bound: 256 x 256 tiles over a long inner dimension, that power (8192 x 8192 x 16384: 499 us, 4.4 PFLOP/s, at 1.85
-// GHz with the matrix cores busy 53 % of the cycles; all zeros 403 us at 2.46 GHz); over a short one, also the
-// stores of C (8192 x 8192 x 1024: 56 us); few rows, the bytes of B.
+// Bound: 256 x 256 tiles over a long inner dimension, the loop's cycles at the clock that the products' power leaves
+// (8192 x 8192 x 16384: 917 thousand cycles, the matrix cores busy 57 % of them; 501 us, 4.4 PFLOP/s; all zeros
+// the same cycles in 380 us); over a short one, also the stores of C (8192 x 8192 x 1024: 53 us), which a tile's first wait
+// for its operands waits for too (one counter); few rows, the bytes of B.
 #include <algorithm>
 #include <type_traits>
 

@@ -2,7 +2,8 @@
 
 Mirrors the C ABI of include/ggemm.h, include/ggemm_graph.h and include/ggemm_oz2.h: same names,
 struct layouts and return codes as the reference's interface; and that of include/ggemm_mx4.h (4-bit
-quantisation and grouped products) and include/ggemm_route.h (the router of an expert layer).  Device memory is passed as plain
+quantisation and grouped products), include/ggemm_route.h (the router of an expert layer), include/ggemm_glu.h (the gated
+feed-forward block and its gradients) and include/ggemm_w8.h (8-bit integer products).  Device memory is passed as plain
 integer addresses (e.g. torch_tensor.data_ptr()); streams as integer handles (0 = default).
 The library must be built (coding-basic-hw-2_amd/build_lib.py); there is no fallback path.
 """
@@ -106,6 +107,10 @@ F32, BF16, F16 = 0, 1, 2
 DTYPES = {"f32": F32, "bf16": BF16, "f16": F16}
 MX4_ROWS, MX4_INNER = 0, 1
 MX4_BLOCK, MX4_MAX_COLS, MX4_MAX_GROUPS = 32, 1 << 25, 4096
+SILU, GELU, GELU_TANH = 1, 2, 3
+ACTS = {"silu": SILU, "gelu": GELU, "gelu_tanh": GELU_TANH}
+GLU_MAX_GROUPS, GLU_MAX_LD = 4096, 1 << 22
+W8_MAX_COLS, W8_MAX_GROUPS, W8_MAX_LD = 1 << 17, 4096, 1 << 23
 ROUTE_MAX_TOKENS, ROUTE_MAX_EXPERTS, ROUTE_MAX_TOPK, ROUTE_MAX_ALIGN = 1 << 30, 1024, 64, 1024
 
 
@@ -142,6 +147,42 @@ class Router(C.Structure):
                 ("logits", C.c_void_p), ("ld", C.c_int64), ("mask", C.c_void_p), ("ids", C.c_void_p),
                 ("gates", C.c_void_p), ("pos", C.c_void_p), ("counts", C.c_void_p), ("offsets", C.c_void_p),
                 ("order", C.c_void_p), ("used", C.c_void_p), ("probs", C.c_void_p), ("loss", C.c_void_p)]
+
+
+class Glu(C.Structure):
+    """include/ggemm_glu.h ggemm_glu_t"""
+    _fields_ = [("groups", C.c_int), ("rows", C.c_int), ("d_model", C.c_int), ("d_ff", C.c_int), ("dtype", C.c_int),
+                ("act", C.c_int), ("x_rows", C.c_int), ("x", C.c_void_p), ("ldx", C.c_int64), ("index", C.c_void_p),
+                ("offsets", C.c_void_p), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("ldw", C.c_int64),
+                ("w_stride", C.c_int64), ("w_down", C.c_void_p), ("ldd", C.c_int64), ("d_stride", C.c_int64),
+                ("gate", C.c_void_p), ("up", C.c_void_p), ("ldg", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64)]
+
+
+class GluGrad(C.Structure):
+    """include/ggemm_glu.h ggemm_glu_grad_t"""
+    _fields_ = [("dy", C.c_void_p), ("lddy", C.c_int64), ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw_dtype", C.c_int),
+                ("dw_beta", C.c_float), ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p), ("lddw", C.c_int64),
+                ("dw_stride", C.c_int64), ("dw_down", C.c_void_p), ("lddd", C.c_int64), ("dd_stride", C.c_int64)]
+
+
+class W8Quant(C.Structure):
+    """include/ggemm_w8.h ggemm_w8_quant_t"""
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int), ("x_rows", C.c_int), ("x", C.c_void_p),
+                ("ld", C.c_int64), ("index", C.c_void_p), ("q", C.c_void_p), ("ldq", C.c_int64), ("scales", C.c_void_p)]
+
+
+class W8Dequant(C.Structure):
+    """include/ggemm_w8.h ggemm_w8_dequant_t"""
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("dtype", C.c_int), ("q", C.c_void_p), ("ldq", C.c_int64),
+                ("scales", C.c_void_p), ("y", C.c_void_p), ("ld", C.c_int64)]
+
+
+class W8Gemm(C.Structure):
+    """include/ggemm_w8.h ggemm_w8_gemm_t"""
+    _fields_ = [("groups", C.c_int), ("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("dtype", C.c_int), ("act", C.c_int),
+                ("a", C.c_void_p), ("lda", C.c_int64), ("a_scales", C.c_void_p), ("b", C.c_void_p), ("b_up", C.c_void_p),
+                ("ldb", C.c_int64), ("b_stride", C.c_int64), ("b_scales", C.c_void_p), ("b_up_scales", C.c_void_p),
+                ("b_scales_stride", C.c_int64), ("offsets", C.c_void_p), ("c", C.c_void_p), ("ldc", C.c_int64)]
 
 
 REUSE_EXACT_N, REUSE_PROMOTE = 0, 1
@@ -201,6 +242,14 @@ SIGNATURES = [
     ("ggemm_mx4_gemm", C.c_int, [C.POINTER(Mx4Gemm), _P, C.c_size_t, _P]),
     ("ggemm_route_workspace", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     ("ggemm_route", C.c_int, [C.POINTER(Router), _P, C.c_size_t, _P]),
+    ("ggemm_glu_workspace", C.c_size_t, [C.POINTER(Glu)]),
+    ("ggemm_glu", C.c_int, [C.POINTER(Glu), _P, C.c_size_t, _P]),
+    ("ggemm_glu_backward_workspace", C.c_size_t, [C.POINTER(Glu), C.POINTER(GluGrad)]),
+    ("ggemm_glu_backward", C.c_int, [C.POINTER(Glu), C.POINTER(GluGrad), _P, C.c_size_t, _P]),
+    ("ggemm_w8_quantize", C.c_int, [C.POINTER(W8Quant), _P]),
+    ("ggemm_w8_dequantize", C.c_int, [C.POINTER(W8Dequant), _P]),
+    ("ggemm_w8_gemm_workspace", C.c_size_t, [C.POINTER(W8Gemm)]),
+    ("ggemm_w8_gemm", C.c_int, [C.POINTER(W8Gemm), _P, C.c_size_t, _P]),
     ("ggemm_route_backward", C.c_int, [C.POINTER(Router), _P, _P, _P, C.c_int64, _P]),
 ]
 

@@ -2,181 +2,394 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "simple.hpp"
+#include "act.hpp"
+#include "tiles.hpp"
 
 namespace ggemm {
 namespace {
 
-template <class T>
-__device__ __forceinline__ float as_f(const void* p, int64_t i) { return (float)static_cast<const T*>(p)[i]; }
-
-// The row of x that row r stands for, -1: none.
-__device__ __forceinline__ int64_t source_row(const ggemm_glu_t& p, int r) {
-  if (!p.index) return r;
-  const int i = p.index[r];
-  return i >= 0 && i < p.x_rows ? i : -1;
+// Where a tile of rows of a group lies: rows [m0, m_end), first column, stages of the inner dimension.
+struct Place {
+  int g, m0, m_end, n0, nk;
+};
+template <class C>
+__device__ __forceinline__ Place row_place(const RowGroups& rows, const GroupTiles<C::BM>& first, int t, int n, int width, int nk) {
+  const int nt = ceil_div(n, width);
+  const RowSpan s = find_group(rows, first, t, nt);
+  if (s.g < 0) return Place{-1};
+  int tm, tn;
+  tile_raster(t, ceil_div(s.hi - s.lo, C::BM), nt, tm, tn);
+  return Place{s.g, s.lo + tm * C::BM, s.hi, tn * width, nk};
 }
+__device__ __forceinline__ const uint8_t* bytes_of(const void* p) { return static_cast<const uint8_t*>(p); }
 
-// h, gate, up
-template <class T, int ACT>
+// The rows of x that an index picks, or none.
+struct Picked {
+  const int32_t* index;
+  int x_rows;
+  // index entry of row r, or -1
+  __device__ __forceinline__ int at(int r) const {
+    const int i = index[r];
+    return (uint32_t)i < (uint32_t)x_rows ? i : -1;
+  }
+  __device__ __forceinline__ bool live(int r) const { return !index || at(r) >= 0; }
+};
+
+// h = act(x Wg^T) (x Wu^T), and gate and up where they are kept
+template <int D, int ACT>
 struct Up {
-  using Acc = float;
-  static constexpr int kPairs = 2;
+  using T = typename Elem<D>::T;
+  using M = typename MmaOf<D>::M;
+  using Place = ggemm::Place;
+  static constexpr bool kADown = false, kBDown = false, kPair = true;
+  static constexpr int E = 8;
   ggemm_glu_t p;
   T* h;
   int64_t ldh;
-  int g, lo, hi, n0;
-  __device__ bool place(int t) {
-    if (!simple_rows(p.offsets, p.groups, p.rows, ceil_div(p.d_ff, 64), t, g, lo, hi, n0)) return false;
-    n0 *= 64;
-    return true;
+  __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
+  template <int BM, int BN>
+  __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_ff, BN / 2)); }
+  template <class C>
+  __device__ __forceinline__ Place place(const GroupTiles<C::BM>& first, int t) const {
+    return row_place<C>(rows(), first, t, p.d_ff, C::BN / 2, ceil_div(p.d_model, 64));
   }
-  __device__ int depth() const { return p.d_model; }
-  __device__ float a(int i, int k) const {
-    if (lo + i >= hi || k >= p.d_model) return 0.0f;
-    const int64_t s = source_row(p, lo + i);
-    return s < 0 ? 0.0f : as_f<T>(p.x, s * p.ldx + k);
+  template <class C>
+  struct Src {
+    Along<C, C::BM> a;
+    Along<C, C::BN, true> b;
+    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
+      a.load(kt, slot, wave);
+      b.load(kt, slot + C::SA, wave);
+    }
+    __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
+    __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
+      a.clear(kt, slot);
+      b.clear(kt, slot + C::SA);
+    }
+  };
+  template <class C>
+  __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
+    const int64_t px = 2 * p.ldx, pw = 2 * p.ldw, w0 = 2 * (c.g * p.w_stride + c.n0 * p.ldw);
+    const int bytes = 2 * p.d_model, n = p.d_ff - c.n0;
+    const Picked pick{p.index, p.x_rows};
+    auto at = [&](int row) -> uint32_t {
+      if (!p.index) return (uint32_t)row * (uint32_t)px;
+      const int i = c.m0 + row < c.m_end ? pick.at(c.m0 + row) : -1;
+      return i < 0 ? kOut : (uint32_t)i * (uint32_t)px;
+    };
+    const uint8_t* const x = bytes_of(p.x) + (p.index ? 0 : c.m0 * px);
+    return Src<C>{Along<C, C::BM>(x, nullptr, px, p.index ? p.x_rows : c.m_end - c.m0, bytes, wave, lane, at),
+                  Along<C, C::BN, true>(bytes_of(p.w_gate) + w0, bytes_of(p.w_up) + w0, pw, n, bytes, wave, lane, InOrder{(uint32_t)pw})};
   }
-  __device__ float b(int z, int j, int k) const {
-    if (n0 + j >= p.d_ff || k >= p.d_model) return 0.0f;
-    return as_f<T>(z ? p.w_up : p.w_gate, g * p.w_stride + (n0 + j) * p.ldw + k);
-  }
-  __device__ void emit(int i, int j, const float* s) const {
-    if (lo + i >= hi || n0 + j >= p.d_ff) return;
-    const int64_t r = lo + i, c = n0 + j;
-    h[r * ldh + c] = (T)(act_value<ACT>(s[0]) * s[1]);
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u) const {
+    const int64_t r = c.m0 + row, j = c.n0 + col;
+    if (r >= c.m_end || j >= p.d_ff) return;
+    const int ok = p.d_ff - (int)j;
+    float g[E], w[E], o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) g[e] = v[e], w[e] = u[e], o[e] = act_value<ACT>(v[e]) * u[e];
+    store_some(h + r * ldh + j, ok, o);
     if (p.gate) {
-      static_cast<T*>(p.gate)[r * p.ldg + c] = (T)s[0];
-      static_cast<T*>(p.up)[r * p.ldg + c] = (T)s[1];
+      store_some(static_cast<T*>(p.gate) + r * p.ldg + j, ok, g);
+      store_some(static_cast<T*>(p.up) + r * p.ldg + j, ok, w);
     }
   }
 };
 
 // y = h Wd^T
-template <class T>
-struct Down {
-  using Acc = float;
-  static constexpr int kPairs = 1;
+template <int D>
+struct DownProduct {
+  using T = typename Elem<D>::T;
+  using M = typename MmaOf<D>::M;
+  using Place = ggemm::Place;
+  static constexpr bool kADown = false, kBDown = false, kPair = false;
+  static constexpr int E = 8;
   ggemm_glu_t p;
   const T* h;
   int64_t ldh;
-  int g, lo, hi, n0;
-  __device__ bool place(int t) {
-    if (!simple_rows(p.offsets, p.groups, p.rows, ceil_div(p.d_model, 64), t, g, lo, hi, n0)) return false;
-    n0 *= 64;
-    return true;
+  __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
+  template <int BM, int BN>
+  __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_model, BN)); }
+  template <class C>
+  __device__ __forceinline__ Place place(const GroupTiles<C::BM>& first, int t) const {
+    return row_place<C>(rows(), first, t, p.d_model, C::BN, ceil_div(p.d_ff, 64));
   }
-  __device__ int depth() const { return p.d_ff; }
-  __device__ float a(int i, int k) const { return lo + i < hi && k < p.d_ff ? (float)h[(lo + i) * ldh + k] : 0.0f; }
-  __device__ float b(int, int j, int k) const {
-    return n0 + j < p.d_model && k < p.d_ff ? as_f<T>(p.w_down, g * p.d_stride + (n0 + j) * p.ldd + k) : 0.0f;
+  template <class C>
+  struct Src {
+    Along<C, C::BM> a;
+    Along<C, C::BN> b;
+    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
+      a.load(kt, slot, wave);
+      b.load(kt, slot + C::SA, wave);
+    }
+    __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
+    __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
+      a.clear(kt, slot);
+      b.clear(kt, slot + C::SA);
+    }
+  };
+  template <class C>
+  __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
+    const int64_t ph = 2 * ldh, pw = 2 * p.ldd;
+    const int bytes = 2 * p.d_ff;
+    return Src<C>{Along<C, C::BM>(bytes_of(h) + c.m0 * ph, nullptr, ph, c.m_end - c.m0, bytes, wave, lane, InOrder{(uint32_t)ph}),
+                  Along<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0 * p.ldd), nullptr, pw, p.d_model - c.n0, bytes, wave,
+                                  lane, InOrder{(uint32_t)pw})};
   }
-  __device__ void emit(int i, int j, const float* s) const {
-    if (lo + i < hi && n0 + j < p.d_model) static_cast<T*>(p.y)[(lo + i) * p.ldy + n0 + j] = (T)s[0];
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+    const int64_t r = c.m0 + row, j = c.n0 + col;
+    if (r >= c.m_end || j >= p.d_model) return;
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = v[e];
+    store_some(static_cast<T*>(p.y) + r * p.ldy + j, p.d_model - (int)j, o);
   }
 };
 
-// dh = dy Wd, and from it dgate, dup and h
-template <class T, int ACT>
-struct Inner {
-  using Acc = float;
-  static constexpr int kPairs = 1;
+// dh = dy Wd, and from it, gate and up: dgate, dup and h
+template <int D, int ACT>
+struct Hidden {
+  using T = typename Elem<D>::T;
+  using M = typename MmaOf<D>::M;
+  using Place = ggemm::Place;
+  static constexpr bool kADown = false, kBDown = true, kPair = false;
+  static constexpr int E = 8;
   ggemm_glu_t p;
-  ggemm_glu_grad_t d;
+  const void* dy;
+  int64_t lddy;
   T *dg, *du, *h;
   int64_t ldh;
-  int g, lo, hi, n0;
-  __device__ bool place(int t) {
-    if (!simple_rows(p.offsets, p.groups, p.rows, ceil_div(p.d_ff, 64), t, g, lo, hi, n0)) return false;
-    n0 *= 64;
-    return true;
+  __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
+  template <int BM, int BN>
+  __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_ff, BN)); }
+  template <class C>
+  __device__ __forceinline__ Place place(const GroupTiles<C::BM>& first, int t) const {
+    return row_place<C>(rows(), first, t, p.d_ff, C::BN, ceil_div(p.d_model, 64));
   }
-  __device__ int depth() const { return p.d_model; }
-  __device__ float a(int i, int k) const { return lo + i < hi && k < p.d_model ? as_f<T>(d.dy, (lo + i) * d.lddy + k) : 0.0f; }
-  __device__ float b(int, int j, int k) const {
-    return n0 + j < p.d_ff && k < p.d_model ? as_f<T>(p.w_down, g * p.d_stride + k * p.ldd + n0 + j) : 0.0f;
+  template <class C>
+  struct Src {
+    Along<C, C::BM> a;
+    Down<C, C::BN> b;
+    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
+      a.load(kt, slot, wave);
+      b.load(b.base, kt, slot + C::SA, wave);
+    }
+    __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
+    __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt, slot); }
+  };
+  template <class C>
+  __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
+    const int64_t py = 2 * lddy;
+    return Src<C>{Along<C, C::BM>(bytes_of(dy) + c.m0 * py, nullptr, py, c.m_end - c.m0, 2 * p.d_model, wave, lane, InOrder{(uint32_t)py}),
+                  Down<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0), 2 * p.ldd, p.d_model, p.d_ff - c.n0, wave, lane)};
   }
-  __device__ void emit(int i, int j, const float* s) const {
-    if (lo + i >= hi || n0 + j >= p.d_ff) return;
-    const int64_t r = lo + i, c = n0 + j;
-    const bool live = source_row(p, (int)r) >= 0;
-    const float v = as_f<T>(p.gate, r * p.ldg + c), u = as_f<T>(p.up, r * p.ldg + c);
-    float q, dq;
-    act_parts<ACT>(v, q, dq);
-    dg[r * ldh + c] = live ? (T)(s[0] * u * (q + v * dq)) : (T)0.0f;
-    du[r * ldh + c] = live ? (T)(s[0] * (v * q)) : (T)0.0f;
-    h[r * ldh + c] = live ? (T)(v * q * u) : (T)0.0f;
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+    const int64_t r = c.m0 + row, j = c.n0 + col;
+    if (r >= c.m_end || j >= p.d_ff) return;
+    const int ok = p.d_ff - (int)j;
+    const bool live = Picked{p.index, p.x_rows}.live((int)r);
+    float g[E], u[E], o[E];
+    load_some(static_cast<const T*>(p.gate) + r * p.ldg + j, ok, g);
+    load_some(static_cast<const T*>(p.up) + r * p.ldg + j, ok, u);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float q, dq;
+      act_parts<ACT>(g[e], q, dq);
+      const float a = g[e] * q, w = u[e];
+      u[e] = live ? v[e] * a : 0.0f;
+      o[e] = live ? a * w : 0.0f;
+      g[e] = live ? v[e] * w * fmaf(g[e], dq, q) : 0.0f;
+    }
+    store_some(dg + r * ldh + j, ok, g);
+    store_some(du + r * ldh + j, ok, u);
+    store_some(h + r * ldh + j, ok, o);
   }
 };
 
-// dx = dgate Wg + dup Wu
-template <class T>
-struct Dx {
-  using Acc = float;
-  static constexpr int kPairs = 1;
+// dx = dgate Wg + dup Wu: two inner dimensions, one after the other
+template <int D>
+struct InputGrad {
+  using T = typename Elem<D>::T;
+  using M = typename MmaOf<D>::M;
+  using Place = ggemm::Place;
+  static constexpr bool kADown = false, kBDown = true, kPair = false;
+  static constexpr int E = 8;
   ggemm_glu_t p;
-  ggemm_glu_grad_t d;
+  void* dx;
+  int64_t lddx;
   const T *dg, *du;
   int64_t ldh;
-  int g, lo, hi, n0;
-  __device__ bool place(int t) {
-    if (!simple_rows(p.offsets, p.groups, p.rows, ceil_div(p.d_model, 64), t, g, lo, hi, n0)) return false;
-    n0 *= 64;
-    return true;
+  __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
+  template <int BM, int BN>
+  __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_model, BN)); }
+  template <class C>
+  __device__ __forceinline__ Place place(const GroupTiles<C::BM>& first, int t) const {
+    return row_place<C>(rows(), first, t, p.d_model, C::BN, 2 * ceil_div(p.d_ff, 64));
   }
-  __device__ int depth() const { return 2 * p.d_ff; }
-  __device__ float a(int i, int k) const {
-    if (lo + i >= hi || k >= 2 * p.d_ff) return 0.0f;
-    return k < p.d_ff ? (float)dg[(lo + i) * ldh + k] : (float)du[(lo + i) * ldh + k - p.d_ff];
+  template <class C>
+  struct Src {
+    Along<C, C::BM> a;   // base2: dup
+    Down<C, C::BN> b;
+    const uint8_t* b2;
+    int half;            // stages of each
+    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
+      const bool second = kt >= half;
+      a.load(second ? a.base2 : a.base, nullptr, second ? kt - half : kt, slot, wave);
+      b.load(second ? b2 : b.base, second ? kt - half : kt, slot + C::SA, wave);
+    }
+    __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt >= half ? kt - half : kt); }
+    __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt >= half ? kt - half : kt, slot); }
+  };
+  template <class C>
+  __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
+    const int64_t ph = 2 * ldh, w0 = 2 * (c.g * p.w_stride + c.n0);
+    return Src<C>{Along<C, C::BM>(bytes_of(dg) + c.m0 * ph, bytes_of(du) + c.m0 * ph, ph, c.m_end - c.m0, 2 * p.d_ff, wave, lane,
+                                  InOrder{(uint32_t)ph}),
+                  Down<C, C::BN>(bytes_of(p.w_gate) + w0, 2 * p.ldw, p.d_ff, p.d_model - c.n0, wave, lane), bytes_of(p.w_up) + w0,
+                  ceil_div(p.d_ff, 64)};
   }
-  __device__ float b(int, int j, int k) const {
-    if (n0 + j >= p.d_model || k >= 2 * p.d_ff) return 0.0f;
-    return k < p.d_ff ? as_f<T>(p.w_gate, g * p.w_stride + k * p.ldw + n0 + j)
-                      : as_f<T>(p.w_up, g * p.w_stride + (k - p.d_ff) * p.ldw + n0 + j);
-  }
-  __device__ void emit(int i, int j, const float* s) const {
-    if (lo + i < hi && n0 + j < p.d_model) static_cast<T*>(d.dx)[(lo + i) * d.lddx + n0 + j] = (T)s[0];
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+    const int64_t r = c.m0 + row, j = c.n0 + col;
+    if (r >= c.m_end || j >= p.d_model) return;
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = v[e];
+    store_some(static_cast<T*>(dx) + r * lddx + j, p.d_model - (int)j, o);
   }
 };
 
-// Gradients of the weights: dWg = dgate^T x and dWu = dup^T x (kDown false, z = 0, 1), dWd = dy^T h
-template <class T, class W, bool kDown>
-struct Dw {
-  using Acc = float;
-  static constexpr int kPairs = 1;
+// Gradients of the weights: dWg = dgate^T x, dWu = dup^T x (d_ff x d_model), dWd = dy^T h (d_model x d_ff), in one launch.
+struct WeightPlace {
+  int g, which, lo, m0, n0, depth, nk;
+};
+template <int D, int W, bool kIndexed>
+struct WeightGrad {
+  using T = typename Elem<D>::T;
+  using O = typename Elem<W>::T;
+  using M = typename MmaOf<D>::M;
+  using Place = WeightPlace;
+  static constexpr bool kADown = true, kBDown = true, kPair = false;
+  static constexpr int E = 8;
   ggemm_glu_t p;
   ggemm_glu_grad_t d;
-  const T *left, *right;
-  int64_t ldl, ldr;
-  W* out;
-  int g, lo, hi, m0, n0;
-  __device__ int m() const { return kDown ? p.d_model : p.d_ff; }
-  __device__ int n() const { return kDown ? p.d_ff : p.d_model; }
-  __device__ bool place(int t) {
-    const int mt = ceil_div(m(), 64), nt = ceil_div(n(), 64);
-    g = t / (mt * nt);
-    m0 = t / nt % mt * 64;
-    n0 = t % nt * 64;
-    lo = p.offsets ? min(max(p.offsets[g], 0), p.rows) : 0;
-    hi = p.offsets ? min(max(p.offsets[g + 1], 0), p.rows) : p.rows;
-    return true;
+  const T *dg, *du, *h;
+  int64_t ldh;
+  int first_of;   // 0: all three, 2: dWd only
+  __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
+  template <int BM, int BN>
+  __device__ __forceinline__ int groups() const { return 0; }
+  template <class C>
+  __device__ __forceinline__ Place place(int, int t) const {
+    static_assert(C::BM == C::BN, "as many tiles of each matrix");
+    const int tf = ceil_div(p.d_ff, C::BM), td = ceil_div(p.d_model, C::BM), per = tf * td;
+    Place a;
+    a.which = first_of + t / (per * p.groups);
+    t %= per * p.groups;
+    a.g = t / per;
+    int hi, tm, tn;
+    rows().span(a.g, a.lo, hi);
+    a.depth = max(hi - a.lo, 0);
+    a.nk = ceil_div(a.depth, 64);
+    const bool down = a.which == 2;
+    tile_raster(t % per, down ? td : tf, down ? tf : td, tm, tn);
+    a.m0 = tm * C::BM;
+    a.n0 = tn * C::BM;
+    return a;
   }
-  __device__ int depth() const { return max(hi - lo, 0); }
-  __device__ float a(int i, int k) const {
-    if (lo + k >= hi || m0 + i >= m()) return 0.0f;
-    return source_row(p, lo + k) < 0 ? 0.0f : (float)left[(lo + k) * ldl + m0 + i];
+  template <class C>
+  struct Src {
+    Down<C, C::BM> a;
+    Down<C, C::BN> b;
+    Picked pick;        // of the group's first row on
+    int depth;
+    bool gather;
+    int64_t all;
+    int row[kIndexed ? Down<C, C::BM>::P : 1];
+    // index entries of stage kt's steps
+    __device__ __forceinline__ void fetch(int kt, int wave, int lane) {
+      if constexpr (kIndexed) {
+#pragma unroll
+        for (int q = 0; q < Down<C, C::BM>::P; ++q) {
+          const int k = 64 * kt + Down<C, C::BM>::step(q, wave, lane);
+          row[q] = k < depth ? pick.at(k) : -1;
+        }
+      }
+    }
+    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) {
+      if constexpr (kIndexed) {
+        a.load(a.base, kt, slot, wave, row, false, 0);
+        b.load(b.base, kt, slot + C::SA, wave, row, gather, all);
+        fetch(kt + 1, wave, threadIdx.x & 63);   // a stage ahead
+      } else {
+        a.load(a.base, kt, slot, wave);
+        b.load(b.base, kt, slot + C::SA, wave);
+      }
+    }
+    __device__ __forceinline__ bool ragged(int) const { return false; }
+    __device__ __forceinline__ void clear(int, uint8_t*) const {}
+  };
+  template <class C>
+  __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
+    const bool down = c.which == 2, gather = kIndexed && !down;
+    const int64_t pa = 2 * (down ? d.lddy : ldh), pb = 2 * (down ? ldh : p.ldx);
+    const uint8_t* const a = bytes_of(down ? d.dy : c.which ? (const void*)du : dg) + c.lo * pa + 2 * c.m0;
+    const uint8_t* const b = bytes_of(down ? (const void*)h : p.x) + (gather ? 0 : c.lo * pb) + 2 * c.n0;
+    const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model;
+    Src<C> s{Down<C, C::BM>(a, pa, c.depth, m - c.m0, wave, lane), Down<C, C::BN>(b, pb, c.depth, n - c.n0, wave, lane),
+             Picked{kIndexed ? p.index + c.lo : nullptr, p.x_rows}, c.depth, gather,
+             (p.x_rows - 1) * pb + ((2 * (n - c.n0) + 15) & ~15)};
+    s.fetch(0, wave, lane);
+    return s;
   }
-  __device__ float b(int, int j, int k) const {
-    if (lo + k >= hi || n0 + j >= n()) return 0.0f;
-    const int64_t s = source_row(p, lo + k);
-    return s < 0 ? 0.0f : (float)right[(kDown ? lo + k : s) * ldr + n0 + j];
-  }
-  __device__ void emit(int i, int j, const float* s) const {
-    if (m0 + i >= m() || n0 + j >= n()) return;
-    W* const c = out + (kDown ? g * d.dd_stride + (m0 + i) * d.lddd : g * d.dw_stride + (m0 + i) * d.lddw) + n0 + j;
-    *c = (W)(d.dw_beta != 0.0f ? s[0] + d.dw_beta * (float)*c : s[0]);
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+    const bool down = c.which == 2;
+    const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model, i = c.m0 + row, j = c.n0 + col;
+    if (i >= m || j >= n) return;
+    O* const base = static_cast<O*>(down ? d.dw_down : c.which ? d.dw_up : d.dw_gate);
+    O* const out = base + (down ? c.g * d.dd_stride + i * d.lddd : c.g * d.dw_stride + i * d.lddw) + j;
+    float o[E];
+    if (d.dw_beta != 0.0f) {
+      load_some(static_cast<const O*>(out), n - j, o);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(d.dw_beta, o[e], v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = v[e];
+    }
+    store_some(out, n - j, o);
   }
 };
+
+using Tile256 = TileShape<256, 256, 2, 4>;
+using Tile128 = TileShape<128, 128, 2, 2>;
+using Tile64 = TileShape<64, 128, 2, 2>;
+
+// Tiles of BM rows and `width` columns that a call's groups can need at most.
+int64_t tiles_of(const ggemm_glu_t& p, int bm, int n, int width) { return row_tiles(p.groups, p.rows, bm) * ceil_div(n, width); }
+
+template <class C, class P>
+void run_tiles(const P& p, int64_t tiles, hipStream_t s) {
+  tile_kernel<C, P><<<(unsigned)std::min(tiles, (int64_t)kCus * C::PER_CU), C::NT, 0, s>>>(p, (int)tiles);
+}
+// The tile shape of a product over rows of groups with n columns (kPair: half of a tile's columns).
+template <class P>
+void run_rows(const P& p, int n, hipStream_t s) {
+  constexpr int H = P::kPair ? 2 : 1;
+  const int64_t big = tiles_of(p.p, 256, n, 256 / H);
+  if (p.p.rows > 64 * (int64_t)p.p.groups) {
+    if (big >= kCus) run_tiles<Tile256>(p, big, s);
+    else run_tiles<Tile128>(p, tiles_of(p.p, 128, n, 128 / H), s);
+  } else {
+    run_tiles<Tile64>(p, tiles_of(p.p, 64, n, 128 / H), s);
+  }
+}
+
+// f(integral_constant<int, D>) for a 16-bit type
+template <class F>
+void with_type(int dtype, F&& f) {
+  if (dtype == GGEMM_BF16) f(std::integral_constant<int, GGEMM_BF16>{});
+  else f(std::integral_constant<int, GGEMM_F16>{});
+}
 
 bool rows_ok(const void* x, int64_t ld, int cols) { return x && aligned(x, 16) && ld % 8 == 0 && ld >= cols && ld <= GGEMM_GLU_MAX_LD; }
 
@@ -198,7 +411,12 @@ bool args_ok(const ggemm_glu_t* p) {
 }
 int64_t ld_hidden(const ggemm_glu_t& p) { return (int64_t)align_up((size_t)p.d_ff, 8); }
 size_t hidden_bytes(const ggemm_glu_t& p) { return align_up((size_t)p.rows * ld_hidden(p) * 2, 256); }
-int64_t row_tiles(const ggemm_glu_t& p, int tm) { return p.groups > 1 ? (int64_t)p.rows / tm + std::min(p.groups, p.rows) : ceil_div(p.rows, tm); }
+// The most tiles that a launch over rows or weights can have, in the smallest shape that it may take.
+bool tiles_fit(const ggemm_glu_t& p, bool weights) {
+  const int64_t n = std::max(p.d_ff, p.d_model);
+  const int64_t w = 3ll * p.groups * ceil_div(p.d_ff, 128) * ceil_div(p.d_model, 128);
+  return tiles_of(p, 64, (int)n, 64) < (1 << 23) && (!weights || w < (1 << 23));
+}
 
 }  // namespace
 
@@ -211,15 +429,13 @@ int glu(const ggemm_glu_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
   if (p->gate && (!aligned(p->gate, 2) || !aligned(p->up, 2) || p->ldg < p->d_ff)) return GGEMM_ERR_INVALID;
   if (ws_bytes < glu_workspace(p)) return GGEMM_ERR_WORKSPACE;
   if (!ws || !aligned(ws, 16)) return GGEMM_ERR_INVALID;
-  const int64_t up = row_tiles(*p, 64) * ceil_div(p->d_ff, 64), down = row_tiles(*p, 64) * ceil_div(p->d_model, 64);
-  if (std::max(up, down) >= (1 << 23)) return GGEMM_ERR_INVALID;
-  return launch([&] { with_elem(p->dtype, [&](auto dt) { with_act(p->act, [&](auto act) {
-    if constexpr (decltype(dt)::value != GGEMM_F32) {
-      using T = typename Elem<decltype(dt)::value>::T;
-      T* const h = static_cast<T*>(ws);
-      simple_kernel<<<(unsigned)up, 256, 0, s>>>(Up<T, decltype(act)::value>{*p, h, ld_hidden(*p)});
-      simple_kernel<<<(unsigned)down, 256, 0, s>>>(Down<T>{*p, h, ld_hidden(*p)});
-    }
+  if (!tiles_fit(*p, false)) return GGEMM_ERR_INVALID;
+  return launch([&] { with_type(p->dtype, [&](auto dt) { with_act(p->act, [&](auto act) {
+    constexpr int D = decltype(dt)::value;
+    using T = typename Elem<D>::T;
+    T* const h = static_cast<T*>(ws);
+    run_rows(Up<D, decltype(act)::value>{*p, h, ld_hidden(*p)}, p->d_ff, s);
+    run_rows(DownProduct<D>{*p, h, ld_hidden(*p)}, p->d_model, s);
   }); }); });
 }
 
@@ -241,27 +457,31 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
     return GGEMM_ERR_INVALID;
   if (ws_bytes < glu_backward_workspace(p, d)) return GGEMM_ERR_WORKSPACE;
   if (p->rows > 0 && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
-  const int64_t in = row_tiles(*p, 64) * ceil_div(p->d_ff, 64), dx = row_tiles(*p, 64) * ceil_div(p->d_model, 64);
-  const int64_t dw = (int64_t)p->groups * ceil_div(p->d_ff, 64) * ceil_div(p->d_model, 64);
-  if (std::max(std::max(in, dx), dw) >= (1 << 23)) return GGEMM_ERR_INVALID;
-  return launch([&] { with_elem(p->dtype, [&](auto dt) { with_act(p->act, [&](auto act) { with_elem(d->dw_dtype, [&](auto wt) {
-    if constexpr (decltype(dt)::value != GGEMM_F32) {
-      using T = typename Elem<decltype(dt)::value>::T;
-      using W = typename Elem<decltype(wt)::value>::T;
-      uint8_t* const b = static_cast<uint8_t*>(ws);
-      const size_t n = hidden_bytes(*p);
-      T *const dg = reinterpret_cast<T*>(b), *const du = reinterpret_cast<T*>(b + n), *const h = reinterpret_cast<T*>(b + 2 * n);
-      const int64_t ldh = ld_hidden(*p);
-      if (in) simple_kernel<<<(unsigned)in, 256, 0, s>>>(Inner<T, decltype(act)::value>{*p, *d, dg, du, h, ldh});
-      if (dx && d->dx) simple_kernel<<<(unsigned)dx, 256, 0, s>>>(Dx<T>{*p, *d, dg, du, ldh});
-      if (d->dw_gate) {
-        simple_kernel<<<(unsigned)dw, 256, 0, s>>>(Dw<T, W, false>{*p, *d, dg, static_cast<const T*>(p->x), ldh, p->ldx, static_cast<W*>(d->dw_gate)});
-        simple_kernel<<<(unsigned)dw, 256, 0, s>>>(Dw<T, W, false>{*p, *d, du, static_cast<const T*>(p->x), ldh, p->ldx, static_cast<W*>(d->dw_up)});
-      }
-      if (d->dw_down)
-        simple_kernel<<<(unsigned)dw, 256, 0, s>>>(Dw<T, W, true>{*p, *d, static_cast<const T*>(d->dy), h, d->lddy, ldh, static_cast<W*>(d->dw_down)});
+  if (!tiles_fit(*p, d->dw_gate || d->dw_down)) return GGEMM_ERR_INVALID;
+  return launch([&] { with_type(p->dtype, [&](auto dt) {
+    constexpr int D = decltype(dt)::value;
+    using T = typename Elem<D>::T;
+    uint8_t* const b = static_cast<uint8_t*>(ws);
+    const size_t n = hidden_bytes(*p);
+    T *const dg = reinterpret_cast<T*>(b), *const du = reinterpret_cast<T*>(b + n), *const h = reinterpret_cast<T*>(b + 2 * n);
+    const int64_t ldh = ld_hidden(*p);
+    if (p->rows > 0) {
+      with_act(p->act, [&](auto act) { run_rows(Hidden<D, decltype(act)::value>{*p, d->dy, d->lddy, dg, du, h, ldh}, p->d_ff, s); });
+      if (d->dx) run_rows(InputGrad<D>{*p, d->dx, d->lddx, dg, du, ldh}, p->d_model, s);
     }
-  }); }); }); });
+    if (!d->dw_gate && !d->dw_down) return;
+    const int matrices = (d->dw_gate ? 2 : 0) + (d->dw_down ? 1 : 0), from = d->dw_gate ? 0 : 2;
+    with_elem(d->dw_dtype, [&](auto wt) {
+      auto go = [&](auto indexed) {
+        const WeightGrad<D, decltype(wt)::value, decltype(indexed)::value> w{*p, *d, dg, du, h, ldh, from};
+        auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
+        if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
+        else run_tiles<Tile128>(w, tiles(128), s);
+      };
+      if (p->index && p->rows > 0) go(std::true_type{});
+      else go(std::false_type{});
+    });
+  }); });
 }
 
 }  // namespace ggemm

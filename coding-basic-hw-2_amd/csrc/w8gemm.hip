@@ -3,33 +3,73 @@
 #include <type_traits>
 
 #include "ggemm_w8.h"
-#include "simple.hpp"
+#include "act.hpp"
+#include "tiles.hpp"
 
 namespace ggemm {
 namespace {
 
-template <class T, int ACT>
+struct Place {
+  int g, m0, m_end, n0, nk;
+};
+
+// c = (s sa) sb, or act of it times the same of the second weights
+template <int D, int ACT>
 struct Product {
-  using Acc = int;
-  static constexpr int kPairs = ACT ? 2 : 1;
+  using T = typename Elem<D>::T;
+  using M = MmaI8;
+  using Place = ggemm::Place;
+  static constexpr bool kADown = false, kBDown = false, kPair = ACT != 0;
+  static constexpr int E = 8;
   ggemm_w8_gemm_t p;
-  int g, lo, hi, n0;
-  __device__ bool place(int t) {
-    if (!simple_rows(p.offsets, p.groups, p.m, ceil_div(p.n, 64), t, g, lo, hi, n0)) return false;
-    n0 *= 64;
-    return true;
+  __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.m}; }
+  template <int BM, int BN>
+  __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.n, kPair ? BN / 2 : BN)); }
+  template <class C>
+  __device__ __forceinline__ Place place(const GroupTiles<C::BM>& first, int t) const {
+    constexpr int width = kPair ? C::BN / 2 : C::BN;
+    const int nt = ceil_div(p.n, width);
+    const RowSpan s = find_group(rows(), first, t, nt);
+    if (s.g < 0) return Place{-1};
+    int tm, tn;
+    tile_raster(t, ceil_div(s.hi - s.lo, C::BM), nt, tm, tn);
+    return Place{s.g, s.lo + tm * C::BM, s.hi, tn * width, ceil_div(p.k, 128)};
   }
-  __device__ int depth() const { return p.k; }
-  __device__ int a(int i, int k) const { return lo + i < hi && k < p.k ? p.a[(lo + i) * p.lda + k] : 0; }
-  __device__ int b(int z, int j, int k) const {
-    return n0 + j < p.n && k < p.k ? (z ? p.b_up : p.b)[g * p.b_stride + (n0 + j) * p.ldb + k] : 0;
+  template <class C>
+  struct Src {
+    Along<C, C::BM> a;
+    Along<C, C::BN, kPair> b;
+    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
+      a.load(kt, slot, wave);
+      b.load(kt, slot + C::SA, wave);
+    }
+    // integers: zeros on one side are enough
+    __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
+    __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt, slot); }
+  };
+  template <class C>
+  __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
+    auto bytes = [](const int8_t* x) { return reinterpret_cast<const uint8_t*>(x); };
+    const int64_t b0 = c.g * p.b_stride + c.n0 * p.ldb;
+    return Src<C>{Along<C, C::BM>(bytes(p.a) + c.m0 * p.lda, nullptr, p.lda, c.m_end - c.m0, p.k, wave, lane, InOrder{(uint32_t)p.lda}),
+                  Along<C, C::BN, kPair>(bytes(p.b) + b0, bytes(p.b_up) + b0, p.ldb, p.n - c.n0, p.k, wave, lane, InOrder{(uint32_t)p.ldb})};
   }
-  __device__ void emit(int i, int j, const int* s) const {
-    if (lo + i >= hi || n0 + j >= p.n) return;
-    const int64_t c = g * p.b_scales_stride + n0 + j;
-    float v = (float)s[0] * p.a_scales[lo + i] * p.b_scales[c];
-    if constexpr (ACT != 0) v = act_value<ACT>(v) * ((float)s[1] * p.a_scales[lo + i] * p.b_up_scales[c]);
-    static_cast<T*>(p.c)[(lo + i) * p.ldc + n0 + j] = (T)v;
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u) const {
+    const int64_t r = c.m0 + row, j = c.n0 + col;
+    if (r >= c.m_end || j >= p.n) return;
+    const int ok = p.n - (int)j;
+    const int64_t sj = c.g * p.b_scales_stride + j;
+    const float sa = p.a_scales[r];
+    float o[E], s[E];
+    load_some(p.b_scales + sj, ok, s);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = v[e] * sa * s[e];
+    if constexpr (kPair) {
+      load_some(p.b_up_scales + sj, ok, s);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = act_value<ACT>(o[e]) * (u[e] * sa * s[e]);
+    }
+    store_some(static_cast<T*>(p.c) + r * p.ldc + j, ok, o);
   }
 };
 
@@ -52,7 +92,23 @@ bool args_ok(const ggemm_w8_gemm_t* p) {
   auto operand = [](const int8_t* x) { return x && aligned(x, 16); };
   return p->k == 0 || (operand(p->a) && operand(p->b) && (!p->act || operand(p->b_up)));
 }
-int64_t row_tiles(const ggemm_w8_gemm_t& p, int tm) { return p.groups > 1 ? (int64_t)p.m / tm + std::min(p.groups, p.m) : ceil_div(p.m, tm); }
+using Tile256 = TileShape<256, 256, 2, 4>;
+using Tile128 = TileShape<128, 128, 2, 2>;
+using Tile64 = TileShape<64, 128, 2, 2>;
+
+int64_t tiles_of(const ggemm_w8_gemm_t& p, int bm, int bn) { return row_tiles(p.groups, p.m, bm) * ceil_div(p.n, p.act ? bn / 2 : bn); }
+
+template <class C, class P>
+void run_tiles(const P& p, hipStream_t s) {
+  const int64_t tiles = tiles_of(p.p, C::BM, C::BN);
+  tile_kernel<C, P><<<(unsigned)std::min(tiles, (int64_t)kCus * C::PER_CU), C::NT, 0, s>>>(p, (int)tiles);
+}
+template <class P>
+void run(const P& p, hipStream_t s) {
+  if (p.p.m <= 64 * (int64_t)p.p.groups) run_tiles<Tile64>(p, s);
+  else if (tiles_of(p.p, 256, 256) >= kCus) run_tiles<Tile256>(p, s);
+  else run_tiles<Tile128>(p, s);
+}
 
 }  // namespace
 
@@ -64,12 +120,11 @@ int w8_gemm(const ggemm_w8_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s) 
   const size_t need = w8_gemm_workspace(p);
   if (ws_bytes < need) return GGEMM_ERR_WORKSPACE;
   if (need && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
-  const int64_t tiles = row_tiles(*p, 64) * ceil_div(p->n, 64);
-  if (tiles >= (1 << 23)) return GGEMM_ERR_INVALID;
+  if (tiles_of(*p, 64, 128) >= (1 << 23)) return GGEMM_ERR_INVALID;
   return launch([&] { with_elem(p->dtype, [&](auto d) {
-    using T = typename Elem<decltype(d)::value>::T;
-    if (!p->act) simple_kernel<<<(unsigned)tiles, 256, 0, s>>>(Product<T, 0>{*p});
-    else with_act(p->act, [&](auto act) { simple_kernel<<<(unsigned)tiles, 256, 0, s>>>(Product<T, decltype(act)::value>{*p}); });
+    constexpr int D = decltype(d)::value;
+    if (!p->act) run(Product<D, 0>{*p}, s);
+    else with_act(p->act, [&](auto act) { run(Product<D, decltype(act)::value>{*p}, s); });
   }); });
 }
 

@@ -7,49 +7,178 @@
 namespace ggemm {
 namespace {
 
-// x / s to the nearest whole number, ties to even, for |x| <= 127 s (1 + 2^-24) and a normal s; r = 1 / s to a few
-// bits.  A first guess from x r is off by at most one, and only next to a half.  The rest x - q s is exact
-// in 32 bits (a multiple of the smaller unit of x and s, at most s or so), so comparing it with s / 2 (exact) decides.
-__device__ __forceinline__ float whole_quotient(float x, float s, float r) {
-  float q = rintf(x * r);
-  const float rest = fmaf(-q, s, x), half = 0.5f * s;
-  const bool odd = fmaf(-2.0f, rintf(0.5f * q), q) != 0.0f;
-  if (rest > half || (rest == half && odd)) q += 1.0f;
-  else if (rest < -half || (rest == -half && odd)) q -= 1.0f;
-  return q;
+// Eight consecutive values of a row from column c0 on, zeros past its end.
+template <int D>
+__device__ __forceinline__ void load8(const void* x, int64_t row_at, int c0, int cols, float (&v)[8]) {
+  using T = typename Elem<D>::T;
+  const T* const p = static_cast<const T*>(x) + row_at + c0;
+  if (c0 + 8 <= cols) {
+    const Run<T, 8> w = Run<T, 8>::load(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)w.x[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c0 + e < cols ? (float)p[e] : 0.0f;
+  }
+}
+__device__ __forceinline__ uint32_t largest(const float (&v)[8], uint32_t m) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);   // NaN above Inf above all else
+  return m;
 }
 
+// x / s to the nearest whole number, ties to even, in the low byte: s = max(fl(a / 127), 2^-126), |x| <= a, r from
+// row_factor.  Adding 1.5 2^23 to x r in one multiply-add rounds once, to a whole number.
+// r = fl(1 / s), so x r is off x / s by 2 parts in 2^24 at most and the number by one at most, next to a half.
+// The rest x - q s is exact (a multiple of the smaller unit of x and s, about s at most), and comparing it with s / 2,
+// exact too, decides.
+// bf16 needs no such step.  With x and a of 8 bits, |254 x - (2 n + 1) a| is either a unit of x or more, i.e.
+// 127 x / a lies a part of 7 10^-6 or more beside the half, where the roundings of s and r come to 2.4 10^-7; or 0:
+// then a is 127 or 254 times a power of two, s and r are powers of two and all is exact, or x = a / 2, n = 63, and for
+// that value row_factor has moved r to the side where it belongs.
+constexpr float kWhole = 12582912.0f;
 template <int D>
-__global__ void __launch_bounds__(256) quant_kernel(ggemm_w8_quant_t p) {
-  using T = typename Elem<D>::T;
-  __shared__ uint32_t top[4];
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    int64_t src = row;
-    if (p.index) {
-      src = p.index[row];
-      if (src < 0 || src >= p.x_rows) src = -1;
-    }
-    const T* const x = static_cast<const T*>(p.x) + src * p.ld;
-    uint32_t m = 0;
-    for (int j = threadIdx.x; src >= 0 && j < p.cols; j += 256) m = max(m, __float_as_uint((float)x[j]) & 0x7fffffffu);
-    for (int d = 1; d < 64; d *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) top[threadIdx.x / 64] = m;
-    __syncthreads();
-    m = max(max(top[0], top[1]), max(top[2], top[3]));
-    const bool bad = m >= 0x7f800000u;
-    const float s = fmaxf(__uint_as_float(m) / 127.0f, 0x1p-126f), r = 1.0f / s;
-    for (int j = threadIdx.x; j < p.cols; j += 256)
-      p.q[row * p.ldq + j] = (int8_t)(bad || src < 0 ? 0.0f : whole_quotient((float)x[j], s, r));
-    if (threadIdx.x == 0) p.scales[row] = bad ? __uint_as_float(0x7fc00000u) : s;
+__device__ __forceinline__ float row_factor(float a, float s) {
+  float r = 1.0f / s;
+  if constexpr (D == GGEMM_BF16) {
+    const float h = 0.5f * a;
+    const bool up = fmaf(-63.5f, s, h) >= 0.0f;   // x / s of 63.5 or more: 64
+    // s is a power of two at its least, and r exact
+    if (s > 0x1p-126f && fmaf(h, r, kWhole) - kWhole != (up ? 64.0f : 63.0f)) r = __uint_as_float(__float_as_uint(r) + (up ? 1u : ~0u));
+  }
+  return r;
+}
+template <int D>
+__device__ __forceinline__ uint32_t whole_quotient(float x, float s, float r) {
+  const float big = fmaf(x, r, kWhole);
+  if constexpr (D == GGEMM_BF16) return __float_as_uint(big);
+  const float q = big - kWhole, rest = fmaf(-q, s, x), half = 0.5f * s;
+  const uint32_t w = __float_as_uint(big), odd = w & 1u;
+  if (rest > half || (rest == half && odd)) return w + 1u;
+  if (rest < -half || (rest == -half && odd)) return w - 1u;
+  return w;
+}
+template <int D>
+__device__ __forceinline__ u32x2 quotients(const float (&v)[8], float s, float r) {
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = whole_quotient<D>(v[e], s, r);
+  u32x2 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)   // the low bytes of four words
+    o[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[4 * h + 3], w[4 * h + 2], 0x0c0c0400u),
+                                 __builtin_amdgcn_perm(w[4 * h + 1], w[4 * h], 0x0c0c0400u), 0x05040100u);
+  return o;
+}
+template <bool kStream>
+__device__ __forceinline__ void store8(int8_t* p, u32x2 w, int ok) {
+  typedef u32x2 at_any __attribute__((aligned(1)));
+  if (ok >= 8) {
+    if constexpr (kStream) __builtin_nontemporal_store(w, reinterpret_cast<at_any*>(p));
+    else *reinterpret_cast<at_any*>(p) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < ok) p[e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
   }
 }
 
+// L lanes share a row (L < 64: part of a wave, else a whole workgroup), N chunks of 8 values a lane in registers; the chunks of a
+// longer row past those are read a second time, out of the caches.
+template <int D, int L, int N>
+__global__ void __launch_bounds__(256) quant_kernel(ggemm_w8_quant_t p) {
+  constexpr int R = 256 / L;   // rows at a time
+  __shared__ uint32_t top[4];
+  const int lane = threadIdx.x % L, chunks = ceil_div(p.cols, 8);
+  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < p.rows; row0 += (int64_t)gridDim.x * R) {
+    const int64_t row = row0 + threadIdx.x / L;
+    int64_t src = row < p.rows ? row : -1;
+    if (p.index && src >= 0) {
+      const int i = p.index[row];
+      src = (uint32_t)i < (uint32_t)p.x_rows ? i : -1;
+    }
+    const int have = src >= 0 ? chunks : 0;
+    const int64_t at = src * p.ld;
+    float v[N][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = 0.0f;
+      if (lane + c * L < have) load8<D>(p.x, at, 8 * (lane + c * L), p.cols, v[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) m = largest(v[c], m);
+    for (int c = lane + N * L; c < have; c += L) {
+      float w[8];
+      load8<D>(p.x, at, 8 * c, p.cols, w);
+      m = largest(w, m);
+    }
+#pragma unroll
+    for (int d = 1; d < (L < 64 ? L : 64); d *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+    if constexpr (L > 64) {
+      __syncthreads();
+      if (threadIdx.x % 64 == 0) top[threadIdx.x / 64] = m;
+      __syncthreads();
+      m = max(max(top[0], top[1]), max(top[2], top[3]));
+    }
+    const bool bad = m >= 0x7f800000u;
+    const float a = __uint_as_float(m), s = fmaxf(a / 127.0f, 0x1p-126f), r = bad ? 0.0f : row_factor<D>(a, s);
+    if (row >= p.rows) continue;
+    int8_t* const out = p.q + row * p.ldq;
+    auto put = [&](int c, const float (&x)[8]) {
+      u32x2 w = quotients<D>(x, s, r);
+      if (bad) w = u32x2{0, 0};
+      store8<false>(out + 8 * c, w, p.cols - 8 * c);
+    };
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (lane + c * L < chunks) put(lane + c * L, v[c]);
+    for (int c = lane + N * L; c < chunks; c += L) {
+      float w[8] = {};
+      if (c < have) load8<D>(p.x, at, 8 * c, p.cols, w);
+      put(c, w);
+    }
+    if (lane == 0) p.scales[row] = bad ? __uint_as_float(0x7fc00000u) : s;
+  }
+}
+
+// Back to values: 256 lanes cover cx chunks of 8 columns (a power of two) of 256 / cx rows.
 template <int D>
-__global__ void __launch_bounds__(256) dequant_kernel(ggemm_w8_dequant_t p) {
+__device__ __forceinline__ void dequant_chunk(const ggemm_w8_dequant_t& p, int64_t row, int c0) {
   using T = typename Elem<D>::T;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x)
-    for (int j = threadIdx.x; j < p.cols; j += 256) static_cast<T*>(p.y)[row * p.ld + j] = (T)((float)p.q[row * p.ldq + j] * p.scales[row]);
+  const int8_t* const q = p.q + row * p.ldq + c0;
+  T* const y = static_cast<T*>(p.y) + row * p.ld + c0;
+  const float s = p.scales[row];
+  Run<T, 8> o;
+  auto value = [&](int b) {
+    float v = (float)b * s;
+    asm("" : "+v"(v));   // a 32-bit product, then the type's rounding: not one instruction that rounds once
+    return (T)v;
+  };
+  if (c0 + 8 <= p.cols) {
+    typedef u32x2 at_any __attribute__((aligned(1)));
+    const u32x2 w = *reinterpret_cast<const at_any*>(q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.x[e] = value((int8_t)(w[e / 4] >> (8 * (e % 4))));
+    o.template store<false>(y);
+  } else {
+    for (int e = 0; c0 + e < p.cols; ++e) y[e] = value(q[e]);
+  }
+}
+template <int D>
+__global__ void __launch_bounds__(256) dequant_kernel(ggemm_w8_dequant_t p, int log_cx) {
+  const int c0 = 8 * ((blockIdx.y << log_cx) + (threadIdx.x & ((1 << log_cx) - 1)));
+  if (c0 >= p.cols) return;
+  const int64_t step = (int64_t)gridDim.x << (8 - log_cx);
+  for (int64_t row = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx); row < p.rows; row += step) dequant_chunk<D>(p, row, c0);
+}
+
+constexpr int64_t kMostGroups = 1 << 16;   // workgroups of a launch, more rows a workgroup past that
+
+template <int D, int L, int N>
+void run_quant(const ggemm_w8_quant_t& p, hipStream_t s) {
+  quant_kernel<D, L, N><<<(unsigned)std::min(kMostGroups, ((int64_t)p.rows + 256 / L - 1) / (256 / L)), 256, 0, s>>>(p);
 }
 
 }  // namespace
@@ -63,7 +192,10 @@ int w8_quantize(const ggemm_w8_quant_t* p, hipStream_t s) {
   if (p->cols > 0 && ((!p->x && !(p->index && p->x_rows == 0)) || !aligned(p->x, elem_bytes(p->dtype)) || p->ld < p->cols || !p->q || p->ldq < p->cols))
     return GGEMM_ERR_INVALID;
   return launch([&] { with_elem(p->dtype, [&](auto d) {
-    quant_kernel<decltype(d)::value><<<(unsigned)std::min(p->rows, 1 << 20), 256, 0, s>>>(*p);
+    constexpr int D = decltype(d)::value;
+    if (p->cols <= 256) run_quant<D, 8, 4>(*p, s);
+    else if (p->cols <= 2048) run_quant<D, 64, 4>(*p, s);
+    else run_quant<D, 256, 4>(*p, s);
   }); });
 }
 
@@ -73,7 +205,11 @@ int w8_dequantize(const ggemm_w8_dequant_t* p, hipStream_t s) {
   if (!p->q || p->ldq < p->cols || !p->scales || !aligned(p->scales, 4) || !p->y || !aligned(p->y, elem_bytes(p->dtype)) || p->ld < p->cols)
     return GGEMM_ERR_INVALID;
   return launch([&] { with_elem(p->dtype, [&](auto d) {
-    dequant_kernel<decltype(d)::value><<<(unsigned)std::min(p->rows, 1 << 20), 256, 0, s>>>(*p);
+    const int chunks = ceil_div(p->cols, 8);
+    int log_cx = 0;
+    while (log_cx < 8 && (1 << log_cx) < chunks) ++log_cx;
+    const int64_t rows = ((int64_t)p->rows + (256 >> log_cx) - 1) >> (8 - log_cx);
+    dequant_kernel<decltype(d)::value><<<dim3((unsigned)std::min(kMostGroups, rows), ceil_div(chunks, 1 << log_cx)), 256, 0, s>>>(*p, log_cx);
   }); });
 }
 

@@ -1,6 +1,7 @@
 // glu.hip -- the gated feed-forward block and its gradients (include/ggemm_glu.h).
 #include <algorithm>
 #include <type_traits>
+#include <cstdlib>
 
 #include "act.hpp"
 #include "tiles.hpp"
@@ -55,12 +56,15 @@ struct Up {
   }
   template <class C>
   struct Src {
+    static constexpr int kTouches = 0;
     Along<C, C::BM> a;
     Along<C, C::BN, true> b;
-    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
-      a.load(kt, slot, wave);
-      b.load(kt, slot + C::SA, wave);
+    __device__ __forceinline__ void prepare(int kt, int wave) {
+      a.prepare(kt, wave);
+      b.prepare(kt, wave);
     }
+    __device__ __forceinline__ void sent(int, int) const {}
+    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
       a.clear(kt, slot);
@@ -81,7 +85,8 @@ struct Up {
     return Src<C>{Along<C, C::BM>(x, nullptr, px, p.index ? p.x_rows : c.m_end - c.m0, bytes, wave, lane, at),
                   Along<C, C::BN, true>(bytes_of(p.w_gate) + w0, bytes_of(p.w_up) + w0, pw, n, bytes, wave, lane, InOrder{(uint32_t)pw})};
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u) const {
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u, Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_ff) return;
     const int ok = p.d_ff - (int)j;
@@ -116,12 +121,15 @@ struct DownProduct {
   }
   template <class C>
   struct Src {
+    static constexpr int kTouches = 0;
     Along<C, C::BM> a;
     Along<C, C::BN> b;
-    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
-      a.load(kt, slot, wave);
-      b.load(kt, slot + C::SA, wave);
+    __device__ __forceinline__ void prepare(int kt, int wave) {
+      a.prepare(kt, wave);
+      b.prepare(kt, wave);
     }
+    __device__ __forceinline__ void sent(int, int) const {}
+    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
       a.clear(kt, slot);
@@ -136,7 +144,8 @@ struct DownProduct {
                   Along<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0 * p.ldd), nullptr, pw, p.d_model - c.n0, bytes, wave,
                                   lane, InOrder{(uint32_t)pw})};
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_model) return;
     float o[E];
@@ -168,11 +177,24 @@ struct Hidden {
   }
   template <class C>
   struct Src {
+    // The tile's lines of gate and up, BM rows of BN 16-bit values each, 64 lines a wave at a time.  Without, the epilogue waits for
+    // HBM: 16 groups of 2048 rows, (2048, 4096), 922 us; with gate and up left out 632.
+    static constexpr int ROW_LINES = C::BN / 64, kTouches = 2 * C::BM * ROW_LINES / 64 / C::NW;
     Along<C, C::BM> a;
     Down<C, C::BN> b;
-    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
-      a.load(kt, slot, wave);
-      b.load(b.base, kt, slot + C::SA, wave);
+    const uint8_t *gate, *up;   // of the tile's first row and column
+    int64_t pitch;
+    int rows, bytes;            // that exist of the tile: rows, bytes of a row
+    __device__ __forceinline__ void prepare(int kt, int wave) {
+      a.prepare(kt, wave);
+      b.prepare(b.base, kt);
+    }
+    __device__ __forceinline__ void sent(int, int) const {}
+    __device__ __forceinline__ void arrived() const {}
+    __device__ __forceinline__ void touch(int part, uint32_t scrap, int wave, int lane) const {
+      const int l = 64 * (part * C::NW + wave) + lane, r = l / ROW_LINES % C::BM, c = 128 * (l % ROW_LINES);
+      const uint8_t* const p = (l / ROW_LINES / C::BM ? up : gate) + min(r, rows - 1) * pitch + min(c, bytes - 2);
+      touch_lines(reinterpret_cast<const void*>((uintptr_t)p & ~(uintptr_t)3), scrap);
     }
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt, slot); }
@@ -181,18 +203,33 @@ struct Hidden {
   __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
     const int64_t py = 2 * lddy;
     return Src<C>{Along<C, C::BM>(bytes_of(dy) + c.m0 * py, nullptr, py, c.m_end - c.m0, 2 * p.d_model, wave, lane, InOrder{(uint32_t)py}),
-                  Down<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0), 2 * p.ldd, p.d_model, p.d_ff - c.n0, wave, lane)};
+                  Down<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0), 2 * p.ldd, p.d_model, p.d_ff - c.n0, wave, lane),
+                  bytes_of(p.gate) + 2 * (c.m0 * p.ldg + c.n0), bytes_of(p.up) + 2 * (c.m0 * p.ldg + c.n0), 2 * p.ldg, c.m_end - c.m0,
+                  2 * (p.d_ff - c.n0)};
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+  struct Kept {
+    Run<T, E> g, u;
+    bool live;
+  };
+  __device__ __forceinline__ Kept fetch(const Place& c, int row, int col) const {
+    Kept k{};
+    const int64_t r = c.m0 + row, j = c.n0 + col;
+    if (r >= c.m_end || j >= p.d_ff) return k;
+    const int ok = p.d_ff - (int)j;
+    k.live = Picked{p.index, p.x_rows}.live((int)r);
+    k.g = run_some<T, E>(static_cast<const T*>(p.gate) + r * p.ldg + j, ok);
+    k.u = run_some<T, E>(static_cast<const T*>(p.up) + r * p.ldg + j, ok);
+    return k;
+  }
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, const Kept& k) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_ff) return;
     const int ok = p.d_ff - (int)j;
-    const bool live = Picked{p.index, p.x_rows}.live((int)r);
+    const bool live = k.live;
     float g[E], u[E], o[E];
-    load_some(static_cast<const T*>(p.gate) + r * p.ldg + j, ok, g);
-    load_some(static_cast<const T*>(p.up) + r * p.ldg + j, ok, u);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+      g[e] = (float)k.g.x[e], u[e] = (float)k.u.x[e];
       float q, dq;
       act_parts<ACT>(g[e], q, dq);
       const float a = g[e] * q, w = u[e];
@@ -228,15 +265,18 @@ struct InputGrad {
   }
   template <class C>
   struct Src {
+    static constexpr int kTouches = 0;
     Along<C, C::BM> a;   // base2: dup
     Down<C, C::BN> b;
     const uint8_t* b2;
     int half;            // stages of each
-    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
+    __device__ __forceinline__ void prepare(int kt, int wave) {
       const bool second = kt >= half;
-      a.load(second ? a.base2 : a.base, nullptr, second ? kt - half : kt, slot, wave);
-      b.load(second ? b2 : b.base, second ? kt - half : kt, slot + C::SA, wave);
+      a.prepare(second ? a.base2 : a.base, nullptr, second ? kt - half : kt, wave);
+      b.prepare(second ? b2 : b.base, second ? kt - half : kt);
     }
+    __device__ __forceinline__ void sent(int, int) const {}
+    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt >= half ? kt - half : kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt >= half ? kt - half : kt, slot); }
   };
@@ -248,7 +288,8 @@ struct InputGrad {
                   Down<C, C::BN>(bytes_of(p.w_gate) + w0, 2 * p.ldw, p.d_ff, p.d_model - c.n0, wave, lane), bytes_of(p.w_up) + w0,
                   ceil_div(p.d_ff, 64)};
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_model) return;
     float o[E];
@@ -298,31 +339,52 @@ struct WeightGrad {
   }
   template <class C>
   struct Src {
+    static constexpr int kTouches = 0;
     Down<C, C::BM> a;
     Down<C, C::BN> b;
-    Picked pick;        // of the group's first row on
-    int depth;
-    bool gather;
-    int64_t all;
-    int row[kIndexed ? Down<C, C::BM>::P : 1];
-    // index entries of stage kt's steps
-    __device__ __forceinline__ void fetch(int kt, int wave, int lane) {
+    const int32_t* index;   // of the group's first row on
+    int x_rows, depth;
+    uint32_t pitch;         // of gathered rows; 0 where the operand's rows are the group's in order
+    // Index entries of this lane's steps.  They are loaded two stages before the loads that go by them and taken over
+    // (arrived) right after a wait for everything in flight: looked at any later or earlier, the compiler's wait for them
+    // would also wait for operands on their way (16 groups of 2048 rows, (2048, 4096): 1930 us, without an index 1607).
+    static constexpr int P = Down<C, C::BM>::P;
+    struct Entries {
+      int at[kIndexed ? P : 1];
+    } row, second, third, coming;   // of the next stage to prepare; of the tile's second and third; in flight
+    __device__ __forceinline__ Entries entries(int kt, int wave, int lane) const {
+      Entries r{};
       if constexpr (kIndexed) {
 #pragma unroll
-        for (int q = 0; q < Down<C, C::BM>::P; ++q) {
-          const int k = 64 * kt + Down<C, C::BM>::step(q, wave, lane);
-          row[q] = k < depth ? pick.at(k) : -1;
+        for (int q = 0; q < P; ++q) r.at[q] = index[(uint32_t)min(64 * kt + Down<C, C::BM>::step(q, wave, lane), depth - 1)];
+      }
+      return r;
+    }
+    __device__ __forceinline__ void prepare(int kt, int wave) {
+      a.prepare(a.base, kt);
+      b.prepare(b.base, kt);
+      if constexpr (kIndexed) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const bool live = (uint32_t)row.at[q] < (uint32_t)x_rows && Down<C, C::BM>::step(q, wave, lane) < depth - 64 * kt;
+          a.o[q] = live ? a.v[q] : kOut;
+          b.o[q] = live ? (uint32_t)row.at[q] * pitch + b.v[q] : kOut;
         }
       }
     }
-    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) {
+    __device__ __forceinline__ void arrived() {
       if constexpr (kIndexed) {
-        a.load(a.base, kt, slot, wave, row, false, 0);
-        b.load(b.base, kt, slot + C::SA, wave, row, gather, all);
-        fetch(kt + 1, wave, threadIdx.x & 63);   // a stage ahead
-      } else {
-        a.load(a.base, kt, slot, wave);
-        b.load(b.base, kt, slot + C::SA, wave);
+#pragma unroll
+        for (int q = 0; q < P; ++q) asm volatile("" : "+v"(coming.at[q]));
+        row = coming;
+      }
+    }
+    __device__ __forceinline__ void sent(int kt, int wave) {
+      if constexpr (kIndexed) {
+        if (kt == 0) row = second;
+        else if (kt == 1) row = third;
+        else coming = entries(kt + 2, wave, threadIdx.x & 63);
       }
     }
     __device__ __forceinline__ bool ragged(int) const { return false; }
@@ -336,12 +398,23 @@ struct WeightGrad {
     const uint8_t* const b = bytes_of(down ? (const void*)h : p.x) + (gather ? 0 : c.lo * pb) + 2 * c.n0;
     const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model;
     Src<C> s{Down<C, C::BM>(a, pa, c.depth, m - c.m0, wave, lane), Down<C, C::BN>(b, pb, c.depth, n - c.n0, wave, lane),
-             Picked{kIndexed ? p.index + c.lo : nullptr, p.x_rows}, c.depth, gather,
-             (p.x_rows - 1) * pb + ((2 * (n - c.n0) + 15) & ~15)};
-    s.fetch(0, wave, lane);
+             p.index + c.lo, p.x_rows, c.depth, gather ? (uint32_t)pb : 0u};
+    if (gather) {   // any row in any stage
+      s.b.stage = 0;
+      s.b.left = (p.x_rows - 1) * pb + ((2 * (n - c.n0) + 15) & ~15);
+#pragma unroll
+      for (int q = 0; q < Src<C>::P; ++q) s.b.v[q] = s.b.col;
+    }
+    if (kIndexed && c.depth > 0) {
+      s.row = s.entries(0, wave, lane);
+      s.second = s.entries(1, wave, lane);
+      s.third = s.entries(2, wave, lane);
+      s.coming = s.entries(3, wave, lane);
+    }
     return s;
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*) const {
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, Nothing) const {
     const bool down = c.which == 2;
     const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model, i = c.m0 + row, j = c.n0 + col;
     if (i >= m || j >= n) return;
@@ -376,6 +449,14 @@ template <class P>
 void run_rows(const P& p, int n, hipStream_t s) {
   constexpr int H = P::kPair ? 2 : 1;
   const int64_t big = tiles_of(p.p, 256, n, 256 / H);
+  static const char* ev = getenv("GLU_TILE");   // EXPERIMENT
+  if (ev) {
+    const int t = atoi(ev);
+    if (t == 256) run_tiles<Tile256>(p, big, s);
+    else if (t == 128) run_tiles<Tile128>(p, tiles_of(p.p, 128, n, 128 / H), s);
+    else run_tiles<Tile64>(p, tiles_of(p.p, 64, n, 128 / H), s);
+    return;
+  }
   if (p.p.rows > 64 * (int64_t)p.p.groups) {
     if (big >= kCus) run_tiles<Tile256>(p, big, s);
     else run_tiles<Tile128>(p, tiles_of(p.p, 128, n, 128 / H), s);
@@ -475,7 +556,8 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
       auto go = [&](auto indexed) {
         const WeightGrad<D, decltype(wt)::value, decltype(indexed)::value> w{*p, *d, dg, du, h, ldh, from};
         auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
-        if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
+        static const char* ev = getenv("GLU_TILE");
+        if (ev ? atoi(ev) == 256 : tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
         else run_tiles<Tile128>(w, tiles(128), s);
       };
       if (p->index && p->rows > 0) go(std::true_type{});

@@ -128,8 +128,10 @@ struct TileShape {
   static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, NW = WGM * WGN, NT = 64 * NW;
   static constexpr int FM = BM / WGM / 32, FN = BN / WGN / 32;
   static constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;
+  static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;   // 1 KB pieces of A and B a wave brings
   static constexpr int EPI = 32 * 32 * FN * 4;               // epilogue bytes per wave, from the second slot on
-  static constexpr int SMEM = STAGE + (NW * EPI > STAGE ? NW * EPI : STAGE);
+  static constexpr int SCRAP = STAGE + (NW * EPI > STAGE ? NW * EPI : STAGE);   // where touched bytes go, 256 a wave
+  static constexpr int SMEM = SCRAP + 256 * NW;
   static constexpr int PER_CU = 163840 / SMEM;               // workgroups, as many as LDS holds
   static constexpr int WAVES = PER_CU * NW / 4;              // per SIMD
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && NW % 2 == 0, "pieces");
@@ -142,9 +144,11 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 // assembly so that the compiler does not wait for all of them before the next LDS read; the waits are stage_done's.
 struct Window {
   i32x4 r;
+  Window() = default;
   __device__ __forceinline__ Window(const uint8_t* base, int64_t left) {
     const uint64_t b = (uint64_t)base;
-    const uint32_t n = (uint32_t)(left < 0 ? 0 : left > kWindow ? kWindow : left);
+    const int high = (int)(left >> 32);   // compared by halves: scalar instructions
+    const uint32_t low = (uint32_t)left, n = high < 0 ? 0u : high > 0 || low > (uint32_t)kWindow ? (uint32_t)kWindow : low;
     r = i32x4{__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff),
               __builtin_amdgcn_readfirstlane((int)n), 0x00020000};
   }
@@ -155,6 +159,12 @@ struct Window {
                      __builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(r) : "memory");
   }
 };
+// 64 lanes' 4 bytes each, only to have their lines in the caches when they are wanted: they land in LDS unread, so that
+// no register waits for them.
+__device__ __forceinline__ void touch_lines(const void* p, uint32_t scrap) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane((int)scrap)), "v"(p)
+               : "memory");
+}
 // This wave's transfers to LDS landed.
 __device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // This wave's LDS operations done; then every wave's.
@@ -169,8 +179,9 @@ struct Along {
   static constexpr int P = ROWS / 8 / C::NW;   // 1 KB pieces (8 rows) of a wave
   const uint8_t *base, *base2;
   int64_t left;
-  uint32_t v[P];
-  int chunk, bytes;   // this lane's chunk of a row; bytes of a row
+  uint32_t v[P], o[P];   // offsets of the pieces in a stage; those of the prepared one
+  Window w, w2;
+  int chunk, bytes;      // this lane's chunk of a row; bytes of a row
   // rows of the matrix from base (and base2) on, `pitch` and `bytes` bytes each; at(row): a row's offset, or kOut
   template <class At>
   __device__ __forceinline__ Along(const uint8_t* base_, const uint8_t* base2_, int64_t pitch, int64_t rows, int bytes_, int wave,
@@ -183,16 +194,25 @@ struct Along {
       v[q] = at((kPair ? 32 * (p >> 3) + 8 * (p & 3) : 8 * p) + (lane >> 3)) + 16 * chunk;
     }
   }
-  __device__ __forceinline__ void load(const uint8_t* from, const uint8_t* from2, int kt, uint32_t slot, int wave) const {
+  // What stage kt's loads need; from, from2: the bases.
+  __device__ __forceinline__ void prepare(const uint8_t* from, const uint8_t* from2, int kt, int wave) {
     const uint32_t out = 128 * kt + 16 * chunk >= bytes ? kOut : 0u;   // v < kOut, or it is out already
 #pragma unroll
-    for (int q = 0; q < P; ++q) {
-      const int p = wave + C::NW * q;
-      const Window w((kPair && (p >> 2 & 1) ? from2 : from) + 128 * (int64_t)kt, left - 128 * (int64_t)kt);
-      w.send(v[q] | out, slot + 1024 * p);
+    for (int q = 0; q < P; ++q) o[q] = v[q] | out;
+    const int64_t at = 128 * (int64_t)kt;
+    if constexpr (kPair && C::NW == 4) {   // piece p = wave + 4 q: its matrix is q's lowest bit
+      w = Window(from + at, left - at);
+      w2 = Window(from2 + at, left - at);
+    } else {                               // p = wave + 8 q: the wave's bit 2
+      w = Window((kPair && (wave >> 2 & 1) ? from2 : from) + at, left - at);
     }
   }
-  __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const { load(base, base2, kt, slot, wave); }
+  __device__ __forceinline__ void prepare(int kt, int wave) { prepare(base, base2, kt, wave); }
+  // Sends piece q of the prepared stage.
+  __device__ __forceinline__ void send(int q, uint32_t slot, int wave) const {
+    static_assert(!kPair || C::NW == 4 || C::NW == 8, "pieces of a pair");
+    (kPair && C::NW == 4 && (q & 1) ? w2 : w).send(o[q], slot + 1024 * (wave + C::NW * q));
+  }
   // Whether stage kt ends inside a chunk, and that chunk's rest to zeros.
   __device__ __forceinline__ bool ragged(int kt) const { return bytes % 16 != 0 && bytes - 128 * kt <= 128; }
   __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
@@ -215,35 +235,29 @@ struct Down {
   static constexpr int P = COLS / 8 / C::NW, LANES = COLS / 8, STEPS = 64 / LANES;   // lanes of a row, rows of a piece
   static constexpr int UNITS = COLS / 32;   // of 64 bytes in a row
   const uint8_t* base;
-  int64_t pitch, left;
-  uint32_t v[P], col;
+  int64_t stage, left;     // bytes of a stage's rows; bytes from base on
+  uint32_t v[P], o[P], col;
+  Window w;
   static __device__ __forceinline__ int turn(int k) { return ((k & 3) | (k >> 1 & 4)) & (UNITS - 1); }
   // step of the stage that piece q brings this lane
   static __device__ __forceinline__ int step(int q, int wave, int lane) { return (wave + C::NW * q) * STEPS + lane / LANES; }
   __device__ __forceinline__ Down(const uint8_t* base_, int64_t pitch_, int64_t depth, int cols, int wave, int lane)
-      : base(base_), pitch(pitch_), left((depth - 1) * pitch_ + ((2 * cols + 15) & ~15)) {
+      : base(base_), stage(64 * pitch_), left((depth - 1) * pitch_ + ((2 * cols + 15) & ~15)) {
     const int pos = lane % LANES;
     // a wave's pieces lie 16 steps (or a multiple) apart, which f does not see
     static_assert(C::NW * STEPS % 16 == 0, "pieces");
     col = 16 * ((((pos >> 2) ^ turn(step(0, wave, lane))) << 2) | (pos & 3));
 #pragma unroll
-    for (int q = 0; q < P; ++q) v[q] = (uint32_t)step(q, wave, lane) * (uint32_t)pitch + col;
+    for (int q = 0; q < P; ++q) v[q] = (uint32_t)step(q, wave, lane) * (uint32_t)pitch_ + col;
   }
-  __device__ __forceinline__ void load(const uint8_t* from, int kt, uint32_t slot, int wave) const {
-    const Window w(from + 64 * kt * pitch, left - 64 * kt * pitch);
+  // What stage kt's loads need; from: the base.
+  __device__ __forceinline__ void prepare(const uint8_t* from, int kt) {
+    w = Window(from + kt * stage, left - kt * stage);
 #pragma unroll
-    for (int q = 0; q < P; ++q) w.send(v[q], slot + 1024 * (wave + C::NW * q));
+    for (int q = 0; q < P; ++q) o[q] = v[q];
   }
-  // with the rows that an index picks: row[q] is that of piece q's step, or -1; kept in place (their order is the
-  // index's), or gathered from `from`, which has `all` bytes
-  __device__ __forceinline__ void load(const uint8_t* from, int kt, uint32_t slot, int wave, const int (&row)[P], bool gather, int64_t all) const {
-    const Window w(gather ? from : from + 64 * kt * pitch, gather ? all : left - 64 * kt * pitch);
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-      const uint32_t at = gather ? (uint32_t)row[q] * (uint32_t)pitch + col : v[q];
-      w.send(row[q] < 0 ? kOut : at, slot + 1024 * (wave + C::NW * q));
-    }
-  }
+  // Sends piece q of the prepared stage.
+  __device__ __forceinline__ void send(int q, uint32_t slot, int wave) const { w.send(o[q], slot + 1024 * (wave + C::NW * q)); }
 };
 
 // Fragments of one operand: `blk0` the wave's first 32-row block of the tile.
@@ -285,9 +299,24 @@ struct Frags {
   }
 };
 
+// Stage kt of both operands.  src.prepare(kt, wave) works out what its loads need, src.a and src.b send it.
+template <class C, class S>
+__device__ __forceinline__ void send_stage(S& src, int kt, uint32_t slot, int wave) {
+  src.prepare(kt, wave);
+#pragma unroll
+  for (int q = 0; q < C::PA; ++q) src.a.send(q, slot, wave);
+#pragma unroll
+  for (int q = 0; q < C::PB; ++q) src.b.send(q, slot + C::SA, wave);
+  src.sent(kt, wave);
+}
+
 // The wave's FM x FN blocks, as C's transpose: lane l holds of block (i, j) row 32 i + l % 32 and columns
-// 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.  src.load(kt, slot) sends for a stage, src.ragged(kt) and clear(kt, slot) as Along's.
-// The first stage has landed (every wave's part).
+// 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.  src.ragged(kt) and clear(kt, slot) as Along's.  The first stage has landed (every
+// wave's part).
+// Between the barrier and the next products nothing but sends is left to do, one after each product: the scalar
+// work of a stage's loads comes before the barrier, under the products of the first half.  (All of it after the barrier, ahead
+// of the products: gradients of weights with an index, 16 groups of 2048 rows, (2048, 4096), 1930 us, as against 1607
+// without.)
 template <class C, class M, bool kADown, bool kBDown, class S>
 __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, typename M::Acc (&acc)[C::FM][C::FN]) {
   constexpr int FM = C::FM, FN = C::FN;
@@ -318,24 +347,47 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
     src.clear(0, lds);
     lds_done();
   }
-  if (nk > 1) src.load(1, ring + C::STAGE, wave);
+  if (nk > 1) send_stage<C>(src, 1, ring + C::STAGE, wave);
   read(0, 0, 0);
   int so = 0;
   for (int kt = 0; kt < nk; ++kt) {
+    const bool more = kt + 2 < nk;
     read(1, 1, so);
     products(0);
     read(0, 2, so);
+    src.prepare(kt + 2, wave);   // past the last stage too (a branch would keep it from mixing with the products)
     products(1);
     read(1, 3, so);
     const int sn = C::STAGE - so;
     pin();
     stage_done();
+    __builtin_amdgcn_sched_barrier(0);   // the compiler takes nothing of this, and no wait of its own for it, above the barrier
+    src.arrived();
     if (kt + 1 < nk && src.ragged(kt + 1)) {
       src.clear(kt + 1, lds + sn);
       lds_done();
     }
-    if (kt + 2 < nk) src.load(kt + 2, ring + so, wave);
-    products(0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        acc[i][j] = M::mma(b[0][j], a[0][i], acc[i][j]);
+        asm volatile("" : "+v"(acc[i][j]));
+        constexpr int all = C::PA + C::PB;
+        const int n = i * FN + j;
+        if (more) {
+#pragma unroll
+          for (int q = n * all / (FM * FN); q < (n + 1) * all / (FM * FN); ++q) {
+            if (q < C::PA) src.a.send(q, ring + so, wave);
+            else src.b.send(q - C::PA, ring + so + C::SA, wave);
+          }
+        }
+      }
+    if (more) src.sent(kt + 2, wave);
+    if constexpr (S::kTouches > 0) {   // in the last stages but one, for the epilogue
+      const int part = nk - 2 - kt;
+      if (part >= 0 && part < S::kTouches) src.touch(part, ring + C::SCRAP + 256 * wave, wave, lane);
+    }
     read(0, 0, sn);   // after the last stage: what an earlier one left, not used
     products(1);
     pin();
@@ -345,20 +397,24 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
 
 // Blocks to an epilogue: a wave turns one row of blocks at a time through its own part of the ring's second slot (32-bit;
 // the 16-byte piece q of row r lies at q ^ r % (pieces of a row), which spreads both the writes and the reads over the
-// banks), then emit(row, col, v, u) gets E neighbouring columns of a row of the tile.  kPair: blocks alternate between two
-// products of the same columns, v and u, and col counts one of them; else u is v.
+// banks), then emit(row, col, v, u, pre) gets E neighbouring columns of a row of the tile.  kPair: blocks alternate between two
+// products of the same columns, v and u, and col counts one of them; else u is v.  pre is what fetch(row, col) gave: the
+// loads of a row of blocks go together.
 // Before the first emit the wave waits for the transfers in flight, the next tile's first stage.
-template <class C, int E, bool kPair, class Acc, class Emit>
-__device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][C::FN], Emit emit) {
+template <class C, int E, bool kPair, class Acc, class Fetch, class Emit>
+__device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][C::FN], Fetch fetch, Emit emit) {
   constexpr int FM = C::FM, FN = C::FN, W = 32 * FN, Q = W / 4;      // columns, 16-byte pieces of an LDS row
-  constexpr int LR = (kPair ? W / 2 : W) / E, RI = 64 / LR;          // lanes a row, rows at a time
+  constexpr int LR = (kPair ? W / 2 : W) / E, RI = 64 / LR, N = 32 / RI;   // lanes a row, rows at a time, times
   static_assert(!kPair || FN == 2, "one block of each product");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % C::WGM, wn = wave / C::WGM;
   f32x4* const st = reinterpret_cast<f32x4*>(lds + C::STAGE + wave * C::EPI);
-  const int c0 = (lane % LR) * E;
+  const int c0 = (lane % LR) * E, row0 = wm * FM * 32 + lane / LR, col0 = wn * (kPair ? W / 2 : W) + c0;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
+    decltype(fetch(0, 0)) pre[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) pre[n] = fetch(row0 + 32 * i + n * RI, col0);
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -367,8 +423,9 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
             f32x4{(float)acc[i][j][4 * q], (float)acc[i][j][4 * q + 1], (float)acc[i][j][4 * q + 2], (float)acc[i][j][4 * q + 3]};
     __builtin_amdgcn_wave_barrier();
     if (i == 0) all_landed();
-#pragma unroll 2
-    for (int r = lane / LR; r < 32; r += RI) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = lane / LR + n * RI;
       float v[E], u[E];
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
@@ -378,16 +435,18 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
 #pragma unroll
         for (int z = 0; z < 4; ++z) v[e + z] = x[z], u[e + z] = y[z];
       }
-      emit((wm * FM + i) * 32 + r, wn * (kPair ? W / 2 : W) + c0, v, u);
+      emit(row0 + 32 * i + n * RI, col0, v, u, pre[n]);
     }
     __builtin_amdgcn_wave_barrier();
   }
 }
+struct Nothing {};
 
 // Workgroup b takes tiles b, b + grid, ... of `total` (some past the last of ragged groups).  The next tile's first stage
 // is on its way while this one's results are stored.
 // P: M (products), kADown, kBDown, kPair, E; groups(), what is looked up once for place(that, t), a tile's Place with g (-1:
-// none) and nk (stages); source(place) with load, ragged and clear; emit(place, row, col, v, u).
+// none) and nk (stages); source(place) with load, ragged and clear; fetch(place, row, col) and
+// emit(place, row, col, v, u, what fetch gave).
 template <class C, class P>
 __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
   __shared__ __attribute__((aligned(128))) uint8_t tile_lds[C::SMEM];
@@ -403,7 +462,7 @@ __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
   auto cur = next();
   if (cur.g < 0) return;
   auto src = p.template source<C>(cur, wave, lane);
-  if (cur.nk > 0) src.load(0, ring, wave);
+  if (cur.nk > 0) send_stage<C>(src, 0, ring, wave);
   all_landed();
   while (true) {
     lds_done();
@@ -412,25 +471,30 @@ __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
     const auto nxt = next();
     if (nxt.g >= 0) {
       src = p.template source<C>(nxt, wave, lane);
-      if (nxt.nk > 0) src.load(0, ring, wave);
+      if (nxt.nk > 0) send_stage<C>(src, 0, ring, wave);
     }
-    tile_emit<C, P::E, P::kPair>(tile_lds, acc, [&](int row, int col, const float* v, const float* u) { p.emit(cur, row, col, v, u); });
+    tile_emit<C, P::E, P::kPair>(
+        tile_lds, acc, [&](int row, int col) { return p.fetch(cur, row, col); },
+        [&](int row, int col, const float* v, const float* u, const auto& pre) { p.emit(cur, row, col, v, u, pre); });
     if (nxt.g < 0) return;
     cur = nxt;
   }
 }
 
-// N values side by side, of which the first `ok` exist; kept in 32 bits.
+// N values side by side, of which the first `ok` exist.
+template <class T, int N>
+__device__ __forceinline__ Run<T, N> run_some(const T* p, int ok) {
+  if (ok >= N) return Run<T, N>::load(p);
+  Run<T, N> w;
+#pragma unroll
+  for (int e = 0; e < N; ++e) w.x[e] = e < ok ? p[e] : (T)0.0f;
+  return w;
+}
 template <class T, int N>
 __device__ __forceinline__ void load_some(const T* p, int ok, float (&v)[N]) {
-  if (ok >= N) {
-    const Run<T, N> w = Run<T, N>::load(p);
+  const Run<T, N> w = run_some<T, N>(p, ok);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = (float)w.x[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = e < ok ? (float)p[e] : 0.0f;
-  }
+  for (int e = 0; e < N; ++e) v[e] = (float)w.x[e];
 }
 template <class T, int N>
 __device__ __forceinline__ void store_some(T* p, int ok, const float (&v)[N]) {

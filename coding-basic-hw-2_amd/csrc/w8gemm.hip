@@ -37,12 +37,15 @@ struct Product {
   }
   template <class C>
   struct Src {
+    static constexpr int kTouches = 0;
     Along<C, C::BM> a;
     Along<C, C::BN, kPair> b;
-    __device__ __forceinline__ void load(int kt, uint32_t slot, int wave) const {
-      a.load(kt, slot, wave);
-      b.load(kt, slot + C::SA, wave);
+    __device__ __forceinline__ void prepare(int kt, int wave) {
+      a.prepare(kt, wave);
+      b.prepare(kt, wave);
     }
+    __device__ __forceinline__ void sent(int, int) const {}
+    __device__ __forceinline__ void arrived() const {}
     // integers: zeros on one side are enough
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt, slot); }
@@ -54,7 +57,8 @@ struct Product {
     return Src<C>{Along<C, C::BM>(bytes(p.a) + c.m0 * p.lda, nullptr, p.lda, c.m_end - c.m0, p.k, wave, lane, InOrder{(uint32_t)p.lda}),
                   Along<C, C::BN, kPair>(bytes(p.b) + b0, bytes(p.b_up) + b0, p.ldb, p.n - c.n0, p.k, wave, lane, InOrder{(uint32_t)p.ldb})};
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u) const {
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u, Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.n) return;
     const int ok = p.n - (int)j;

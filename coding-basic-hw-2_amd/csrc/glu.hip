@@ -1,7 +1,6 @@
 // glu.hip -- the gated feed-forward block and its gradients (include/ggemm_glu.h).
 #include <algorithm>
 #include <type_traits>
-#include <cstdlib>
 
 #include "act.hpp"
 #include "tiles.hpp"
@@ -85,8 +84,22 @@ struct Up {
     return Src<C>{Along<C, C::BM>(x, nullptr, px, p.index ? p.x_rows : c.m_end - c.m0, bytes, wave, lane, at),
                   Along<C, C::BN, true>(bytes_of(p.w_gate) + w0, bytes_of(p.w_up) + w0, pw, n, bytes, wave, lane, InOrder{(uint32_t)pw})};
   }
+  __device__ __forceinline__ FewRows few(const Place& c, int i) const {
+    const int64_t px = 2 * p.ldx, pw = 2 * p.ldw, w0 = 2 * (c.g * p.w_stride + c.n0 * p.ldw);
+    const int bytes = 2 * p.d_model, end = (bytes + 15) & ~15;
+    uint32_t va = (uint32_t)i * (uint32_t)px;
+    if (p.index) {
+      const int r = c.m0 + i < c.m_end ? Picked{p.index, p.x_rows}.at(c.m0 + i) : -1;
+      va = r < 0 ? kOut : (uint32_t)r * (uint32_t)px;
+    }
+    const int64_t left = (p.d_ff - c.n0 - 1) * pw + end;
+    return FewRows{bytes_of(p.x) + (p.index ? 0 : c.m0 * px), {bytes_of(p.w_gate) + w0, bytes_of(p.w_up) + w0},
+                   ((p.index ? p.x_rows : c.m_end - c.m0) - 1) * px + end, {left, left}, va, {(uint32_t)i * (uint32_t)pw, (uint32_t)i * (uint32_t)pw},
+                   bytes};
+  }
   __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u, Nothing) const {
+  template <int E>
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&u)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_ff) return;
     const int ok = p.d_ff - (int)j;
@@ -144,8 +157,17 @@ struct DownProduct {
                   Along<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0 * p.ldd), nullptr, pw, p.d_model - c.n0, bytes, wave,
                                   lane, InOrder{(uint32_t)pw})};
   }
+  __device__ __forceinline__ FewRows few(const Place& c, int i) const {
+    const int64_t ph = 2 * ldh, pw = 2 * p.ldd;
+    const int bytes = 2 * p.d_ff, end = (bytes + 15) & ~15;
+    const uint8_t* const w = bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0 * p.ldd);
+    const int64_t left = (p.d_model - c.n0 - 1) * pw + end;   // 16 columns on: that much less, nothing if there are none
+    return FewRows{bytes_of(h) + c.m0 * ph, {w, w + 16 * pw}, (c.m_end - c.m0 - 1) * ph + end, {left, left - 16 * pw},
+                   (uint32_t)i * (uint32_t)ph, {(uint32_t)i * (uint32_t)pw, (uint32_t)i * (uint32_t)pw}, bytes};
+  }
   __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, Nothing) const {
+  template <int E>
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_model) return;
     float o[E];
@@ -221,7 +243,7 @@ struct Hidden {
     k.u = run_some<T, E>(static_cast<const T*>(p.up) + r * p.ldg + j, ok);
     return k;
   }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, const Kept& k) const {
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], const Kept& k) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_ff) return;
     const int ok = p.d_ff - (int)j;
@@ -289,7 +311,8 @@ struct InputGrad {
                   ceil_div(p.d_ff, 64)};
   }
   __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, Nothing) const {
+  template <int E>
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.d_model) return;
     float o[E];
@@ -414,7 +437,8 @@ struct WeightGrad {
     return s;
   }
   __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float*, Nothing) const {
+  template <int E>
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], Nothing) const {
     const bool down = c.which == 2;
     const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model, i = c.m0 + row, j = c.n0 + col;
     if (i >= m || j >= n) return;
@@ -433,36 +457,18 @@ struct WeightGrad {
   }
 };
 
-using Tile256 = TileShape<256, 256, 2, 4>;
-using Tile128 = TileShape<128, 128, 2, 2>;
-using Tile64 = TileShape<64, 128, 2, 2>;
-
 // Tiles of BM rows and `width` columns that a call's groups can need at most.
 int64_t tiles_of(const ggemm_glu_t& p, int bm, int n, int width) { return row_tiles(p.groups, p.rows, bm) * ceil_div(n, width); }
 
-template <class C, class P>
-void run_tiles(const P& p, int64_t tiles, hipStream_t s) {
-  tile_kernel<C, P><<<(unsigned)std::min(tiles, (int64_t)kCus * C::PER_CU), C::NT, 0, s>>>(p, (int)tiles);
-}
-// The tile shape of a product over rows of groups with n columns (kPair: half of a tile's columns).
+// A product over rows of groups with n columns.
 template <class P>
 void run_rows(const P& p, int n, hipStream_t s) {
   constexpr int H = P::kPair ? 2 : 1;
-  const int64_t big = tiles_of(p.p, 256, n, 256 / H);
-  static const char* ev = getenv("GLU_TILE");   // EXPERIMENT
-  if (ev) {
-    const int t = atoi(ev);
-    if (t == 256) run_tiles<Tile256>(p, big, s);
-    else if (t == 128) run_tiles<Tile128>(p, tiles_of(p.p, 128, n, 128 / H), s);
-    else run_tiles<Tile64>(p, tiles_of(p.p, 64, n, 128 / H), s);
-    return;
-  }
-  if (p.p.rows > 64 * (int64_t)p.p.groups) {
-    if (big >= kCus) run_tiles<Tile256>(p, big, s);
-    else run_tiles<Tile128>(p, tiles_of(p.p, 128, n, 128 / H), s);
-  } else {
-    run_tiles<Tile64>(p, tiles_of(p.p, 64, n, 128 / H), s);
-  }
+  const int bm = rows_tile(p.p.groups, p.p.rows, n, 128 / H, !P::kBDown);
+  if (bm == 256) run_tiles<Tile256>(p, tiles_of(p.p, 256, n, 256 / H), s);
+  else if (bm == 128) run_tiles<Tile128>(p, tiles_of(p.p, 128, n, 128 / H), s);
+  else if (bm == 64) run_tiles<Tile64>(p, tiles_of(p.p, 64, n, 128 / H), s);
+  else if constexpr (!P::kBDown) few_kernel<P><<<(unsigned)tiles_of(p.p, 16, n, 32 / H), 256, 0, s>>>(p);
 }
 
 // f(integral_constant<int, D>) for a 16-bit type
@@ -556,8 +562,7 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
       auto go = [&](auto indexed) {
         const WeightGrad<D, decltype(wt)::value, decltype(indexed)::value> w{*p, *d, dg, du, h, ldh, from};
         auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
-        static const char* ev = getenv("GLU_TILE");
-        if (ev ? atoi(ev) == 256 : tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
+        if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
         else run_tiles<Tile128>(w, tiles(128), s);
       };
       if (p->index && p->rows > 0) go(std::true_type{});

@@ -40,18 +40,30 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 struct MmaBf16 {
   using Acc = f32x16;
+  using Acc4 = f32x4;
+  static __device__ __forceinline__ Acc4 mma16(u32x4 b, u32x4 a, Acc4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ Acc mma(u32x4 b, u32x4 a, Acc c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), c, 0, 0, 0);
   }
 };
 struct MmaF16 {
   using Acc = f32x16;
+  using Acc4 = f32x4;
+  static __device__ __forceinline__ Acc4 mma16(u32x4 b, u32x4 a, Acc4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ Acc mma(u32x4 b, u32x4 a, Acc c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
   }
 };
 struct MmaI8 {
   using Acc = i32x16;
+  using Acc4 = i32x4;
+  static __device__ __forceinline__ Acc4 mma16(u32x4 b, u32x4 a, Acc4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ Acc mma(u32x4 b, u32x4 a, Acc c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c, 0, 0, 0);
   }
@@ -152,6 +164,12 @@ struct Window {
     r = i32x4{__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff),
               __builtin_amdgcn_readfirstlane((int)n), 0x00020000};
   }
+  // 16 bytes to a register
+  __device__ __forceinline__ u32x4 fetch(uint32_t off) const {
+    const auto b = __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<void*>(((uint64_t)(uint32_t)r[1] << 32) | (uint32_t)r[0]), 0, r[2], r[3]);
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+  }
   __device__ __forceinline__ void send(uint32_t off, uint32_t lds) const {
     // s_nop 3: with the move, the five wait states that a scalar register written by a vector instruction (the compiler may
     // have kept one in a lane) needs before a memory instruction reads it; the compiler's own check does not see in here
@@ -200,7 +218,7 @@ struct Along {
 #pragma unroll
     for (int q = 0; q < P; ++q) o[q] = v[q] | out;
     const int64_t at = 128 * (int64_t)kt;
-    if constexpr (kPair && C::NW == 4) {   // piece p = wave + 4 q: its matrix is q's lowest bit
+    if constexpr (kPair && C::NW < 8) {   // piece p = wave + NW q: its matrix is p's bit 2, a bit of q
       w = Window(from + at, left - at);
       w2 = Window(from2 + at, left - at);
     } else {                               // p = wave + 8 q: the wave's bit 2
@@ -210,8 +228,8 @@ struct Along {
   __device__ __forceinline__ void prepare(int kt, int wave) { prepare(base, base2, kt, wave); }
   // Sends piece q of the prepared stage.
   __device__ __forceinline__ void send(int q, uint32_t slot, int wave) const {
-    static_assert(!kPair || C::NW == 4 || C::NW == 8, "pieces of a pair");
-    (kPair && C::NW == 4 && (q & 1) ? w2 : w).send(o[q], slot + 1024 * (wave + C::NW * q));
+    static_assert(!kPair || C::NW == 2 || C::NW == 4 || C::NW == 8, "pieces of a pair");
+    (kPair && C::NW < 8 && (C::NW * q >> 2 & 1) ? w2 : w).send(o[q], slot + 1024 * (wave + C::NW * q));
   }
   // Whether stage kt ends inside a chunk, and that chunk's rest to zeros.
   __device__ __forceinline__ bool ragged(int kt) const { return bytes % 16 != 0 && bytes - 128 * kt <= 128; }
@@ -475,7 +493,7 @@ __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
     }
     tile_emit<C, P::E, P::kPair>(
         tile_lds, acc, [&](int row, int col) { return p.fetch(cur, row, col); },
-        [&](int row, int col, const float* v, const float* u, const auto& pre) { p.emit(cur, row, col, v, u, pre); });
+        [&](int row, int col, const float (&v)[P::E], const float (&u)[P::E], const auto& pre) { p.emit(cur, row, col, v, u, pre); });
     if (nxt.g < 0) return;
     cur = nxt;
   }
@@ -508,6 +526,112 @@ __device__ __forceinline__ void store_some(T* p, int ok, const float (&v)[N]) {
     for (int e = 0; e < N; ++e)
       if (e < ok) p[e] = (T)v[e];
   }
+}
+
+// Few rows: a workgroup computes 16 rows x 32 columns (kPair: 16 columns of both products); its 4 waves take every fourth
+// run of 256 bytes of the inner dimension straight from memory into registers and join their sums in LDS in order.
+// Products are 16 x 16: lane l holds 16 bytes of row l % 16 from byte 16 (l / 16) of 64, so that a load takes 64 bytes side
+// by side of each of 16 rows, and the four loads of a run whole lines.
+// Bound: the bytes of B, which nobody else reads: 134 MB of 8 experts' weights (2048 x 4096, 16-bit) 29 us, 4.6 TB/s.  8 or 16
+// waves: equal where there are fewer workgroups than compute units, up to twice as long (64 experts); two runs
+// on the way: 5 to 30 % slower; room for 6 or 8 waves a SIMD: 40 to 90 % slower (fewer loads of a wave at once);
+// non-temporal loads: equal to 30 % slower.
+struct FewShape {
+  static constexpr int BM = 16, BN = 32;
+};
+// Where a lane's operands are: rows of A and of the two blocks of B, as offsets in windows.
+struct FewRows {
+  const uint8_t *a, *b[2];
+  int64_t a_left, b_left[2];
+  uint32_t va, vb[2];
+  int bytes;   // of a row
+};
+template <class P>
+__global__ void __launch_bounds__(256, 4) few_kernel(P p) {
+  using Acc4 = typename P::M::Acc4;
+  constexpr int NW = 4;
+  __shared__ Acc4 sums[NW][2][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+  const auto c = p.template place<FewShape>(p.template groups<FewShape::BM, FewShape::BN>(), blockIdx.x);
+  if (c.g < 0) return;
+  const FewRows f = p.few(c, lane & 15);
+  Acc4 acc[2] = {};
+  const int runs = ceil_div(f.bytes, 256);
+  for (int r = wave; r < runs; r += NW) {
+    const int64_t at = 256 * (int64_t)r;
+    u32x4 x[3][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t off = 64 * s + 16 * quarter;
+      const uint32_t out = at + off >= f.bytes ? kOut : 0u;
+      x[0][s] = Window(f.a + at, f.a_left - at).fetch((f.va + off) | out);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[1 + j][s] = Window(f.b[j] + at, f.b_left[j] - at).fetch((f.vb[j] + off) | out);
+    }
+    if (f.bytes % 16 != 0 && r + 1 == runs) {   // what lies between the row's end and the next 16 bytes
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int have = f.bytes - (int)at - 64 * s - 16 * quarter;   // bytes of this lane's that exist
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int n = have - 4 * w;
+            x[i][s][w] &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+          }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[j] = P::M::mma16(x[1 + j][s], x[0][s], acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) sums[wave][j][lane] = acc[j];
+  __syncthreads();
+  if (wave >= (P::kPair ? 1 : 2)) return;
+  // C's transpose: row lane % 16, columns 4 (lane / 16) + 0 .. 3 of a block
+  Acc4 s = sums[0][P::kPair ? 0 : wave][lane], t = sums[0][1][lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    s += sums[w][P::kPair ? 0 : wave][lane];
+    if constexpr (P::kPair) t += sums[w][1][lane];
+  }
+  const float v[4] = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
+  const float u[4] = {(float)t[0], (float)t[1], (float)t[2], (float)t[3]};
+  p.emit(c, lane & 15, (P::kPair ? 0 : 16 * wave) + 4 * quarter, v, u, Nothing{});
+}
+
+using Tile256 = TileShape<256, 256, 2, 4>;
+using Tile128 = TileShape<128, 128, 2, 2>;
+using Tile64 = TileShape<64, 128, 2, 2>;
+template <class C, class P>
+void run_tiles(const P& p, int64_t tiles, hipStream_t s) {
+  tile_kernel<C, P><<<(unsigned)std::min(tiles, (int64_t)kCus * C::PER_CU), C::NT, 0, s>>>(p, (int)tiles);
+}
+
+// Which kernel computes rows of groups (m in all) times n columns: rows of its tile, 16 for the few rows'.  width: columns of a
+// tile of 128 (64 where they are two products').  The host does not know the groups' own rows: half a tile more for each.
+// Times of one round of workgroups, all compute units filled, to those of a half-filled one, 8-bit products, n = 4096, k =
+// 4096, us: 64 x 128 tiles (two a compute unit) 26, 24; 128 x 128 (two) 40, 29; 256 x 256 (one) 64, 52; the same
+// ratios at k = 2048 and 1024.  So the tile with the least rounds times cost is taken; at 2048 rows 52, 42, 54 us, at 3001 78,
+// 65, 59, at 4096 101, 79, 67.
+// Few rows: up to two workgroups a compute unit (n = k = 4096: 64 rows 15.1, by tiles 15.9; 128 rows 25 and 22), up to four
+// if groups have 16 rows at most on average, so that nobody else reads their weights (32 groups, 1024 x 1024: 7.6 and 8.7; 8
+// experts' 16-bit weights of 4096 x 2048 twice, 8 workgroups a compute unit: 57 and 52).
+inline int rows_tile(int groups, int64_t m, int64_t n, int width, bool may_be_few) {
+  const int64_t g = std::min<int64_t>(groups, m);
+  auto tiles = [&](int bm, int cols) { return (m / bm + (groups > 1 ? (g + 1) / 2 : m % bm != 0)) * ((n + cols - 1) / cols); };
+  const bool one = m <= 16 * (int64_t)groups;
+  const int64_t few = (one ? g : groups > 1 ? m / 16 + g : (m + 15) / 16) * ((n + width / 4 - 1) / (width / 4));
+  if (may_be_few && few <= (one ? 4 : 2) * kCus) return 16;
+  auto cost = [](int64_t t, int64_t slots, int full, int half) {
+    const int64_t rest = t % slots, over = rest - slots / 2;
+    return t / slots * full + (rest == 0 ? 0 : half) + (over > 0 ? (full - half) * over / (slots / 2) : 0);
+  };
+  const int64_t c64 = cost(tiles(64, width), 2 * kCus, 26, 24), c128 = cost(tiles(128, width), 2 * kCus, 40, 29);
+  const int64_t c256 = cost(tiles(256, 2 * width), kCus, 64, 52);
+  return c256 <= std::min(c64, c128) ? 256 : c128 <= c64 ? 128 : 64;
 }
 
 }  // namespace ggemm

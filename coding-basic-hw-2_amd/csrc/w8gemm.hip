@@ -57,8 +57,18 @@ struct Product {
     return Src<C>{Along<C, C::BM>(bytes(p.a) + c.m0 * p.lda, nullptr, p.lda, c.m_end - c.m0, p.k, wave, lane, InOrder{(uint32_t)p.lda}),
                   Along<C, C::BN, kPair>(bytes(p.b) + b0, bytes(p.b_up) + b0, p.ldb, p.n - c.n0, p.k, wave, lane, InOrder{(uint32_t)p.ldb})};
   }
+  __device__ __forceinline__ FewRows few(const Place& c, int i) const {
+    auto bytes = [](const int8_t* x) { return reinterpret_cast<const uint8_t*>(x); };
+    const int64_t b0 = c.g * p.b_stride + c.n0 * p.ldb;
+    const int end = (p.k + 15) & ~15;
+    const int64_t left = (p.n - c.n0 - 1) * p.ldb + end;   // 16 columns on: that much less, nothing if there are none
+    const uint32_t vb = (uint32_t)i * (uint32_t)p.ldb;
+    return FewRows{bytes(p.a) + c.m0 * p.lda, {bytes(p.b) + b0, kPair ? bytes(p.b_up) + b0 : bytes(p.b) + b0 + 16 * p.ldb},
+                   (c.m_end - c.m0 - 1) * p.lda + end, {left, kPair ? left : left - 16 * p.ldb}, (uint32_t)i * (uint32_t)p.lda, {vb, vb}, p.k};
+  }
   __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float* v, const float* u, Nothing) const {
+  template <int E>
+  __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&u)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
     if (r >= c.m_end || j >= p.n) return;
     const int ok = p.n - (int)j;
@@ -96,22 +106,16 @@ bool args_ok(const ggemm_w8_gemm_t* p) {
   auto operand = [](const int8_t* x) { return x && aligned(x, 16); };
   return p->k == 0 || (operand(p->a) && operand(p->b) && (!p->act || operand(p->b_up)));
 }
-using Tile256 = TileShape<256, 256, 2, 4>;
-using Tile128 = TileShape<128, 128, 2, 2>;
-using Tile64 = TileShape<64, 128, 2, 2>;
+// Tiles of BM rows that a call's groups can need at most; cols: of a tile, half of them columns of C where it computes a pair.
+int64_t tiles_of(const ggemm_w8_gemm_t& p, int bm, int cols) { return row_tiles(p.groups, p.m, bm) * ceil_div(p.n, p.act ? cols / 2 : cols); }
 
-int64_t tiles_of(const ggemm_w8_gemm_t& p, int bm, int bn) { return row_tiles(p.groups, p.m, bm) * ceil_div(p.n, p.act ? bn / 2 : bn); }
-
-template <class C, class P>
-void run_tiles(const P& p, hipStream_t s) {
-  const int64_t tiles = tiles_of(p.p, C::BM, C::BN);
-  tile_kernel<C, P><<<(unsigned)std::min(tiles, (int64_t)kCus * C::PER_CU), C::NT, 0, s>>>(p, (int)tiles);
-}
 template <class P>
 void run(const P& p, hipStream_t s) {
-  if (p.p.m <= 64 * (int64_t)p.p.groups) run_tiles<Tile64>(p, s);
-  else if (tiles_of(p.p, 256, 256) >= kCus) run_tiles<Tile256>(p, s);
-  else run_tiles<Tile128>(p, s);
+  const int bm = rows_tile(p.p.groups, p.p.m, p.p.n, P::kPair ? 64 : 128, true);
+  if (bm == 256) run_tiles<Tile256>(p, tiles_of(p.p, 256, 256), s);
+  else if (bm == 128) run_tiles<Tile128>(p, tiles_of(p.p, 128, 128), s);
+  else if (bm == 64) run_tiles<Tile64>(p, tiles_of(p.p, 64, 128), s);
+  else few_kernel<P><<<(unsigned)tiles_of(p.p, 16, 32), 256, 0, s>>>(p);
 }
 
 }  // namespace

@@ -188,7 +188,7 @@ struct Hidden {
   ggemm_glu_t p;
   const void* dy;
   int64_t lddy;
-  T *dg, *du, *h;
+  T *dg, *du, *h;   // dg and du or h: NULL where nobody reads them
   int64_t ldh;
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
@@ -259,9 +259,11 @@ struct Hidden {
       o[e] = live ? a * w : 0.0f;
       g[e] = live ? v[e] * w * fmaf(g[e], dq, q) : 0.0f;
     }
-    store_some(dg + r * ldh + j, ok, g);
-    store_some(du + r * ldh + j, ok, u);
-    store_some(h + r * ldh + j, ok, o);
+    if (dg) {
+      store_some(dg + r * ldh + j, ok, g);
+      store_some(du + r * ldh + j, ok, u);
+    }
+    if (h) store_some(h + r * ldh + j, ok, o);
   }
 };
 
@@ -545,6 +547,7 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
   if (ws_bytes < glu_backward_workspace(p, d)) return GGEMM_ERR_WORKSPACE;
   if (p->rows > 0 && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
   if (!tiles_fit(*p, d->dw_gate || d->dw_down)) return GGEMM_ERR_INVALID;
+  if (!d->dw_gate && !d->dw_down && (!d->dx || p->rows == 0)) return GGEMM_OK;
   return launch([&] { with_type(p->dtype, [&](auto dt) {
     constexpr int D = decltype(dt)::value;
     using T = typename Elem<D>::T;
@@ -553,7 +556,11 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
     T *const dg = reinterpret_cast<T*>(b), *const du = reinterpret_cast<T*>(b + n), *const h = reinterpret_cast<T*>(b + 2 * n);
     const int64_t ldh = ld_hidden(*p);
     if (p->rows > 0) {
-      with_act(p->act, [&](auto act) { run_rows(Hidden<D, decltype(act)::value>{*p, d->dy, d->lddy, dg, du, h, ldh}, p->d_ff, s); });
+      const bool gu = d->dx || d->dw_gate;
+      with_act(p->act, [&](auto act) {
+        run_rows(Hidden<D, decltype(act)::value>{*p, d->dy, d->lddy, gu ? dg : nullptr, gu ? du : nullptr, d->dw_down ? h : nullptr, ldh},
+                 p->d_ff, s);
+      });
       if (d->dx) run_rows(InputGrad<D>{*p, d->dx, d->lddx, dg, du, ldh}, p->d_model, s);
     }
     if (!d->dw_gate && !d->dw_down) return;

@@ -62,8 +62,6 @@ struct Up {
       a.prepare(kt, wave);
       b.prepare(kt, wave);
     }
-    __device__ __forceinline__ void sent(int, int) const {}
-    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
       a.clear(kt, slot);
@@ -141,8 +139,6 @@ struct DownProduct {
       a.prepare(kt, wave);
       b.prepare(kt, wave);
     }
-    __device__ __forceinline__ void sent(int, int) const {}
-    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const {
       a.clear(kt, slot);
@@ -211,8 +207,6 @@ struct Hidden {
       a.prepare(kt, wave);
       b.prepare(b.base, kt);
     }
-    __device__ __forceinline__ void sent(int, int) const {}
-    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ void touch(int part, uint32_t scrap, int wave, int lane) const {
       const int l = 64 * (part * C::NW + wave) + lane, r = l / ROW_LINES % C::BM, c = 128 * (l % ROW_LINES);
       const uint8_t* const p = (l / ROW_LINES / C::BM ? up : gate) + min(r, rows - 1) * pitch + min(c, bytes - 2);
@@ -299,8 +293,6 @@ struct InputGrad {
       a.prepare(second ? a.base2 : a.base, nullptr, second ? kt - half : kt, wave);
       b.prepare(second ? b2 : b.base, second ? kt - half : kt);
     }
-    __device__ __forceinline__ void sent(int, int) const {}
-    __device__ __forceinline__ void arrived() const {}
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt >= half ? kt - half : kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt >= half ? kt - half : kt, slot); }
   };
@@ -328,7 +320,7 @@ struct InputGrad {
 struct WeightPlace {
   int g, which, lo, m0, n0, depth, nk;
 };
-template <int D, int W, bool kIndexed>
+template <int D, int W>
 struct WeightGrad {
   using T = typename Elem<D>::T;
   using O = typename Elem<W>::T;
@@ -336,7 +328,7 @@ struct WeightGrad {
   using Place = WeightPlace;
   static constexpr bool kADown = true, kBDown = true, kPair = false;
   static constexpr int E = 8;
-  ggemm_glu_t p;
+  ggemm_glu_t p;        // x and dy: one row for each of the call's rows
   ggemm_glu_grad_t d;
   const T *dg, *du, *h;
   int64_t ldh;
@@ -367,76 +359,21 @@ struct WeightGrad {
     static constexpr int kTouches = 0;
     Down<C, C::BM> a;
     Down<C, C::BN> b;
-    const int32_t* index;   // of the group's first row on
-    int x_rows, depth;
-    uint32_t pitch;         // of gathered rows; 0 where the operand's rows are the group's in order
-    // Index entries of this lane's steps.  They are loaded two stages before the loads that go by them and taken over
-    // (arrived) right after a wait for everything in flight: looked at any later or earlier, the compiler's wait for them
-    // would also wait for operands on their way (16 groups of 2048 rows, (2048, 4096): 1930 us, without an index 1607).
-    static constexpr int P = Down<C, C::BM>::P;
-    struct Entries {
-      int at[kIndexed ? P : 1];
-    } row, second, third, coming;   // of the next stage to prepare; of the tile's second and third; in flight
-    __device__ __forceinline__ Entries entries(int kt, int wave, int lane) const {
-      Entries r{};
-      if constexpr (kIndexed) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) r.at[q] = index[(uint32_t)min(64 * kt + Down<C, C::BM>::step(q, wave, lane), depth - 1)];
-      }
-      return r;
-    }
-    __device__ __forceinline__ void prepare(int kt, int wave) {
+    __device__ __forceinline__ void prepare(int kt, int) {
       a.prepare(a.base, kt);
       b.prepare(b.base, kt);
-      if constexpr (kIndexed) {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-          const bool live = (uint32_t)row.at[q] < (uint32_t)x_rows && Down<C, C::BM>::step(q, wave, lane) < depth - 64 * kt;
-          a.o[q] = live ? a.v[q] : kOut;
-          b.o[q] = live ? (uint32_t)row.at[q] * pitch + b.v[q] : kOut;
-        }
-      }
-    }
-    __device__ __forceinline__ void arrived() {
-      if constexpr (kIndexed) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) asm volatile("" : "+v"(coming.at[q]));
-        row = coming;
-      }
-    }
-    __device__ __forceinline__ void sent(int kt, int wave) {
-      if constexpr (kIndexed) {
-        if (kt == 0) row = second;
-        else if (kt == 1) row = third;
-        else coming = entries(kt + 2, wave, threadIdx.x & 63);
-      }
     }
     __device__ __forceinline__ bool ragged(int) const { return false; }
     __device__ __forceinline__ void clear(int, uint8_t*) const {}
   };
   template <class C>
   __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
-    const bool down = c.which == 2, gather = kIndexed && !down;
+    const bool down = c.which == 2;
     const int64_t pa = 2 * (down ? d.lddy : ldh), pb = 2 * (down ? ldh : p.ldx);
     const uint8_t* const a = bytes_of(down ? d.dy : c.which ? (const void*)du : dg) + c.lo * pa + 2 * c.m0;
-    const uint8_t* const b = bytes_of(down ? (const void*)h : p.x) + (gather ? 0 : c.lo * pb) + 2 * c.n0;
+    const uint8_t* const b = bytes_of(down ? (const void*)h : p.x) + c.lo * pb + 2 * c.n0;
     const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model;
-    Src<C> s{Down<C, C::BM>(a, pa, c.depth, m - c.m0, wave, lane), Down<C, C::BN>(b, pb, c.depth, n - c.n0, wave, lane),
-             p.index + c.lo, p.x_rows, c.depth, gather ? (uint32_t)pb : 0u};
-    if (gather) {   // any row in any stage
-      s.b.stage = 0;
-      s.b.left = (p.x_rows - 1) * pb + ((2 * (n - c.n0) + 15) & ~15);
-#pragma unroll
-      for (int q = 0; q < Src<C>::P; ++q) s.b.v[q] = s.b.col;
-    }
-    if (kIndexed && c.depth > 0) {
-      s.row = s.entries(0, wave, lane);
-      s.second = s.entries(1, wave, lane);
-      s.third = s.entries(2, wave, lane);
-      s.coming = s.entries(3, wave, lane);
-    }
-    return s;
+    return Src<C>{Down<C, C::BM>(a, pa, c.depth, m - c.m0, wave, lane), Down<C, C::BN>(b, pb, c.depth, n - c.n0, wave, lane)};
   }
   __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
   template <int E>
@@ -458,6 +395,23 @@ struct WeightGrad {
     store_some(out, n - j, o);
   }
 };
+
+// Rows of x in the call's order and rows of dy, zeros where the index names none, for the weights' gradients: 256 lanes cover cx
+// chunks of 8 columns (a power of two) of 256 / cx rows.  (Rows looked up in the products' loop instead: 16 groups of
+// 2048 rows, (2048, 4096), 1820 us for the products, 1570 without an index; these copies take about 90.)  xg or yg may be NULL.
+__global__ void __launch_bounds__(256) gather_kernel(ggemm_glu_t p, const void* dy, int64_t lddy, u32x4* xg, u32x4* yg, int chunks, int log_cx) {
+  const int c = (blockIdx.y << log_cx) + (threadIdx.x & ((1 << log_cx) - 1));
+  if (c >= chunks) return;
+  const int64_t step = (int64_t)gridDim.x << (8 - log_cx);
+  for (int64_t r = ((int64_t)blockIdx.x << (8 - log_cx)) + (threadIdx.x >> log_cx); r < p.rows; r += step) {
+    const int64_t at = Picked{p.index, p.x_rows}.at((int)r);
+    u32x4 x{}, y{};
+    if (at >= 0 && xg) x = *reinterpret_cast<const u32x4*>(bytes_of(p.x) + 2 * (at * p.ldx + 8 * c));
+    if (at >= 0 && yg) y = *reinterpret_cast<const u32x4*>(bytes_of(dy) + 2 * (r * lddy + 8 * c));
+    if (xg) xg[r * chunks + c] = x;
+    if (yg) yg[r * chunks + c] = y;
+  }
+}
 
 // Tiles of BM rows and `width` columns that a call's groups can need at most.
 int64_t tiles_of(const ggemm_glu_t& p, int bm, int n, int width) { return row_tiles(p.groups, p.rows, bm) * ceil_div(n, width); }
@@ -528,8 +482,11 @@ int glu(const ggemm_glu_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
   }); }); });
 }
 
+int64_t ld_model(const ggemm_glu_t& p) { return (int64_t)align_up((size_t)p.d_model, 8); }
+size_t model_bytes(const ggemm_glu_t& p) { return align_up((size_t)p.rows * ld_model(p) * 2, 256); }
+
 size_t glu_backward_workspace(const ggemm_glu_t* p, const ggemm_glu_grad_t* d) {
-  return shape_ok(p) && d ? 3 * hidden_bytes(*p) : 0;
+  return shape_ok(p) && d ? 3 * hidden_bytes(*p) + (p->index ? 2 * model_bytes(*p) : 0) : 0;
 }
 
 int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size_t ws_bytes, hipStream_t s) {
@@ -565,15 +522,26 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
     }
     if (!d->dw_gate && !d->dw_down) return;
     const int matrices = (d->dw_gate ? 2 : 0) + (d->dw_down ? 1 : 0), from = d->dw_gate ? 0 : 2;
+    ggemm_glu_t rows = *p;
+    ggemm_glu_grad_t grad = *d;
+    if (p->index && p->rows > 0) {
+      uint8_t *const xg = b + 3 * n, *const yg = xg + model_bytes(*p);
+      const int chunks = (int)(ld_model(*p) / 8);
+      int log_cx = 0;
+      while (log_cx < 8 && (1 << log_cx) < chunks) ++log_cx;
+      const int64_t groups = ((int64_t)p->rows + (256 >> log_cx) - 1) >> (8 - log_cx);
+      gather_kernel<<<dim3((unsigned)std::min(groups, (int64_t)1 << 16), ceil_div(chunks, 1 << log_cx)), 256, 0, s>>>(
+          *p, d->dy, d->lddy, d->dw_gate ? reinterpret_cast<u32x4*>(xg) : nullptr, d->dw_down ? reinterpret_cast<u32x4*>(yg) : nullptr, chunks,
+          log_cx);
+      rows.x = xg;
+      grad.dy = yg;
+      rows.ldx = grad.lddy = ld_model(*p);
+    }
     with_elem(d->dw_dtype, [&](auto wt) {
-      auto go = [&](auto indexed) {
-        const WeightGrad<D, decltype(wt)::value, decltype(indexed)::value> w{*p, *d, dg, du, h, ldh, from};
-        auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
-        if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
-        else run_tiles<Tile128>(w, tiles(128), s);
-      };
-      if (p->index && p->rows > 0) go(std::true_type{});
-      else go(std::false_type{});
+      const WeightGrad<D, decltype(wt)::value> w{rows, grad, dg, du, h, ldh, from};
+      auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
+      if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
+      else run_tiles<Tile128>(w, tiles(128), s);
     });
   }); });
 }

@@ -325,7 +325,6 @@ __device__ __forceinline__ void send_stage(S& src, int kt, uint32_t slot, int wa
   for (int q = 0; q < C::PA; ++q) src.a.send(q, slot, wave);
 #pragma unroll
   for (int q = 0; q < C::PB; ++q) src.b.send(q, slot + C::SA, wave);
-  src.sent(kt, wave);
 }
 
 // The wave's FM x FN blocks, as C's transpose: lane l holds of block (i, j) row 32 i + l % 32 and columns
@@ -333,8 +332,7 @@ __device__ __forceinline__ void send_stage(S& src, int kt, uint32_t slot, int wa
 // wave's part).
 // Between the barrier and the next products nothing but sends is left to do, one after each product: the scalar
 // work of a stage's loads comes before the barrier, under the products of the first half.  (All of it after the barrier, ahead
-// of the products: gradients of weights with an index, 16 groups of 2048 rows, (2048, 4096), 1930 us, as against 1607
-// without.)
+// of the products: 8-bit 8192^3 480 us, as it is 456.)
 template <class C, class M, bool kADown, bool kBDown, class S>
 __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, typename M::Acc (&acc)[C::FM][C::FN]) {
   constexpr int FM = C::FM, FN = C::FN;
@@ -379,8 +377,6 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
     const int sn = C::STAGE - so;
     pin();
     stage_done();
-    __builtin_amdgcn_sched_barrier(0);   // the compiler takes nothing of this, and no wait of its own for it, above the barrier
-    src.arrived();
     if (kt + 1 < nk && src.ragged(kt + 1)) {
       src.clear(kt + 1, lds + sn);
       lds_done();
@@ -401,7 +397,6 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
           }
         }
       }
-    if (more) src.sent(kt + 2, wave);
     if constexpr (S::kTouches > 0) {   // in the last stages but one, for the epilogue
       const int part = nk - 2 - kt;
       if (part >= 0 && part < S::kTouches) src.touch(part, ring + C::SCRAP + 256 * wave, wave, lane);

@@ -44,8 +44,6 @@ struct Product {
       a.prepare(kt, wave);
       b.prepare(kt, wave);
     }
-    __device__ __forceinline__ void sent(int, int) const {}
-    __device__ __forceinline__ void arrived() const {}
     // integers: zeros on one side are enough
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt, slot); }

@@ -69,7 +69,7 @@ int ggemm_glu(const ggemm_glu_t* p, void* workspace, size_t workspace_bytes, hip
  *   dWd_e  = dy^T h + dw_beta dWd_e        and these too are written for groups without rows
  * Rows whose index lies outside [0, x_rows) count as zeros throughout, dy among them, and get dx = 0.
  * dx may be NULL, dw_gate and dw_up together, and dw_down: what is not wanted is not computed.  With dw_beta == 0 the
- * gradients of the weights are not read. */
+ * gradients of the weights are not read.  The workspace also goes by whether index is NULL. */
 typedef struct {
   const void* dy; int64_t lddy;
   void* dx; int64_t lddx;

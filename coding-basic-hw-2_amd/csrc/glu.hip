@@ -11,6 +11,7 @@ namespace {
 // Where a tile of rows of a group lies: rows [m0, m_end), first column, stages of the inner dimension.
 struct Place {
   int g, m0, m_end, n0, nk;
+  bool whole;   // every row and column of the tile exists
 };
 template <class C>
 __device__ __forceinline__ Place row_place(const RowGroups& rows, const GroupTiles<C::BM>& first, int t, int n, int width, int nk) {
@@ -19,7 +20,8 @@ __device__ __forceinline__ Place row_place(const RowGroups& rows, const GroupTil
   if (s.g < 0) return Place{-1};
   int tm, tn;
   tile_raster(t, ceil_div(s.hi - s.lo, C::BM), nt, tm, tn);
-  return Place{s.g, s.lo + tm * C::BM, s.hi, tn * width, nk};
+  const int m0 = s.lo + tm * C::BM, n0 = tn * width;
+  return Place{s.g, m0, s.hi, n0, nk, m0 + C::BM <= s.hi && n0 + width <= n};
 }
 __device__ __forceinline__ const uint8_t* bytes_of(const void* p) { return static_cast<const uint8_t*>(p); }
 
@@ -95,12 +97,15 @@ struct Up {
                    ((p.index ? p.x_rows : c.m_end - c.m0) - 1) * px + end, {left, left}, va, {(uint32_t)i * (uint32_t)pw, (uint32_t)i * (uint32_t)pw},
                    bytes};
   }
-  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  template <int E>
+  template <bool kWhole>
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const {
+    return {};
+  }
+  template <bool kWhole, int E>
   __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&u)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
-    if (r >= c.m_end || j >= p.d_ff) return;
-    const int ok = p.d_ff - (int)j;
+    if (!kWhole && (r >= c.m_end || j >= p.d_ff)) return;
+    const int ok = kWhole ? E : p.d_ff - (int)j;
     float g[E], w[E], o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) g[e] = v[e], w[e] = u[e], o[e] = act_value<ACT>(v[e]) * u[e];
@@ -161,15 +166,18 @@ struct DownProduct {
     return FewRows{bytes_of(h) + c.m0 * ph, {w, w + 16 * pw}, (c.m_end - c.m0 - 1) * ph + end, {left, left - 16 * pw},
                    (uint32_t)i * (uint32_t)ph, {(uint32_t)i * (uint32_t)pw, (uint32_t)i * (uint32_t)pw}, bytes};
   }
-  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  template <int E>
+  template <bool kWhole>
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const {
+    return {};
+  }
+  template <bool kWhole, int E>
   __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
-    if (r >= c.m_end || j >= p.d_model) return;
+    if (!kWhole && (r >= c.m_end || j >= p.d_model)) return;
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = v[e];
-    store_some(static_cast<T*>(p.y) + r * p.ldy + j, p.d_model - (int)j, o);
+    store_some(static_cast<T*>(p.y) + r * p.ldy + j, kWhole ? E : p.d_model - (int)j, o);
   }
 };
 
@@ -227,20 +235,22 @@ struct Hidden {
     Run<T, E> g, u;
     bool live;
   };
+  template <bool kWhole>
   __device__ __forceinline__ Kept fetch(const Place& c, int row, int col) const {
     Kept k{};
     const int64_t r = c.m0 + row, j = c.n0 + col;
-    if (r >= c.m_end || j >= p.d_ff) return k;
-    const int ok = p.d_ff - (int)j;
+    if (!kWhole && (r >= c.m_end || j >= p.d_ff)) return k;
+    const int ok = kWhole ? E : p.d_ff - (int)j;
     k.live = Picked{p.index, p.x_rows}.live((int)r);
     k.g = run_some<T, E>(static_cast<const T*>(p.gate) + r * p.ldg + j, ok);
     k.u = run_some<T, E>(static_cast<const T*>(p.up) + r * p.ldg + j, ok);
     return k;
   }
+  template <bool kWhole, int E>
   __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], const Kept& k) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
-    if (r >= c.m_end || j >= p.d_ff) return;
-    const int ok = p.d_ff - (int)j;
+    if (!kWhole && (r >= c.m_end || j >= p.d_ff)) return;
+    const int ok = kWhole ? E : p.d_ff - (int)j;
     const bool live = k.live;
     float g[E], u[E], o[E];
 #pragma unroll
@@ -304,21 +314,25 @@ struct InputGrad {
                   Down<C, C::BN>(bytes_of(p.w_gate) + w0, 2 * p.ldw, p.d_ff, p.d_model - c.n0, wave, lane), bytes_of(p.w_up) + w0,
                   ceil_div(p.d_ff, 64)};
   }
-  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  template <int E>
+  template <bool kWhole>
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const {
+    return {};
+  }
+  template <bool kWhole, int E>
   __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
-    if (r >= c.m_end || j >= p.d_model) return;
+    if (!kWhole && (r >= c.m_end || j >= p.d_model)) return;
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = v[e];
-    store_some(static_cast<T*>(dx) + r * lddx + j, p.d_model - (int)j, o);
+    store_some(static_cast<T*>(dx) + r * lddx + j, kWhole ? E : p.d_model - (int)j, o);
   }
 };
 
 // Gradients of the weights: dWg = dgate^T x, dWu = dup^T x (d_ff x d_model), dWd = dy^T h (d_model x d_ff), in one launch.
 struct WeightPlace {
   int g, which, lo, m0, n0, depth, nk;
+  bool whole;
 };
 template <int D, int W>
 struct WeightGrad {
@@ -352,6 +366,7 @@ struct WeightGrad {
     tile_raster(t % per, down ? td : tf, down ? tf : td, tm, tn);
     a.m0 = tm * C::BM;
     a.n0 = tn * C::BM;
+    a.whole = a.m0 + C::BM <= (down ? p.d_model : p.d_ff) && a.n0 + C::BM <= (down ? p.d_ff : p.d_model);
     return a;
   }
   template <class C>
@@ -375,24 +390,27 @@ struct WeightGrad {
     const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model;
     return Src<C>{Down<C, C::BM>(a, pa, c.depth, m - c.m0, wave, lane), Down<C, C::BN>(b, pb, c.depth, n - c.n0, wave, lane)};
   }
-  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  template <int E>
+  template <bool kWhole>
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const {
+    return {};
+  }
+  template <bool kWhole, int E>
   __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&)[E], Nothing) const {
     const bool down = c.which == 2;
     const int m = down ? p.d_model : p.d_ff, n = down ? p.d_ff : p.d_model, i = c.m0 + row, j = c.n0 + col;
-    if (i >= m || j >= n) return;
+    if (!kWhole && (i >= m || j >= n)) return;
     O* const base = static_cast<O*>(down ? d.dw_down : c.which ? d.dw_up : d.dw_gate);
     O* const out = base + (down ? c.g * d.dd_stride + i * d.lddd : c.g * d.dw_stride + i * d.lddw) + j;
     float o[E];
     if (d.dw_beta != 0.0f) {
-      load_some(static_cast<const O*>(out), n - j, o);
+      load_some(static_cast<const O*>(out), kWhole ? E : n - j, o);
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = fmaf(d.dw_beta, o[e], v[e]);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = v[e];
     }
-    store_some(out, n - j, o);
+    store_some(out, kWhole ? E : n - j, o);
   }
 };
 

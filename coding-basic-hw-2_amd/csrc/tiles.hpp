@@ -23,6 +23,7 @@
 // bytes between an odd inner dimension and the next 16 are cleared in LDS.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "mx4.hpp"
 
@@ -414,7 +415,9 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
 // products of the same columns, v and u, and col counts one of them; else u is v.  pre is what fetch(row, col) gave: the
 // loads of a row of blocks go together.
 // Before the first emit the wave waits for the transfers in flight, the next tile's first stage.
-template <class C, int E, bool kPair, class Acc, class Fetch, class Emit>
+// kWhole: every row and column exists; the rows of a block are unrolled, so that their loads go together.  Else one after another:
+// the checks of every row unrolled make the code of a tile longer than the instruction cache.
+template <class C, int E, bool kPair, bool kWhole, class Acc, class Fetch, class Emit>
 __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][C::FN], Fetch fetch, Emit emit) {
   constexpr int FM = C::FM, FN = C::FN, W = 32 * FN, Q = W / 4;      // columns, 16-byte pieces of an LDS row
   constexpr int LR = (kPair ? W / 2 : W) / E, RI = 64 / LR, N = 32 / RI;   // lanes a row, rows at a time, times
@@ -423,11 +426,7 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
   const int wm = wave % C::WGM, wn = wave / C::WGM;
   f32x4* const st = reinterpret_cast<f32x4*>(lds + C::STAGE + wave * C::EPI);
   const int c0 = (lane % LR) * E, row0 = wm * FM * 32 + lane / LR, col0 = wn * (kPair ? W / 2 : W) + c0;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    decltype(fetch(0, 0)) pre[N];
-#pragma unroll
-    for (int n = 0; n < N; ++n) pre[n] = fetch(row0 + 32 * i + n * RI, col0);
+  auto turn = [&](int i) {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -436,19 +435,33 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
             f32x4{(float)acc[i][j][4 * q], (float)acc[i][j][4 * q + 1], (float)acc[i][j][4 * q + 2], (float)acc[i][j][4 * q + 3]};
     __builtin_amdgcn_wave_barrier();
     if (i == 0) all_landed();
+  };
+  auto rows = [&](int i, int n, const auto& pre) {
+    const int r = lane / LR + n * RI;
+    float v[E], u[E];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int r = lane / LR + n * RI;
-      float v[E], u[E];
+    for (int e = 0; e < E; e += 4) {
+      const f32x4 x = st[r * Q + (((c0 + e) / 4) ^ (r & (Q - 1)))];
+      f32x4 y = x;
+      if constexpr (kPair) y = st[r * Q + ((8 + (c0 + e) / 4) ^ (r & (Q - 1)))];
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const f32x4 x = st[r * Q + (((c0 + e) / 4) ^ (r & (Q - 1)))];
-        f32x4 y = x;
-        if constexpr (kPair) y = st[r * Q + ((8 + (c0 + e) / 4) ^ (r & (Q - 1)))];
+      for (int z = 0; z < 4; ++z) v[e + z] = x[z], u[e + z] = y[z];
+    }
+    emit(row0 + 32 * i + n * RI, col0, v, u, pre);
+  };
 #pragma unroll
-        for (int z = 0; z < 4; ++z) v[e + z] = x[z], u[e + z] = y[z];
-      }
-      emit(row0 + 32 * i + n * RI, col0, v, u, pre[n]);
+  for (int i = 0; i < FM; ++i) {
+    if constexpr (kWhole) {
+      decltype(fetch(0, 0)) pre[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) pre[n] = fetch(row0 + 32 * i + n * RI, col0);
+      turn(i);
+#pragma unroll
+      for (int n = 0; n < N; ++n) rows(i, n, pre[n]);
+    } else {
+      turn(i);
+#pragma unroll 1
+      for (int n = 0; n < N; ++n) rows(i, n, fetch(row0 + 32 * i + n * RI, col0));
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -458,7 +471,7 @@ struct Nothing {};
 // Workgroup b takes tiles b, b + grid, ... of `total` (some past the last of ragged groups).  The next tile's first stage
 // is on its way while this one's results are stored.
 // P: M (products), kADown, kBDown, kPair, E; groups(), what is looked up once for place(that, t), a tile's Place with g (-1:
-// none) and nk (stages); source(place) with load, ragged and clear; fetch(place, row, col) and
+// none), nk (stages) and whole; source(place) with load, ragged and clear; fetch(place, row, col) and
 // emit(place, row, col, v, u, what fetch gave).
 template <class C, class P>
 __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
@@ -486,9 +499,16 @@ __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
       src = p.template source<C>(nxt, wave, lane);
       if (nxt.nk > 0) send_stage<C>(src, 0, ring, wave);
     }
-    tile_emit<C, P::E, P::kPair>(
-        tile_lds, acc, [&](int row, int col) { return p.fetch(cur, row, col); },
-        [&](int row, int col, const float (&v)[P::E], const float (&u)[P::E], const auto& pre) { p.emit(cur, row, col, v, u, pre); });
+    auto store = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+      tile_emit<C, P::E, P::kPair, kWhole>(
+          tile_lds, acc, [&](int row, int col) { return p.template fetch<kWhole>(cur, row, col); },
+          [&](int row, int col, const float (&v)[P::E], const float (&u)[P::E], const auto& pre) {
+            p.template emit<kWhole>(cur, row, col, v, u, pre);
+          });
+    };
+    if (cur.whole) store(std::true_type{});
+    else store(std::false_type{});
     if (nxt.g < 0) return;
     cur = nxt;
   }
@@ -594,7 +614,7 @@ __global__ void __launch_bounds__(256, 4) few_kernel(P p) {
   }
   const float v[4] = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
   const float u[4] = {(float)t[0], (float)t[1], (float)t[2], (float)t[3]};
-  p.emit(c, lane & 15, (P::kPair ? 0 : 16 * wave) + 4 * quarter, v, u, Nothing{});
+  p.template emit<false>(c, lane & 15, (P::kPair ? 0 : 16 * wave) + 4 * quarter, v, u, Nothing{});
 }
 
 using Tile256 = TileShape<256, 256, 2, 4>;

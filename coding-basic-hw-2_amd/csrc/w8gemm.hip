@@ -11,6 +11,7 @@ namespace {
 
 struct Place {
   int g, m0, m_end, n0, nk;
+  bool whole;   // every row and column of the tile exists
 };
 
 // c = (s sa) sb, or act of it times the same of the second weights
@@ -33,7 +34,8 @@ struct Product {
     if (s.g < 0) return Place{-1};
     int tm, tn;
     tile_raster(t, ceil_div(s.hi - s.lo, C::BM), nt, tm, tn);
-    return Place{s.g, s.lo + tm * C::BM, s.hi, tn * width, ceil_div(p.k, 128)};
+    const int m0 = s.lo + tm * C::BM, n0 = tn * width;
+    return Place{s.g, m0, s.hi, n0, ceil_div(p.k, 128), m0 + C::BM <= s.hi && n0 + width <= p.n};
   }
   template <class C>
   struct Src {
@@ -64,12 +66,15 @@ struct Product {
     return FewRows{bytes(p.a) + c.m0 * p.lda, {bytes(p.b) + b0, kPair ? bytes(p.b_up) + b0 : bytes(p.b) + b0 + 16 * p.ldb},
                    (c.m_end - c.m0 - 1) * p.lda + end, {left, kPair ? left : left - 16 * p.ldb}, (uint32_t)i * (uint32_t)p.lda, {vb, vb}, p.k};
   }
-  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const { return {}; }
-  template <int E>
+  template <bool kWhole>
+  __device__ __forceinline__ Nothing fetch(const Place&, int, int) const {
+    return {};
+  }
+  template <bool kWhole, int E>
   __device__ __forceinline__ void emit(const Place& c, int row, int col, const float (&v)[E], const float (&u)[E], Nothing) const {
     const int64_t r = c.m0 + row, j = c.n0 + col;
-    if (r >= c.m_end || j >= p.n) return;
-    const int ok = p.n - (int)j;
+    if (!kWhole && (r >= c.m_end || j >= p.n)) return;
+    const int ok = kWhole ? E : p.n - (int)j;
     const int64_t sj = c.g * p.b_scales_stride + j;
     const float sa = p.a_scales[r];
     float o[E], s[E];

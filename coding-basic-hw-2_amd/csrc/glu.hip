@@ -48,6 +48,7 @@ struct Up {
   ggemm_glu_t p;
   T* h;
   int64_t ldh;
+  bool stream;   // gate and up
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_ff, BN / 2)); }
@@ -57,7 +58,6 @@ struct Up {
   }
   template <class C>
   struct Src {
-    static constexpr int kTouches = 0;
     Along<C, C::BM> a;
     Along<C, C::BN, true> b;
     __device__ __forceinline__ void prepare(int kt, int wave) {
@@ -109,10 +109,10 @@ struct Up {
     float g[E], w[E], o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) g[e] = v[e], w[e] = u[e], o[e] = act_value<ACT>(v[e]) * u[e];
-    store_some(h + r * ldh + j, ok, o);
+    store_some(h + r * ldh + j, ok, o, true);
     if (p.gate) {
-      store_some(static_cast<T*>(p.gate) + r * p.ldg + j, ok, g);
-      store_some(static_cast<T*>(p.up) + r * p.ldg + j, ok, w);
+      store_some(static_cast<T*>(p.gate) + r * p.ldg + j, ok, g, stream);
+      store_some(static_cast<T*>(p.up) + r * p.ldg + j, ok, w, stream);
     }
   }
 };
@@ -128,6 +128,7 @@ struct DownProduct {
   ggemm_glu_t p;
   const T* h;
   int64_t ldh;
+  bool stream;
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_model, BN)); }
@@ -137,7 +138,6 @@ struct DownProduct {
   }
   template <class C>
   struct Src {
-    static constexpr int kTouches = 0;
     Along<C, C::BM> a;
     Along<C, C::BN> b;
     __device__ __forceinline__ void prepare(int kt, int wave) {
@@ -177,7 +177,7 @@ struct DownProduct {
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = v[e];
-    store_some(static_cast<T*>(p.y) + r * p.ldy + j, kWhole ? E : p.d_model - (int)j, o);
+    store_some(static_cast<T*>(p.y) + r * p.ldy + j, kWhole ? E : p.d_model - (int)j, o, stream);
   }
 };
 
@@ -203,22 +203,11 @@ struct Hidden {
   }
   template <class C>
   struct Src {
-    // The tile's lines of gate and up, BM rows of BN 16-bit values each, 64 lines a wave at a time.  Without, the epilogue waits for
-    // HBM: 16 groups of 2048 rows, (2048, 4096), 922 us; with gate and up left out 632.
-    static constexpr int ROW_LINES = C::BN / 64, kTouches = 2 * C::BM * ROW_LINES / 64 / C::NW;
     Along<C, C::BM> a;
     Down<C, C::BN> b;
-    const uint8_t *gate, *up;   // of the tile's first row and column
-    int64_t pitch;
-    int rows, bytes;            // that exist of the tile: rows, bytes of a row
     __device__ __forceinline__ void prepare(int kt, int wave) {
       a.prepare(kt, wave);
       b.prepare(b.base, kt);
-    }
-    __device__ __forceinline__ void touch(int part, uint32_t scrap, int wave, int lane) const {
-      const int l = 64 * (part * C::NW + wave) + lane, r = l / ROW_LINES % C::BM, c = 128 * (l % ROW_LINES);
-      const uint8_t* const p = (l / ROW_LINES / C::BM ? up : gate) + min(r, rows - 1) * pitch + min(c, bytes - 2);
-      touch_lines(reinterpret_cast<const void*>((uintptr_t)p & ~(uintptr_t)3), scrap);
     }
     __device__ __forceinline__ bool ragged(int kt) const { return a.ragged(kt); }
     __device__ __forceinline__ void clear(int kt, uint8_t* slot) const { a.clear(kt, slot); }
@@ -227,9 +216,7 @@ struct Hidden {
   __device__ __forceinline__ Src<C> source(const Place& c, int wave, int lane) const {
     const int64_t py = 2 * lddy;
     return Src<C>{Along<C, C::BM>(bytes_of(dy) + c.m0 * py, nullptr, py, c.m_end - c.m0, 2 * p.d_model, wave, lane, InOrder{(uint32_t)py}),
-                  Down<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0), 2 * p.ldd, p.d_model, p.d_ff - c.n0, wave, lane),
-                  bytes_of(p.gate) + 2 * (c.m0 * p.ldg + c.n0), bytes_of(p.up) + 2 * (c.m0 * p.ldg + c.n0), 2 * p.ldg, c.m_end - c.m0,
-                  2 * (p.d_ff - c.n0)};
+                  Down<C, C::BN>(bytes_of(p.w_down) + 2 * (c.g * p.d_stride + c.n0), 2 * p.ldd, p.d_model, p.d_ff - c.n0, wave, lane)};
   }
   struct Kept {
     Run<T, E> g, u;
@@ -264,10 +251,10 @@ struct Hidden {
       g[e] = live ? v[e] * w * fmaf(g[e], dq, q) : 0.0f;
     }
     if (dg) {
-      store_some(dg + r * ldh + j, ok, g);
-      store_some(du + r * ldh + j, ok, u);
+      store_some(dg + r * ldh + j, ok, g, true);
+      store_some(du + r * ldh + j, ok, u, true);
     }
-    if (h) store_some(h + r * ldh + j, ok, o);
+    if (h) store_some(h + r * ldh + j, ok, o, true);
   }
 };
 
@@ -284,6 +271,7 @@ struct InputGrad {
   int64_t lddx;
   const T *dg, *du;
   int64_t ldh;
+  bool stream;
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_model, BN)); }
@@ -293,7 +281,6 @@ struct InputGrad {
   }
   template <class C>
   struct Src {
-    static constexpr int kTouches = 0;
     Along<C, C::BM> a;   // base2: dup
     Down<C, C::BN> b;
     const uint8_t* b2;
@@ -325,7 +312,7 @@ struct InputGrad {
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = v[e];
-    store_some(static_cast<T*>(dx) + r * lddx + j, kWhole ? E : p.d_model - (int)j, o);
+    store_some(static_cast<T*>(dx) + r * lddx + j, kWhole ? E : p.d_model - (int)j, o, stream);
   }
 };
 
@@ -347,6 +334,7 @@ struct WeightGrad {
   const T *dg, *du, *h;
   int64_t ldh;
   int first_of;   // 0: all three, 2: dWd only
+  bool stream;
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ int groups() const { return 0; }
@@ -371,7 +359,6 @@ struct WeightGrad {
   }
   template <class C>
   struct Src {
-    static constexpr int kTouches = 0;
     Down<C, C::BM> a;
     Down<C, C::BN> b;
     __device__ __forceinline__ void prepare(int kt, int) {
@@ -410,7 +397,7 @@ struct WeightGrad {
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = v[e];
     }
-    store_some(out, kWhole ? E : n - j, o);
+    store_some(out, kWhole ? E : n - j, o, stream);
   }
 };
 
@@ -470,7 +457,7 @@ bool args_ok(const ggemm_glu_t* p) {
   if ((!p->x && !(p->index && p->x_rows == 0)) || !aligned(p->x, 16)) return false;
   return p->w_gate && p->w_up && p->w_down && aligned(p->w_gate, 16) && aligned(p->w_up, 16) && aligned(p->w_down, 16);
 }
-int64_t ld_hidden(const ggemm_glu_t& p) { return (int64_t)align_up((size_t)p.d_ff, 8); }
+int64_t ld_hidden(const ggemm_glu_t& p) { return (int64_t)align_up((size_t)p.d_ff, 32); }   // rows of whole runs of 64 bytes
 size_t hidden_bytes(const ggemm_glu_t& p) { return align_up((size_t)p.rows * ld_hidden(p) * 2, 256); }
 // The most tiles that a launch over rows or weights can have, in the smallest shape that it may take.
 bool tiles_fit(const ggemm_glu_t& p, bool weights) {
@@ -495,8 +482,9 @@ int glu(const ggemm_glu_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
     constexpr int D = decltype(dt)::value;
     using T = typename Elem<D>::T;
     T* const h = static_cast<T*>(ws);
-    run_rows(Up<D, decltype(act)::value>{*p, h, ld_hidden(*p)}, p->d_ff, s);
-    run_rows(DownProduct<D>{*p, h, ld_hidden(*p)}, p->d_model, s);
+    const bool kept = whole_runs(p->gate, 2 * p->ldg) && whole_runs(p->up, 2 * p->ldg);
+    run_rows(Up<D, decltype(act)::value>{*p, h, ld_hidden(*p), kept}, p->d_ff, s);
+    run_rows(DownProduct<D>{*p, h, ld_hidden(*p), whole_runs(p->y, 2 * p->ldy)}, p->d_model, s);
   }); }); });
 }
 
@@ -536,7 +524,7 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
         run_rows(Hidden<D, decltype(act)::value>{*p, d->dy, d->lddy, gu ? dg : nullptr, gu ? du : nullptr, d->dw_down ? h : nullptr, ldh},
                  p->d_ff, s);
       });
-      if (d->dx) run_rows(InputGrad<D>{*p, d->dx, d->lddx, dg, du, ldh}, p->d_model, s);
+      if (d->dx) run_rows(InputGrad<D>{*p, d->dx, d->lddx, dg, du, ldh, whole_runs(d->dx, 2 * d->lddx)}, p->d_model, s);
     }
     if (!d->dw_gate && !d->dw_down) return;
     const int matrices = (d->dw_gate ? 2 : 0) + (d->dw_down ? 1 : 0), from = d->dw_gate ? 0 : 2;
@@ -555,8 +543,13 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
       grad.dy = yg;
       rows.ldx = grad.lddy = ld_model(*p);
     }
+    auto runs = [&](const void* w, int64_t ld, int64_t stride) {
+      const int64_t es = elem_bytes(d->dw_dtype);
+      return !w || (whole_runs(w, ld * es) && (p->groups == 1 || stride * es % 64 == 0));
+    };
+    const bool stream = runs(d->dw_gate, d->lddw, d->dw_stride) && runs(d->dw_up, d->lddw, d->dw_stride) && runs(d->dw_down, d->lddd, d->dd_stride);
     with_elem(d->dw_dtype, [&](auto wt) {
-      const WeightGrad<D, decltype(wt)::value> w{rows, grad, dg, du, h, ldh, from};
+      const WeightGrad<D, decltype(wt)::value> w{rows, grad, dg, du, h, ldh, from, stream};
       auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
       if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
       else run_tiles<Tile128>(w, tiles(128), s);

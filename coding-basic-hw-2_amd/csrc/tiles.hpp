@@ -143,8 +143,7 @@ struct TileShape {
   static constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;   // 1 KB pieces of A and B a wave brings
   static constexpr int EPI = 32 * 32 * FN * 4;               // epilogue bytes per wave, from the second slot on
-  static constexpr int SCRAP = STAGE + (NW * EPI > STAGE ? NW * EPI : STAGE);   // where touched bytes go, 256 a wave
-  static constexpr int SMEM = SCRAP + 256 * NW;
+  static constexpr int SMEM = STAGE + (NW * EPI > STAGE ? NW * EPI : STAGE);
   static constexpr int PER_CU = 163840 / SMEM;               // workgroups, as many as LDS holds
   static constexpr int WAVES = PER_CU * NW / 4;              // per SIMD
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && NW % 2 == 0, "pieces");
@@ -178,12 +177,6 @@ struct Window {
                      __builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(r) : "memory");
   }
 };
-// 64 lanes' 4 bytes each, only to have their lines in the caches when they are wanted: they land in LDS unread, so that
-// no register waits for them.
-__device__ __forceinline__ void touch_lines(const void* p, uint32_t scrap) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane((int)scrap)), "v"(p)
-               : "memory");
-}
 // This wave's transfers to LDS landed.
 __device__ __forceinline__ void all_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // This wave's LDS operations done; then every wave's.
@@ -398,10 +391,6 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
           }
         }
       }
-    if constexpr (S::kTouches > 0) {   // in the last stages but one, for the epilogue
-      const int part = nk - 2 - kt;
-      if (part >= 0 && part < S::kTouches) src.touch(part, ring + C::SCRAP + 256 * wave, wave, lane);
-    }
     read(0, 0, sn);   // after the last stage: what an earlier one left, not used
     products(1);
     pin();
@@ -529,19 +518,29 @@ __device__ __forceinline__ void load_some(const T* p, int ok, float (&v)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) v[e] = (float)w.x[e];
 }
+// stream: non-temporally, where rows are whole runs of 64 bytes (whole_runs): forward and gradients of 4096 tokens, 2 of 16 experts
+// (1024, 2048), 162 -> 156 and 386 -> 367 us, the launches that read the results next included; other rows are stored faster
+// by way of the caches (1237 tokens, 3 of 23 experts (1001, 1371), 73 and 76).
 template <class T, int N>
-__device__ __forceinline__ void store_some(T* p, int ok, const float (&v)[N]) {
+__device__ __forceinline__ void store_some(T* p, int ok, const float (&v)[N], bool stream) {
   if (ok >= N) {
     Run<T, N> w;
 #pragma unroll
     for (int e = 0; e < N; ++e) w.x[e] = (T)v[e];
-    w.template store<false>(p);
+    if (stream) {
+      asm volatile("");   // else the compiler makes one ordinary store of both
+      w.template store<true>(p);
+      asm volatile("");
+    } else {
+      w.template store<false>(p);
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
       if (e < ok) p[e] = (T)v[e];
   }
 }
+inline bool whole_runs(const void* p, int64_t pitch_bytes) { return aligned(p, 64) && pitch_bytes % 64 == 0; }
 
 // Few rows: a workgroup computes 16 rows x 32 columns (kPair: 16 columns of both products); its 4 waves take every fourth
 // run of 256 bytes of the inner dimension straight from memory into registers and join their sums in LDS in order.

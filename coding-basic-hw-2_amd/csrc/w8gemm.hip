@@ -23,6 +23,7 @@ struct Product {
   static constexpr bool kADown = false, kBDown = false, kPair = ACT != 0;
   static constexpr int E = 8;
   ggemm_w8_gemm_t p;
+  bool stream;
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.m}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.n, kPair ? BN / 2 : BN)); }
@@ -39,7 +40,6 @@ struct Product {
   }
   template <class C>
   struct Src {
-    static constexpr int kTouches = 0;
     Along<C, C::BM> a;
     Along<C, C::BN, kPair> b;
     __device__ __forceinline__ void prepare(int kt, int wave) {
@@ -86,7 +86,7 @@ struct Product {
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = act_value<ACT>(o[e]) * (u[e] * sa * s[e]);
     }
-    store_some(static_cast<T*>(p.c) + r * p.ldc + j, ok, o);
+    store_some(static_cast<T*>(p.c) + r * p.ldc + j, ok, o, stream);
   }
 };
 
@@ -134,8 +134,9 @@ int w8_gemm(const ggemm_w8_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s) 
   if (tiles_of(*p, 64, 128) >= (1 << 23)) return GGEMM_ERR_INVALID;
   return launch([&] { with_elem(p->dtype, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (!p->act) run(Product<D, 0>{*p}, s);
-    else with_act(p->act, [&](auto act) { run(Product<D, decltype(act)::value>{*p}, s); });
+    const bool stream = whole_runs(p->c, p->ldc * elem_bytes(D));
+    if (!p->act) run(Product<D, 0>{*p, stream}, s);
+    else with_act(p->act, [&](auto act) { run(Product<D, decltype(act)::value>{*p, stream}, s); });
   }); });
 }
 

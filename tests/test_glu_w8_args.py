@@ -5,9 +5,6 @@ import ctypes as C
 import pytest
 
 import ggemm as G
-from conftest import card_present
-
-pytestmark = pytest.mark.skipif(card_present(), reason="made-up addresses: run where no card can follow them")
 
 P = 0x7f0000000000      # an address, aligned to everything
 BIG = 1 << 50

@@ -94,7 +94,9 @@ struct GroupTiles {
   __device__ __forceinline__ GroupTiles(const RowGroups& p, int g0, int nt) {
     const int lane = threadIdx.x & 63;
     p.span(min(g0 + lane, p.groups - 1), lo, hi);
-    own = sum = g0 + lane < p.groups ? ceil_div(max(hi - lo, 0), TM) * nt : 0;
+    // A launch has fewer than 2^23 tiles, so a group may count as 2^24: offsets that are not ascending can name any rows many
+    // times over, and their sums must not run over either.
+    own = sum = g0 + lane < p.groups ? min(ceil_div(max(hi - lo, 0), TM), (1 << 24) / nt + 1) * nt : 0;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int up = __shfl_up(sum, d);

@@ -37,8 +37,10 @@ extern "C" {
 #define GGEMM_GLU_MAX_GROUPS 4096
 #define GGEMM_GLU_MAX_LD (1 << 22)     /* leading dimensions of x, dy and the weights, and d_model, d_ff */
 
-/* Alignment: x, the weights and dy 16 bytes, their leading dimensions and strides multiples of 8; gate, up, y, dx and the
- * weights' gradients their type's.  Any d_model and d_ff from 1 on.  With an index, x_rows ldx < 2^30. */
+/* Alignment: x, the weights and dy 16 bytes, their leading dimensions and strides multiples of 8 (of a row of them, what lies up
+ * to the next 16 bytes may be read, to no effect); gate, up, y, dx and the weights' gradients their type's.  Any d_model and
+ * d_ff from 1 on.  With an index, x_rows ldx < 2^30.  Calls of 2^23 or more tiles (64 x 64 of y and gate, 128 x 128 of the
+ * weights' gradients) are refused. */
 typedef struct {
   int groups, rows;              /* rows: of y, gate, up and index */
   int d_model, d_ff;
@@ -68,7 +70,8 @@ int ggemm_glu(const ggemm_glu_t* p, void* workspace, size_t workspace_bytes, hip
  *   dWg_e  = dgate^T x_r + dw_beta dWg_e   of dw_dtype (any of the three), as dWu_e = dup^T x_r
  *   dWd_e  = dy^T h + dw_beta dWd_e        and these too are written for groups without rows
  * Rows whose index lies outside [0, x_rows) count as zeros throughout, dy among them, and get dx = 0.
- * dx may be NULL, dw_gate and dw_up together, and dw_down: what is not wanted is not computed.  With dw_beta == 0 the
+ * dx may be NULL, dw_gate and dw_up together, and dw_down: what is not wanted is not computed.  Results must not overlap the
+ * inputs or each other.  With dw_beta == 0 the
  * gradients of the weights are not read.  The workspace also goes by whether index is NULL. */
 typedef struct {
   const void* dy; int64_t lddy;

@@ -53,13 +53,15 @@ int ggemm_w8_dequantize(const ggemm_w8_dequant_t* d, hipStream_t stream);
 
 /* Grouped products: for the rows r of group e, offsets[e] <= r < offsets[e + 1],
  *   s[r, j] = sum_i a[r, i] b_e[j, i]           a whole number, exact
- *   v[r, j] = (s a_scales[r]) b_scales_e[j]     in 32 bits
+ *   v[r, j] = (s a_scales[r]) b_scales_e[j]     in 32-bit floating point (s is rounded to it first)
  *   act 0:    c[r, j] = v
  *   GGEMM_SILU, GGEMM_GELU, GGEMM_GELU_TANH (ggemm_glu.h): c[r, j] = act(v) w, with w the same of b_up and its scales
  * rounded once to c's type.  A m x k, B_e n x k (b_stride elements apart, its scales b_scales_stride; b_up alike), C m x n.
  * Rows in no group are not written.  Offsets are read on the device and clamped to [0, m]: wrong ones give wrong results
  * but no access out of bounds.  Every int8 value may occur.  C must not overlap the inputs.
- * Alignment: a, b, b_up 16 bytes, their leading dimensions and strides multiples of 16; scales 4 bytes; C its type's. */
+ * Alignment: a, b, b_up 16 bytes, their leading dimensions and strides multiples of 16; scales 4 bytes; C its type's.
+ * Of a row of a, b, b_up, what lies up to the next 16 bytes may be read, to no effect.  Products of 2^23 or more tiles (64 x 128 of
+ * C, 64 x 64 of a pair) are refused. */
 typedef struct {
   int groups;
   int m, n, k;

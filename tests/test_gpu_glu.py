@@ -328,3 +328,32 @@ def test_large_values():
         assert bool(torch.isfinite(got["dx"]).all()) and bool(torch.isfinite(got["dwg"]).all())
         want = b.backward64(gate.double().clamp(-1e4, 1e4), u.double())   # the same slopes
         assert R.worst(got["dwg"].view(1, 64, 64), want["dwg"][0], want["dwg"][1] + 1e-3 * want["dwg"][0].abs()) <= 1.0
+
+
+def test_long_rows():
+    """Rows of x, dy and the weights 2^23 bytes apart: offsets past 32 bits from the 512th row on, and past 31 within a tile's."""
+    say("long rows")
+    for rows, d, f in ((300, 40, 24), (9, 24, 300), (600, 40, 40)):
+        b = R.Block([0, rows], rows, d, f, seed=20)
+        for n in ("x", "dy", "wg", "wu", "wd"):
+            t = getattr(b, n)
+            wide = torch.empty(t.shape[0], G.GLU_MAX_LD, dtype=t.dtype, device="cuda")
+            wide[:, :t.shape[1]] = t
+            setattr(b, n, wide)
+        check_forward(b)
+        check_backward(b, *kept(b))
+        del b
+
+
+def test_offsets_that_name_rows_many_times():
+    """Not ascending: results of rows named twice are anybody's, but nothing outside the results is touched and the calls end."""
+    say("offsets over and over")
+    for rows, groups in ((40, 9), (3000, 201)):
+        b = R.Block([0 if g % 2 == 0 else rows for g in range(groups + 1)], rows, 16, 24, seed=21)
+        y, gate, u, dx = (torch.full((rows + 64, w), 7.0, dtype=torch.bfloat16, device="cuda") for w in (16, 24, 24, 16))
+        R.run_forward(b.struct(gate[32:], u[32:], y[32:]))
+        dwg, dwu, dwd = b.out(groups * 24, 16, "f32"), b.out(groups * 24, 16, "f32"), b.out(groups * 16, 24, "f32")
+        R.run_backward(b.struct(gate[32:], u[32:], None), R.grad_struct(b, dx[32:], dwg, dwu, dwd))
+        torch.cuda.synchronize()
+        for t in (y, gate, u, dx):
+            assert bool((t[:32] == 7.0).all()) and bool((t[rows + 32:] == 7.0).all())

@@ -250,6 +250,43 @@ def test_groups_and_offsets():
     assert torch.equal(one.run(None), one.run([0, 50]))
 
 
+def test_offsets_that_name_rows_many_times():
+    """Not ascending: results of rows named twice are anybody's, but nothing outside C is touched and the call ends."""
+    say("offsets over and over")
+    for m, groups in ((40, 9), (2000, 300), (50000, 2001)):
+        n, k = 40, 32
+        o = Operands(16, m, n, k, groups, False)
+        store = torch.full((m + 64, n), 7.0, device="cuda")
+        off = torch.tensor([0 if g % 2 == 0 else m for g in range(groups + 1)], dtype=torch.int32, device="cuda")
+        p = G.W8Gemm(groups, m, n, k, G.F32, 0, o.a.data_ptr(), o.a.stride(0), o.sa.data_ptr(), o.b.data_ptr(), None, o.b.stride(0),
+                     n * o.b.stride(0), o.sb.data_ptr(), None, n, off.data_ptr(), store[32:].data_ptr(), n)
+        G.check(G.lib().ggemm_w8_gemm(C.byref(p), None, 0, stream()), "ggemm_w8_gemm")
+        torch.cuda.synchronize()
+        assert bool((store[:32] == 7.0).all()) and bool((store[m + 32:] == 7.0).all())
+
+
+def test_offsets_past_32_bits():
+    """Weights of more than 4 GiB with rows in the first and the last group, and operands whose rows lie 2^23 bytes apart."""
+    say("large weights")
+    m, n, k, groups = 70, 8192, 8192, 72
+    o = Operands(17, m, 1, k, 1, False)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    o.n, o.groups = n, groups
+    o.b = torch.randint(-128, 128, (groups * n, k), dtype=torch.int8, device="cuda", generator=gen)
+    o.sb = torch.exp(torch.randn(groups * n, device="cuda", generator=gen)) / 1e6
+    check(o, [0] + [30] * (groups - 1) + [m], "f32", None)
+    del o
+    say("long rows")
+    for m, n in ((300, 40), (9, 300), (300, 300)):
+        o = Operands(18, m, n, 100, 1, False)
+        for name, rows in (("a", m), ("b", n)):
+            wide = torch.empty(rows, G.W8_MAX_LD, dtype=torch.int8, device="cuda")
+            wide[:, :112] = getattr(o, name)[:, :112]
+            setattr(o, name, wide)
+        check(o, [0, m], "bf16", None)
+
+
 def test_no_inner_dimension():
     say("k = 0")
     o = Operands(8, 20, 40, 0, 2, True)

@@ -116,6 +116,19 @@ def test_large(rows, groups, d, f, gather):
     check_backward(b, gate, u, dw_dtype="bf16" if gather else "f32")
 
 
+@pytest.mark.parametrize("rows,groups,d,f", [(8192, 1, 4096, 2048), (8200, 3, 4096, 2056), (3000, 2, 1500, 1000)])
+@pytest.mark.parametrize("dtype,act", [("f16", "gelu_tanh"), ("bf16", "gelu")])
+def test_every_product_in_large_tiles(rows, groups, d, f, dtype, act):
+    say("large tiles", rows, groups, d, f, dtype, act)
+    rng = np.random.default_rng(rows)
+    b = R.Block(cut(rng, rows, groups, 0.0), rows, d, f, dtype, act, seed=22)
+    check_forward(b)
+    gate, u = kept(b)
+    # gradients of 1 / 16, so that sums over 8192 rows of f16 factors stay within its range
+    b.dy *= 0.0625
+    check_backward(b, gate, u, dw_dtype=dtype)
+
+
 def test_rows_of_no_group_are_left_alone():
     say("rows of no group")
     b = R.Block([3, 20, 20, 300], 350, 72, 136, seed=3)      # rows 0 .. 2 and 300 .. 349

@@ -46,7 +46,7 @@ def values(gen, rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4096), (3, 7), (5, 64), (17, 1000), (257, 33), (64, 8192), (9, 12345), (2, 131071),
-                                       (4000, 520), (1000, 2049), (300, 16384)])
+                                       (4000, 520), (1000, 2049), (300, 16384), (3000, 1500), (2100, 4000), (5000, 3999)])
 def test_quantise(rows, cols, dtype):
     say("quantise", rows, cols, dtype)
     gen = torch.Generator(device="cuda")
@@ -56,6 +56,17 @@ def test_quantise(rows, cols, dtype):
     wide = torch.zeros(rows, cols + 5, dtype=x.dtype, device="cuda")     # rows at any element
     wide[:, 1:cols + 1] = x
     same(quantise(wide[:, 1:cols + 1], ldq=cols + 3, shift=1), R.quantise64(x))
+
+
+@pytest.mark.parametrize("rows,cols", [(20000, 4096), (9000, 8200), (70000, 1001), (300000, 250)])
+def test_quantise_large(rows, cols):
+    """More integers than are stored by way of the caches."""
+    say("quantise large", rows, cols)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows)
+    for dtype in ("f32", "bf16"):
+        x = values(gen, rows, cols, dtype)
+        same(quantise(x), R.quantise64(x))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -222,7 +233,7 @@ def test_product(m, n, k, groups, act):
 def test_result_types_and_the_last_activation():
     say("types")
     rng = np.random.default_rng(5)
-    for m, n, k, groups in ((7, 40, 96, 2), (200, 136, 264, 3), (1500, 1200, 160, 2)):
+    for m, n, k, groups in ((7, 40, 96, 2), (200, 136, 264, 3), (1500, 1200, 160, 2), (3000, 2600, 136, 2), (8200, 4100, 200, 3)):
         o = Operands(m, m, n, k, groups, True)
         for dtype in ("f32", "bf16", "f16"):
             for act in (None, "gelu_tanh"):

@@ -29,7 +29,8 @@ extern "C" {
  *   scales[i] = max(a / 127, 2^-126), a = max |x| of the row, the quotient rounded to 32 bits
  *   q[i, j]   = x / scales[i] to the nearest whole number, ties to the even one (the quotient itself, not a rounding of it)
  * A row with a NaN or an Inf gets a NaN scale and q = 0.  Columns of q past cols are not written.  Any alignment of x and q
- * that suits their types; as operands of products, q has to be 16-byte aligned with ldq a multiple of 16. */
+ * that suits their types; as operands of products, q has to be 16-byte aligned with ldq a multiple of 16.  q and scales must
+ * not overlap x. */
 typedef struct {
   int rows, cols;
   int dtype;                     /* of x: GGEMM_F32, GGEMM_BF16, GGEMM_F16 */
@@ -41,7 +42,7 @@ typedef struct {
 } ggemm_w8_quant_t;
 int ggemm_w8_quantize(const ggemm_w8_quant_t* q, hipStream_t stream);
 
-/* y[i, j] = q[i, j] scales[i], in 32 bits, then rounded to y's type. */
+/* y[i, j] = q[i, j] scales[i], in 32 bits, then rounded to y's type.  y must not overlap q and scales. */
 typedef struct {
   int rows, cols;
   int dtype;                     /* of y */

@@ -136,12 +136,14 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 // 64 lanes' 16 (or 4) bytes at base + off to LDS byte address lds + 16 (4) lane.  Written as assembly so that the
-// compiler does not wait for all of them before the next LDS read; the waits are stage_wait's.
+// compiler does not wait for all of them before the next LDS read; the waits are stage_wait's.  s_nop 3: with the move, the five
+// wait states that a base written by a vector instruction (the compiler may have kept it in a lane) needs before a memory
+// instruction reads it; the compiler's own check does not see in here.
 __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void dma4(const uint8_t* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 // This wave's transfers to LDS landed.
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }

@@ -49,8 +49,8 @@ __device__ __forceinline__ uint32_t largest_bits(uint32_t m) {
 // x / s to the nearest whole number, ties to even, in the low byte: s = max(fl(a / 127), 2^-126), |x| <= a, r from
 // row_factor.  Adding 1.5 2^23 to x r in one multiply-add rounds once, to a whole number.
 // r = fl(1 / s), so x r is off x / s by 2 parts in 2^24 at most and the number by one at most, next to a half.
-// The rest x - q s is exact (a multiple of the smaller unit of x and s, about s at most), and comparing it with s / 2,
-// exact too, decides.
+// The rest x - q s is exact (a multiple of the smaller unit of x and s, about s at most), and comparing twice it with s
+// decides, exact too (s / 2 would lose a bit where s is below 2^-125; twice the rest is below 2^123).
 // bf16 needs no such step.  With x and a of 8 bits, |254 x - (2 n + 1) a| is either a unit of x or more, i.e.
 // 127 x / a lies a part of 7 10^-6 or more beside the half, where the roundings of s and r come to 2.4 10^-7; or 0:
 // then a is 127 or 254 times a power of two, s and r are powers of two and all is exact, or x = a / 2, n = 63, and for
@@ -71,10 +71,10 @@ template <int D>
 __device__ __forceinline__ uint32_t whole_quotient(float x, float s, float r) {
   const float big = fmaf(x, r, kWhole);
   if constexpr (D == GGEMM_BF16) return __float_as_uint(big);
-  const float q = big - kWhole, rest = fmaf(-q, s, x), half = 0.5f * s;
+  const float q = big - kWhole, rest = fmaf(-q, s, x), twice = rest + rest;
   const uint32_t w = __float_as_uint(big), odd = w & 1u;
-  if (rest > half || (rest == half && odd)) return w + 1u;
-  if (rest < -half || (rest == -half && odd)) return w - 1u;
+  if (twice > s || (twice == s && odd)) return w + 1u;
+  if (twice < -s || (twice == -s && odd)) return w - 1u;
   return w;
 }
 template <int D>

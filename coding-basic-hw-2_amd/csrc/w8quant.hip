@@ -61,7 +61,8 @@ __device__ __forceinline__ float row_factor(float a, float s) {
   float r = 1.0f / s;
   if constexpr (D == GGEMM_BF16) {
     const float h = 0.5f * a;
-    const bool up = fmaf(-63.5f, s, h) >= 0.0f;   // x / s of 63.5 or more: 64
+    // h / s of 63.5 or more: 64.  a - 127 s is a whole number of 2^-149, so its sign is right (half of it can come out as zero).
+    const bool up = fmaf(-127.0f, s, a) >= 0.0f;
     // s is a power of two at its least, and r exact
     if (s > 0x1p-126f && fmaf(h, r, kWhole) - kWhole != (up ? 64.0f : 63.0f)) r = __uint_as_float(__float_as_uint(r) + (up ? 1u : ~0u));
   }

@@ -1,5 +1,5 @@
-"""Row quantisation next to halves (include/ggemm_w8.h) where 32-bit numbers run out of bits: rows whose scale lies just above
-the least one; bit for bit."""
+"""Row quantisation next to halves (include/ggemm_w8.h) where 32-bit numbers run out of bits: 32-bit rows whose scale lies just
+above the least one, and every 16-bit row maximum with every value below it; bit for bit."""
 import numpy as np
 import pytest
 import torch
@@ -36,3 +36,21 @@ def test_a_half_below_the_least_normal_number():
     say("one half")
     x = torch.tensor([[float.fromhex("0x1.6212b6p-119"), float.fromhex("0x1.8be48ap-121")]], device="cuda")
     assert quantise(x)[0].tolist() == [[127, 35]]
+
+
+def test_half_of_a_small_bf16_maximum():
+    """a = 222 2^-126, x = a / 2: x / s = 63.499999966, 63."""
+    say("bf16 half")
+    x = torch.tensor([[222 * 2.0 ** -126, 111 * 2.0 ** -126]], device="cuda").bfloat16()
+    assert quantise(x)[0].tolist() == [[127, 63]]
+
+
+@pytest.mark.parametrize("dtype,top", [("bf16", 0x7f80), ("f16", 0x7c00)])
+def test_every_16_bit_maximum_with_every_value(dtype, top):
+    """Rows: every positive finite maximum; columns: every value up to it (the maximum itself instead of larger ones)."""
+    say("every", dtype)
+    every = torch.arange(0, top, dtype=torch.int16, device="cuda")
+    for i in range(1, top, 1024):
+        a = torch.arange(i, min(i + 1024, top), dtype=torch.int16, device="cuda")
+        x = torch.minimum(every[None], a[:, None]).view(R.TORCH[dtype])      # positive values order as their bits
+        same(quantise(x), R.quantise64(x))

@@ -42,6 +42,12 @@ struct Picked {
   }
   __device__ __forceinline__ bool live(int r) const { return !index || at(r) >= 0; }
 };
+// Products over rows that an index may pick: results of rows of which it names none are stored as zeros, not as what zeros times
+// the weights give, which is NaN for an Inf.
+__device__ __forceinline__ int row_entry(const ggemm_glu_t& p, const Place& c, int row) {
+  return p.index && c.m0 + row < c.m_end ? p.index[c.m0 + row] : 0;
+}
+__device__ __forceinline__ bool names_row(const ggemm_glu_t& p, int entry) { return !p.index || (uint32_t)entry < (uint32_t)p.x_rows; }
 
 // h = act(x Wg^T) (x Wu^T), and gate and up where they are kept.  Both products in one tile: half the columns, twice the
 // weights, x read once (8192 x 4096 x 8192: 1000 us, 1.1 PFLOP/s; 4096 tokens, 2 of 16 experts (1024, 2048), all kept: 111 us, of
@@ -52,11 +58,14 @@ struct Up {
   using M = typename MmaOf<D>::M;
   using Place = ggemm::Place;
   static constexpr bool kADown = false, kBDown = false, kPair = true;
+  static constexpr bool kDead = true;
   static constexpr int E = 8;
   ggemm_glu_t p;
   T* h;
   int64_t ldh;
   bool stream;   // gate and up
+  __device__ __forceinline__ int entry(const Place& c, int row) const { return row_entry(p, c, row); }
+  __device__ __forceinline__ bool names(int e) const { return names_row(p, e); }
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_ff, BN / 2)); }
@@ -132,11 +141,14 @@ struct DownProduct {
   using M = typename MmaOf<D>::M;
   using Place = ggemm::Place;
   static constexpr bool kADown = false, kBDown = false, kPair = false;
+  static constexpr bool kDead = true;
   static constexpr int E = 8;
   ggemm_glu_t p;
   const T* h;
   int64_t ldh;
   bool stream;
+  __device__ __forceinline__ int entry(const Place& c, int row) const { return row_entry(p, c, row); }
+  __device__ __forceinline__ bool names(int e) const { return names_row(p, e); }
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_model, BN)); }
@@ -198,6 +210,7 @@ struct Hidden {
   using M = typename MmaOf<D>::M;
   using Place = ggemm::Place;
   static constexpr bool kADown = false, kBDown = true, kPair = false;
+  static constexpr bool kDead = false;
   static constexpr int E = 8;
   ggemm_glu_t p;
   const void* dy;
@@ -276,6 +289,7 @@ struct InputGrad {
   using M = typename MmaOf<D>::M;
   using Place = ggemm::Place;
   static constexpr bool kADown = false, kBDown = true, kPair = false;
+  static constexpr bool kDead = true;
   static constexpr int E = 8;
   ggemm_glu_t p;
   void* dx;
@@ -283,6 +297,8 @@ struct InputGrad {
   const T *dg, *du;
   int64_t ldh;
   bool stream;
+  __device__ __forceinline__ int entry(const Place& c, int row) const { return row_entry(p, c, row); }
+  __device__ __forceinline__ bool names(int e) const { return names_row(p, e); }
   __device__ __forceinline__ RowGroups rows() const { return RowGroups{p.offsets, p.groups, p.rows}; }
   template <int BM, int BN>
   __device__ __forceinline__ GroupTiles<BM> groups() const { return GroupTiles<BM>(rows(), 0, ceil_div(p.d_model, BN)); }
@@ -341,6 +357,7 @@ struct WeightGrad {
   using M = typename MmaOf<D>::M;
   using Place = WeightPlace;
   static constexpr bool kADown = true, kBDown = true, kPair = false;
+  static constexpr bool kDead = false;
   static constexpr int E = 8;
   ggemm_glu_t p;        // x and dy: one row for each of the call's rows
   ggemm_glu_grad_t d;

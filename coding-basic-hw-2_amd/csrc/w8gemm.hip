@@ -28,6 +28,7 @@ struct Product {
   using M = MmaI8;
   using Place = ggemm::Place;
   static constexpr bool kADown = false, kBDown = false, kPair = ACT != 0;
+  static constexpr bool kDead = false;
   static constexpr int E = 8;
   ggemm_w8_gemm_t p;
   bool stream;

@@ -56,7 +56,8 @@ typedef struct {
   void* y; int64_t ldy;
 } ggemm_glu_t;
 
-/* Forward.  Rows in no group are not written.  Offsets are read on the device and clamped to [0, rows]: wrong ones give
+/* Forward.  Rows in no group are not written; of rows whose index lies outside [0, x_rows), gate, up and y are zeros, whatever the weights
+ * hold (an Inf, a NaN).  Offsets are read on the device and clamped to [0, rows]: wrong ones give
  * wrong results but no access out of bounds.  y, gate and up must not overlap the inputs.
  * Workspace: 16-byte aligned, contents need not be kept or cleared between calls; calls that may overlap need one each; too
  * small: GGEMM_ERR_WORKSPACE.  Its size goes by sizes and leading dimensions only (pointers may still be NULL), 0 for
@@ -69,7 +70,7 @@ int ggemm_glu(const ggemm_glu_t* p, void* workspace, size_t workspace_bytes, hip
  *   dx[r]  = dgate Wg_e + dup Wu_e         rows x d_model of dtype; with an index the caller adds up a row's copies
  *   dWg_e  = dgate^T x_r + dw_beta dWg_e   of dw_dtype (any of the three), as dWu_e = dup^T x_r
  *   dWd_e  = dy^T h + dw_beta dWd_e        and these too are written for groups without rows
- * Rows whose index lies outside [0, x_rows) count as zeros throughout, dy among them, and get dx = 0.
+ * Rows whose index lies outside [0, x_rows) count as zeros throughout, dy among them, and get dx = 0, whatever the weights hold.
  * dx may be NULL, dw_gate and dw_up together, and dw_down: what is not wanted is not computed.  Results must not overlap the
  * inputs or each other.  With dw_beta == 0 the
  * gradients of the weights are not read.  The workspace also goes by whether index is NULL. */

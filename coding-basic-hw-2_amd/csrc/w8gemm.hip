@@ -131,14 +131,9 @@ void run(const P& p, hipStream_t s) {
 
 }  // namespace
 
-size_t w8_gemm_workspace(const ggemm_w8_gemm_t*) { return 0; }
-
-int w8_gemm(const ggemm_w8_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
+int w8_gemm(const ggemm_w8_gemm_t* p, hipStream_t s) {
   if (!args_ok(p)) return GGEMM_ERR_INVALID;
   if (p->m == 0 || p->n == 0) return GGEMM_OK;
-  const size_t need = w8_gemm_workspace(p);
-  if (ws_bytes < need) return GGEMM_ERR_WORKSPACE;
-  if (need && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
   if (tiles_of(*p, 64, 128) >= (1 << 23)) return GGEMM_ERR_INVALID;
   return launch([&] { with_elem(p->dtype, [&](auto d) {
     constexpr int D = decltype(d)::value;
@@ -150,7 +145,5 @@ int w8_gemm(const ggemm_w8_gemm_t* p, void* ws, size_t ws_bytes, hipStream_t s) 
 
 }  // namespace ggemm
 
-extern "C" size_t ggemm_w8_gemm_workspace(const ggemm_w8_gemm_t* p) { return ggemm::w8_gemm_workspace(p); }
-extern "C" int ggemm_w8_gemm(const ggemm_w8_gemm_t* p, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  return ggemm::w8_gemm(p, workspace, workspace_bytes, stream);
-}
+extern "C" size_t ggemm_w8_gemm_workspace(const ggemm_w8_gemm_t*) { return 0; }
+extern "C" int ggemm_w8_gemm(const ggemm_w8_gemm_t* p, void*, size_t, hipStream_t stream) { return ggemm::w8_gemm(p, stream); }

@@ -75,11 +75,9 @@ typedef struct {
   const int32_t* offsets;        /* groups + 1 ascending values, or NULL for one group of all rows */
   void* c; int64_t ldc;
 } ggemm_w8_gemm_t;
-/* Bytes of workspace (16-byte aligned) that a call with these sizes, leading dimensions and strides needs: often 0, and
- * 0 for invalid ones.  Pointers are not looked at: they may still be NULL. */
+/* Bytes of workspace that a call needs: 0, whatever its sizes, in this version of the library. */
 size_t ggemm_w8_gemm_workspace(const ggemm_w8_gemm_t* p);
-/* Too small a workspace: GGEMM_ERR_WORKSPACE.  Its contents need not be kept or cleared between calls; calls that may
- * overlap need one each. */
+/* workspace and workspace_bytes are not looked at (NULL and 0 will do); they stand for kernels that may come to need some. */
 int ggemm_w8_gemm(const ggemm_w8_gemm_t* p, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus

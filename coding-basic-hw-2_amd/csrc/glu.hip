@@ -498,16 +498,15 @@ bool tiles_fit(const ggemm_glu_t& p, bool weights) {
 
 }  // namespace
 
-size_t glu_workspace(const ggemm_glu_t* p) { return shape_ok(p) ? hidden_bytes(*p) : 0; }
+size_t glu_workspace(const ggemm_glu_t* p) { return shape_ok(p) && tiles_fit(*p, false) ? hidden_bytes(*p) : 0; }
 
 int glu(const ggemm_glu_t* p, void* ws, size_t ws_bytes, hipStream_t s) {
-  if (!args_ok(p) || !p->gate != !p->up) return GGEMM_ERR_INVALID;
+  if (!args_ok(p) || !p->gate != !p->up || !tiles_fit(*p, false)) return GGEMM_ERR_INVALID;
   if (p->rows == 0) return GGEMM_OK;
   if (!p->y || !aligned(p->y, 2) || p->ldy < p->d_model) return GGEMM_ERR_INVALID;
   if (p->gate && (!aligned(p->gate, 2) || !aligned(p->up, 2) || p->ldg < p->d_ff)) return GGEMM_ERR_INVALID;
   if (ws_bytes < glu_workspace(p)) return GGEMM_ERR_WORKSPACE;
   if (!ws || !aligned(ws, 16)) return GGEMM_ERR_INVALID;
-  if (!tiles_fit(*p, false)) return GGEMM_ERR_INVALID;
   return launch([&] { with_type(p->dtype, [&](auto dt) { with_act(p->act, [&](auto act) {
     constexpr int D = decltype(dt)::value;
     using T = typename Elem<D>::T;
@@ -522,11 +521,12 @@ int64_t ld_model(const ggemm_glu_t& p) { return (int64_t)align_up((size_t)p.d_mo
 size_t model_bytes(const ggemm_glu_t& p) { return align_up((size_t)p.rows * ld_model(p) * 2, 256); }
 
 size_t glu_backward_workspace(const ggemm_glu_t* p, const ggemm_glu_grad_t* d) {
-  return shape_ok(p) && d ? 3 * hidden_bytes(*p) + (p->index ? 2 * model_bytes(*p) : 0) : 0;
+  return shape_ok(p) && d && tiles_fit(*p, d->dw_gate || d->dw_down) ? 3 * hidden_bytes(*p) + (p->index ? 2 * model_bytes(*p) : 0) : 0;
 }
 
 int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size_t ws_bytes, hipStream_t s) {
-  if (!args_ok(p) || !d || !elem_known(d->dw_dtype) || !d->dw_gate != !d->dw_up) return GGEMM_ERR_INVALID;
+  if (!args_ok(p) || !d || !elem_known(d->dw_dtype) || !d->dw_gate != !d->dw_up || !tiles_fit(*p, d->dw_gate || d->dw_down))
+    return GGEMM_ERR_INVALID;
   const size_t es = elem_bytes(d->dw_dtype);
   auto grads = [&](const void* w, int64_t ld, int64_t stride, int m, int n) {
     return !w || (aligned(w, es) && ld >= n && (p->groups == 1 || stride >= (m - 1) * ld + n));
@@ -539,7 +539,6 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
     return GGEMM_ERR_INVALID;
   if (ws_bytes < glu_backward_workspace(p, d)) return GGEMM_ERR_WORKSPACE;
   if (p->rows > 0 && (!ws || !aligned(ws, 16))) return GGEMM_ERR_INVALID;
-  if (!tiles_fit(*p, d->dw_gate || d->dw_down)) return GGEMM_ERR_INVALID;
   if (!d->dw_gate && !d->dw_down && (!d->dx || p->rows == 0)) return GGEMM_OK;
   return launch([&] { with_type(p->dtype, [&](auto dt) {
     constexpr int D = decltype(dt)::value;

@@ -60,8 +60,8 @@ typedef struct {
  * hold (an Inf, a NaN).  Offsets are read on the device and clamped to [0, rows]: wrong ones give
  * wrong results but no access out of bounds.  y, gate and up must not overlap the inputs.
  * Workspace: 16-byte aligned, contents need not be kept or cleared between calls; calls that may overlap need one each; too
- * small: GGEMM_ERR_WORKSPACE.  Its size goes by sizes and leading dimensions only (pointers may still be NULL), 0 for
- * invalid ones. */
+ * small: GGEMM_ERR_WORKSPACE.  Its size goes by sizes and the inputs' leading dimensions only (pointers may still be NULL), 0 for
+ * invalid ones and for more tiles than a call takes. */
 size_t ggemm_glu_workspace(const ggemm_glu_t* p);
 int ggemm_glu(const ggemm_glu_t* p, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
@@ -73,7 +73,8 @@ int ggemm_glu(const ggemm_glu_t* p, void* workspace, size_t workspace_bytes, hip
  * Rows whose index lies outside [0, x_rows) count as zeros throughout, dy among them, and get dx = 0, whatever the weights hold.
  * dx may be NULL, dw_gate and dw_up together, and dw_down: what is not wanted is not computed.  Results must not overlap the
  * inputs or each other.  With dw_beta == 0 the
- * gradients of the weights are not read.  The workspace also goes by whether index is NULL. */
+ * gradients of the weights are not read.  The workspace also goes by whether index is NULL, and is 0 for too many tiles of
+ * weights' gradients that are not NULL. */
 typedef struct {
   const void* dy; int64_t lddy;
   void* dx; int64_t lddx;

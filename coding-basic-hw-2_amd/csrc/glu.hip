@@ -580,7 +580,12 @@ int glu_backward(const ggemm_glu_t* p, const ggemm_glu_grad_t* d, void* ws, size
     with_elem(d->dw_dtype, [&](auto wt) {
       const WeightGrad<D, decltype(wt)::value> w{rows, grad, dg, du, h, ldh, from, stream};
       auto tiles = [&](int b) { return (int64_t)matrices * p->groups * ceil_div(p->d_ff, b) * ceil_div(p->d_model, b); };
-      if (tiles(256) >= kCus) run_tiles<Tile256>(w, tiles(256), s);
+      // 256 x 256 where they fill the compute units and cover at most a seventh more than 128 x 128 tiles do, whose loop is slower but
+      // which fit the edges better and store beside another workgroup.  us, 256 and 128: unfilled, 96 tiles over 8192 rows 194 and
+      // 136; filled, 16 groups (2048, 4096) of 2048 rows 1451 and 1912, of 512 rows (1024, 2048) 156 and 167, 384 tiles in a round
+      // and a half 154 and 143; a ninth more, 8 groups (1100, 2304) of 4096 rows 545 and 575, 64 groups (1152, 1024) of 1024 rows 655 and
+      // 604; a sixth more (1152, 2944) 737 and 674, a third more (384, 1024) 397 and 293, 2.7 times (100, 300) 178 and 71.
+      if (tiles(256) >= kCus && 7 * tiles(256) <= 2 * tiles(128)) run_tiles<Tile256>(w, tiles(256), s);
       else run_tiles<Tile128>(w, tiles(128), s);
     });
   }); });

@@ -18,6 +18,15 @@ def test_many_rows_of_few_tiles(offsets, d, f, dw_dtype, beta):
     check_backward(b, gate, u, dw_dtype=dw_dtype, beta=beta)
 
 
+@pytest.mark.parametrize("groups,d,f", [(64, 100, 300), (40, 136, 264), (20, 520, 1032)])
+def test_many_groups_whose_edges_waste_large_tiles(groups, d, f):
+    say("edges", groups, d, f)
+    b = R.Block([9 * g for g in range(groups)] + [9 * groups + 200], 9 * groups + 200, d, f, "bf16", "silu", seed=25)
+    gate, u = kept(b)
+    for dw_dtype, beta in (("bf16", 0.0), ("f32", -1.0)):
+        check_backward(b, gate, u, dw_dtype=dw_dtype, beta=beta)
+
+
 def test_deep_sums_of_picked_rows():
     say("deep, picked")
     rows, d, f = 16384, 136, 72

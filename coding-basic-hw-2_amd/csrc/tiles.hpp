@@ -400,12 +400,6 @@ __device__ __forceinline__ void tile_products(uint8_t* lds, S& src, int nk, type
   }
 }
 
-// Zeros where a row names none.
-template <int E>
-__device__ __forceinline__ void clear_unless(bool live, float (&v)[E], float (&u)[E]) {
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = live ? v[e] : 0.0f, u[e] = live ? u[e] : 0.0f;
-}
 // Blocks to an epilogue: a wave turns one row of blocks at a time through its own part of the ring's second slot (32-bit;
 // the 16-byte piece q of row r lies at q ^ r % (pieces of a row), which spreads both the writes and the reads over the
 // banks), then emit(row, col, v, u, pre) gets E neighbouring columns of a row of the tile.  kPair: blocks alternate between two
@@ -415,11 +409,8 @@ __device__ __forceinline__ void clear_unless(bool live, float (&v)[E], float (&u
 // kWhole: every row and column exists; the rows of a block are unrolled, so that their loads go together.  Else one after another:
 // the checks of every row unrolled make the code of a tile longer than the instruction cache (hidden gradients of 32768 rows,
 // (2048, 4096): 940 us, so 849).
-// kDead: rows for which names(entry(row)) is false come to emit as zeros.  The entries of all of the wave's rows are loaded once, ahead
-// of that wait: a load among the stores would wait for those before it (forward of 4096 tokens, 2 of 16 experts (1024, 2048): without
-// any 157 us, so 159, entries fetched with each row 176).
-template <class C, int E, bool kPair, bool kWhole, bool kDead, class Acc, class Entry, class Names, class Fetch, class Emit>
-__device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][C::FN], Entry entry, Names names, Fetch fetch, Emit emit) {
+template <class C, int E, bool kPair, bool kWhole, class Acc, class Fetch, class Emit>
+__device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][C::FN], Fetch fetch, Emit emit) {
   constexpr int FM = C::FM, FN = C::FN, W = 32 * FN, Q = W / 4;      // columns, 16-byte pieces of an LDS row
   constexpr int LR = (kPair ? W / 2 : W) / E, RI = 64 / LR, N = 32 / RI;   // lanes a row, rows at a time, times
   static_assert(!kPair || FN == 2, "one block of each product");
@@ -427,12 +418,6 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
   const int wm = wave % C::WGM, wn = wave / C::WGM;
   f32x4* const st = reinterpret_cast<f32x4*>(lds + C::STAGE + wave * C::EPI);
   const int c0 = (lane % LR) * E, row0 = wm * FM * 32 + lane / LR, col0 = wn * (kPair ? W / 2 : W) + c0;
-  int mine[FM];         // entry of row lane % 32 of each row of blocks
-  uint32_t live[FM];    // of the rows, one bit each
-  if constexpr (kDead) {
-#pragma unroll
-    for (int i = 0; i < FM; ++i) mine[i] = entry((wm * FM + i) * 32 + (lane & 31));
-  }
   auto turn = [&](int i) {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
@@ -441,16 +426,7 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
         st[(lane & 31) * Q + ((8 * j + 2 * q + (lane >> 5)) ^ (lane & (Q - 1)))] =
             f32x4{(float)acc[i][j][4 * q], (float)acc[i][j][4 * q + 1], (float)acc[i][j][4 * q + 2], (float)acc[i][j][4 * q + 3]};
     __builtin_amdgcn_wave_barrier();
-    if (i == 0) {
-      all_landed();
-      if constexpr (kDead) {
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          asm volatile("" : "+v"(mine[j]));   // not looked at before
-          live[j] = (uint32_t)__ballot(names(mine[j]));
-        }
-      }
-    }
+    if (i == 0) all_landed();
   };
   auto rows = [&](int i, int n, const auto& pre) {
     const int r = lane / LR + n * RI;
@@ -463,7 +439,6 @@ __device__ __forceinline__ void tile_emit(uint8_t* lds, const Acc (&acc)[C::FM][
 #pragma unroll
       for (int z = 0; z < 4; ++z) v[e + z] = x[z], u[e + z] = y[z];
     }
-    if constexpr (kDead) clear_unless(live[i] >> r & 1, v, u);
     emit(row0 + 32 * i + n * RI, col0, v, u, pre);
   };
 #pragma unroll
@@ -489,7 +464,8 @@ struct Nothing {};
 // is on its way while this one's results are stored.
 // P: M (products), kADown, kBDown, kPair, E; groups(), what is looked up once for place(that, t), a tile's Place with g (-1:
 // none), nk (stages) and whole; source(place) with the operands a and b, prepare(kt, wave), ragged(kt) and clear(kt, slot);
-// fetch(place, row, col) and emit(place, row, col, v, u, what fetch gave); kDead, with it entry(place, row) and names(entry).
+// fetch(place, row, col) and emit(place, row, col, v, u, what fetch gave); kDead: sums of rows for which names(entry(place, row)) is false
+// come to emit as zeros.
 template <class C, class P>
 __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
   __shared__ __attribute__((aligned(128))) uint8_t tile_lds[C::SMEM];
@@ -511,22 +487,35 @@ __global__ void __launch_bounds__(C::NT, C::WAVES) tile_kernel(P p, int total) {
     lds_done();
     typename P::M::Acc acc[C::FM][C::FN] = {};
     if (cur.nk > 0) tile_products<C, typename P::M, P::kADown, P::kBDown>(tile_lds, src, cur.nk, acc);
+    // Of row lane % 32 of each of the wave's rows of blocks, the one whose sums the lane has.  Looked at ahead of the epilogue, where a load
+    // would wait for the stores before it (forward of 4096 tokens, 2 of 16 experts (1024, 2048): 176 us with a look at each row as it
+    // is stored, 157 so and without any).
+    int entry[C::FM];
+    if constexpr (P::kDead) {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) entry[i] = p.entry(cur, (wave % C::WGM * C::FM + i) * 32 + (lane & 31));
+    }
     const auto nxt = next();
     if (nxt.g >= 0) {
       src = p.template source<C>(nxt, wave, lane);
       if (nxt.nk > 0) send_stage<C>(src, 0, ring, wave);
     }
+    if constexpr (P::kDead) {
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        const bool live = p.names(entry[i]);
+        if (!__all(live)) {
+#pragma unroll
+          for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = live ? acc[i][j][e] : 0;
+        }
+      }
+    }
     auto store = [&](auto whole) {
       constexpr bool kWhole = decltype(whole)::value;
-      tile_emit<C, P::E, P::kPair, kWhole, P::kDead>(
-          tile_lds, acc,
-          [&](int row) {
-            if constexpr (P::kDead) return p.entry(cur, row);
-          },
-          [&](int entry) {
-            if constexpr (P::kDead) return p.names(entry);
-          },
-          [&](int row, int col) { return p.template fetch<kWhole>(cur, row, col); },
+      tile_emit<C, P::E, P::kPair, kWhole>(
+          tile_lds, acc, [&](int row, int col) { return p.template fetch<kWhole>(cur, row, col); },
           [&](int row, int col, const float (&v)[P::E], const float (&u)[P::E], const auto& pre) {
             p.template emit<kWhole>(cur, row, col, v, u, pre);
           });
@@ -650,7 +639,11 @@ __global__ void __launch_bounds__(256, 4) few_kernel(P p) {
   }
   float v[4] = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
   float u[4] = {(float)t[0], (float)t[1], (float)t[2], (float)t[3]};
-  if constexpr (P::kDead) clear_unless(p.names(mine), v, u);
+  if constexpr (P::kDead) {
+    const bool live = p.names(mine);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = live ? v[e] : 0.0f, u[e] = live ? u[e] : 0.0f;
+  }
   p.template emit<false>(c, lane & 15, (P::kPair ? 0 : 16 * wave) + 4 * quarter, v, u, Nothing{});
 }
 

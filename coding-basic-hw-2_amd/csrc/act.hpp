@@ -26,7 +26,8 @@ __device__ __forceinline__ float logistic(float z) {
 //   GELU       p = Phi(v), the normal distribution's, p' = its density.  By Abramowitz and Stegun 7.1.26: with
 //              x = |v| / sqrt 2, t = 1 / (1 + 0.3275911 x): erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), off by at most
 //              1.5e-7; p = 1 - erfc / 2 or erfc / 2 by v's sign.  Nine multiply-adds and the density's exponential, where
-//              a library error function takes several times that in the epilogue of every tile.
+//              a library error function takes several times that in the epilogue of every tile.  v p is off by 4.2e-7 at most
+//              (at 3.06; of itself, 3e-6 above -2, 5e-5 above -3, 2e-3 above -5, 1e-2 above -8).
 //   GELU_TANH  p = logistic(2 z), z = sqrt(2 / pi) (v + 0.044715 v^3), p' = p (1 - p) 2 z'.  Past |v| = 16, p is 0 or 1 to the
 //              last bit; the clamp keeps v^3 and z' finite, so that no 0 Inf arises.
 template <int ACT>

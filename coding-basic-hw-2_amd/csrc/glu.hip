@@ -3,8 +3,11 @@
 // Five products by the tiles of tiles.hpp, each with the work that belongs to its result in the epilogue: two launches
 // forward (gate, up, activation and product; down), three backward (hidden gradients; dx; the weights' gradients), one more
 // for the copies of gathered rows.  What is kept between launches is 16-bit: h, dgate and dup are matrix operands.
-// Bound: the matrix cores at the clock that their power leaves, 1.0 to 1.28 PFLOP/s on products with long inner dimensions;
-// short ones by a tile's first loads and its stores.
+// Bound: long inner dimensions, the loop's idle cycles: matrix cores busy 66 % of them forward and 55 to 60 % where an operand lies down the
+// inner dimension, at 1.55 to 1.95 GHz in the same launches, 1.1 to 1.26 and 1.0 to 1.1 PFLOP/s; short ones, a tile's first loads and
+// its stores.
+// Registers: the 256 x 256 tiles take all 256; hidden keeps one to three values of the epilogue's in scratch memory over the stages, the
+// kernels over rows 23 to 66 scalars in lanes, both outside the loop of the stages.
 #include <algorithm>
 #include <type_traits>
 
@@ -50,7 +53,7 @@ __device__ __forceinline__ int row_entry(const ggemm_glu_t& p, const Place& c, i
 __device__ __forceinline__ bool names_row(const ggemm_glu_t& p, int entry) { return !p.index || (uint32_t)entry < (uint32_t)p.x_rows; }
 
 // h = act(x Wg^T) (x Wu^T), and gate and up where they are kept.  Both products in one tile: half the columns, twice the
-// weights, x read once (8192 x 4096 x 8192: 1000 us, 1.1 PFLOP/s; 4096 tokens, 2 of 16 experts (1024, 2048), all kept: 111 us, of
+// weights, x read once (8192 x 4096 x 8192: 880 to 1000 us, 1.1 to 1.25 PFLOP/s; 4096 tokens, 2 of 16 experts (1024, 2048), all kept: 107 us, of
 // which 18 are the stores).
 template <int D, int ACT>
 struct Up {
@@ -134,7 +137,7 @@ struct Up {
   }
 };
 
-// y = h Wd^T (8192 x 8192 x 4096: 490 us, 1.1 PFLOP/s)
+// y = h Wd^T (8192 x 8192 x 4096: 430 to 500 us, 1.1 to 1.27 PFLOP/s)
 template <int D>
 struct DownProduct {
   using T = typename Elem<D>::T;
@@ -202,8 +205,8 @@ struct DownProduct {
 };
 
 // dh = dy Wd, and from it, gate and up: dgate = dh up act'(gate), dup = dh act(gate), h = act(gate) up.  dh stays in registers.  Bound:
-// five matrices pass through the epilogue, under which nothing else is multiplied (32768 rows, (2048, 4096): 830 us,
-// 0.66 PFLOP/s; 632 without reading gate and up, 540 would be the product's).
+// five matrices pass through the epilogue, under which nothing else is multiplied (32768 rows, (2048, 4096): 760 to 830 us,
+// 0.66 to 0.72 PFLOP/s; 632 without reading gate and up, 540 would be the product's).
 template <int D, int ACT>
 struct Hidden {
   using T = typename Elem<D>::T;

@@ -145,7 +145,7 @@ struct TileShape {
   static constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;
   static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;   // 1 KB pieces of A and B a wave brings
   static constexpr int EPI = 32 * 32 * FN * 4;               // epilogue bytes per wave, from the second slot on
-  static constexpr int SMEM = STAGE + (NW * EPI > STAGE ? NW * EPI : STAGE);
+  static constexpr int SMEM = STAGE + (NW * EPI > STAGE ? NW * EPI : STAGE);   // 64 x 128: 56 KB, of which 32 the epilogue's
   static constexpr int PER_CU = 163840 / SMEM;               // workgroups, as many as LDS holds
   static constexpr int WAVES = PER_CU * NW / 4;              // per SIMD
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && NW % 2 == 0, "pieces");
@@ -661,6 +661,10 @@ void run_tiles(const P& p, int64_t tiles, hipStream_t s) {
 // 4096, us: 64 x 128 tiles (two a compute unit) 26, 24; 128 x 128 (two) 40, 29; 256 x 256 (one) 64, 52; the same
 // ratios at k = 2048 and 1024.  So the tile with the least rounds times cost is taken; at 2048 rows 52, 42, 54 us, at 3001 78,
 // 65, 59, at 4096 101, 79, 67.
+// 16-bit products by the same costs: of 48 (twelve blocks from 300 to 65536 rows, forward with gate and up kept, and backward) in all
+// three shapes, the one taken is the fastest or within 2 % of it in 42.  The others, 5 to 20 % slower, store three matrices after a short
+// inner dimension, which two workgroups on a compute unit do in turns: gate and up of 4096 tokens, 2 of 16 experts
+// (1024, 2048), 106 us by 256 x 256, 91 by 128 x 128; hidden gradients of 32768 rows, 8 groups (1024, 1024), 172 and 147.
 // Few rows: up to two workgroups a compute unit (n = k = 4096: 64 rows 15.1, by tiles 15.9; 128 rows 25 and 22), up to four
 // if groups have 16 rows at most on average, so that nobody else reads their weights (32 groups, 1024 x 1024: 7.6 and 8.7; 8
 // experts' 16-bit weights of 4096 x 2048 twice, 8 workgroups a compute unit: 57 and 52).

@@ -3,9 +3,9 @@
 // Tiles and the kernel for few rows of tiles.hpp on v_mfma_i32_32x32x32_i8 (16x16x64): sums are exact, k < 2^17 keeps them
 // below 2^31.  A row's and a column's scale, the activation and the pair's product come in the epilogue, in 32-bit floating
 // point; the sum is rounded to it first (at most 2^-24 of it).
-// Bound: large products, the matrix cores at the clock that their power leaves (8192^3: 441 to 466 us, 2.4 to 2.5 POP/s); decoding,
-// the bytes of the weights (64 experts of 4096 x 2048 twice, 8 rows each: 180 us, 5.8 TB/s).
-
+// Bound: large products, the loop's idle cycles, a third (matrix cores busy 65 % of 0.80 million), and the clock, which ranges from 1.43
+// to 1.77 GHz over launches one after another (8192^3: 434 to 557 us, 2.0 to 2.5 POP/s); decoding, the bytes of the weights (64
+// experts of 4096 x 2048 twice, 8 rows each: 180 us, 5.8 TB/s).
 #include <algorithm>
 #include <type_traits>
 

@@ -1,8 +1,8 @@
 // w8quant.hip -- rows to 8-bit integers with a scale each, and back (include/ggemm_w8.h).
 //
 // One pass: a row is held in registers while its largest magnitude is found, the next row's values on their way and the
-// index entry of the row after (without: 32768 gathered rows of 4096 bf16 86 us, with 62).
-// Bound: HBM; 6.4 TB/s with every gathered row counted, 16384 rows read twice each.
+// index entry of the row after (without: 32768 gathered rows of 4096 bf16 86 us, with 62; 70 on two other cards).
+// Bound: HBM; 5.8 to 6.4 TB/s with every gathered row counted, 16384 rows read twice each.
 #include <algorithm>
 
 #include "ggemm_w8.h"

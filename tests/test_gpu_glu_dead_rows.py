@@ -1,8 +1,11 @@
 """Rows of the gated block (include/ggemm_glu.h) whose index names none, with weights that are not finite: zeros all the same, in every
-kernel that computes them."""
+kernel that computes them, also from a captured graph."""
+import ctypes as C
+
 import pytest
 import torch
 
+import ggemm as G
 import glu_ref as R
 from gpu_util import say
 
@@ -58,3 +61,51 @@ def test_no_live_row_at_all():
         got = b.backward(gate, u)
         for n, t in (("gate", gate), ("up", u), ("y", y), *got.items()):
             assert bool((t[:rows] == 0).all() if n in ("gate", "up", "y", "dx") else (t == 0).all()), n
+
+
+def test_captured_with_an_index_that_changes():
+    """Forward and backward in one graph; index, offsets and inputs are other ones at every replay, eager calls in between."""
+    say("graph")
+    rows, d, f = 700, 136, 264
+    b = block(rows, [200, 450, rows], d, f, "bf16", "silu", 0.3)
+    y, gate, u, dx = b.out(rows, d), b.out(rows, f), b.out(rows, f), b.out(rows, d)
+    dwg, dwu, dwd = b.out(3 * f, d, "f32"), b.out(3 * f, d, "f32"), b.out(3 * d, f, "f32")
+    out = (y, gate, u, dx, dwg, dwu, dwd)
+    p, q = b.struct(gate, u, y), R.grad_struct(b, dx, dwg, dwu, dwd)
+    n1, n2 = G.lib().ggemm_glu_workspace(C.byref(p)), G.lib().ggemm_glu_backward_workspace(C.byref(p), C.byref(q))
+    ws = torch.empty(max(n1, n2), dtype=torch.uint8, device="cuda")
+
+    def step():
+        s = torch.cuda.current_stream().cuda_stream
+        G.check(G.lib().ggemm_glu(C.byref(p), ws.data_ptr(), n1, s), "ggemm_glu")
+        G.check(G.lib().ggemm_glu_backward(C.byref(p), C.byref(q), ws.data_ptr(), n2, s), "ggemm_glu_backward")
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    gen = torch.Generator()
+    for i in range(5):
+        gen.manual_seed(i)
+        b.index.copy_(torch.randint(-rows // 4, rows + 20, (rows,), generator=gen).int())
+        b.offs.copy_(torch.tensor([0, *sorted(torch.randint(0, rows + 1, (2,), generator=gen).tolist()), rows]).int())
+        b.x[:, :d] = torch.randn(rows, d, device="cuda", generator=b.gen).to(b.x.dtype)
+        for t in out:
+            t.fill_(3.0)
+        ws.fill_(255)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for t in out:
+            t.fill_(3.0)
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, t) for g, t in zip(got, out)), i
+        dead = ~b.live()
+        assert bool(dead.any()) and all(bool((t[:rows][dead] == 0).all()) for t in (y, gate, u, dx))
+        b.offsets = b.offs.tolist()
+        want = b.forward64()
+        for n, t in (("gate", gate), ("up", u), ("y", y)):
+            assert R.worst(t, *want[n]) <= 1.0, (i, n)
+        for n, (v, e) in b.backward64(gate.double(), u.double()).items():
+            assert R.worst({"dx": dx, "dwg": dwg, "dwu": dwu, "dwd": dwd}[n].reshape(v.shape), v, e) <= 1.0, (i, n)

@@ -1,5 +1,5 @@
 """The transfers to LDS of the tiled products read scalar registers in inline assembly: compile their sources for gfx950 and check
-that no such register was written by a vector instruction fewer than five wait states before (CPU only).  The checker itself is
+that no such register was written by a vector instruction fewer than five wait states before (CPU only).  The check itself is
 tested on hand-written fragments."""
 import subprocess
 from pathlib import Path
@@ -13,7 +13,7 @@ CSRC = REPO / "coding-basic-hw-2_amd" / "csrc"
 SOURCES = ("mx4gemm.hip", "w8gemm.hip", "glu.hip")
 
 
-def test_checker_counts_wait_states():
+def test_check_counts_wait_states():
     def asm(n, between=()):
         return ["\tv_readlane_b32 s1, v96, 3", *between, "\ts_mov_b32 m0, s7", f"\ts_nop {n}", "\tglobal_load_lds_dwordx4 v4, s[0:1]",
                 "\ts_endpgm"]
@@ -25,7 +25,7 @@ def test_checker_counts_wait_states():
     assert not S.check_kernel(["\tv_cmp_eq_u32_e64 s[4:5], v0, v1", "\tbuffer_load_dwordx4 v1, s[0:3], 0 offen lds", "\ts_endpgm"])
 
 
-def test_checker_takes_the_shortest_way():
+def test_check_takes_the_shortest_way():
     asm = ["\tv_readfirstlane_b32 s0, v1", "\ts_cbranch_scc1 .LBB0_2", "\ts_nop 4", ".LBB0_2:", "\ts_nop 2",
            "\tbuffer_load_dwordx4 v1, s[0:3], 0 offen lds", "\ts_endpgm"]
     assert [r for _, _, r in S.check_kernel(asm)] == [(0,)]
